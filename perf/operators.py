@@ -255,7 +255,7 @@ def run(s: dict):
     s["refs"].copy_(s["refs0"])
     if own:
         from harsh4b_amd.paged import pages_compact
-        pages_compact(*pools, s["table"], s["refs"], s["status"], live=s["live"])
+        pages_compact(*pools, s["table"], s["refs"], live=s["live"])
     else:
         _plain_compact(s)
     return (*pools, s["table"], s["refs"], s["live"])
