@@ -48,6 +48,17 @@ class HqState(ctypes.Structure):
     ]
 
 
+class HqPages(ctypes.Structure):
+    _fields_ = [
+        ("layers", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("sequences", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("keys", vp), ("values", vp), ("table", vp), ("lengths", vp), ("refs", vp), ("status", vp),
+    ]
+
+
+HQ_PAGES_FULL = 1
+HQ_PAGES_BAD = 2
 HQ_STEP_BAD_TOKEN = 1
 HQ_STEP_FULL = 2
 HQ_STEP_SYNC = 4
@@ -70,6 +81,14 @@ _SIGNATURES = {
     "hq_gemm_workspace_bytes": ([c_int, c_int, c_int], c_size),
     "hq_int4_i8_gemm": ([vp, vp, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp], c_int),
     "hq_quant_int4_gemm": ([vp, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp, vp, vp], c_int),
+    "hq_pages_workspace_bytes": ([ctypes.POINTER(HqPages)], c_size),
+    "hq_pages_resize": ([ctypes.POINTER(HqPages), vp, c_int, c_int, vp, vp], c_int),
+    "hq_pages_fork": ([ctypes.POINTER(HqPages), vp, vp, vp], c_int),
+    "hq_pages_compact": ([ctypes.POINTER(HqPages), vp, vp, vp], c_int),
+    "hq_paged_append": ([ctypes.POINTER(HqPages), vp, vp, c_int, c_int, vp, vp, c_float, vp, vp, c_int, vp, vp],
+                        c_int),
+    "hq_paged_attention_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int], c_size),
+    "hq_paged_attention": ([ctypes.POINTER(HqPages), vp, vp, c_int, c_int, c_int, c_int, vp, vp, vp], c_int),
     "hq_step_layer_blocks": ([ctypes.POINTER(HqModel)], c_int),
     "hq_step_workspace_bytes": ([ctypes.POINTER(HqModel), c_int], c_size),
     "hq_decode_step": ([ctypes.POINTER(HqModel), ctypes.POINTER(HqState), vp], c_int),

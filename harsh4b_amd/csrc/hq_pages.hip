@@ -1,0 +1,458 @@
+// hq_pages.hip - management of the paged K/V cache on gfx950: growth and
+// release of sequences (hq_pages_resize), forks (hq_pages_fork) and
+// compaction (hq_pages_compact).  No reference counterpart.
+//
+// All of it runs on the device, so that a captured step can cross a page
+// border without the host.  A page is free while no table entry holds it
+// (refs = 0) and allocation takes the lowest free pages, so every call's
+// outcome is a function of the tables alone, whatever order its atomics run
+// in.  Each call is two launches:
+//   plan    one block (resize, compact): counts, prefix sums, the list of free
+//           pages; decides whether the call can be done at all
+//   apply   many blocks: table rows, reference counts and the page copies
+// A copy's source may be released by the same call and its target was free
+// before it, so copies and releases need no order between them.
+#include <algorithm>
+
+#include "hq_device.h"
+#include "hq_internal.h"
+
+namespace hq {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int kPlanStep = 16;          // pages a lane looks at per round of the free-page search
+
+struct PagesParams {
+    hq_pages c;
+    int32_t shift;                     // log2(page_size)
+    const int32_t* want;               // resize: new lengths; fork: parents
+    int window, sinks;                 // resize
+    int32_t* live;                     // compact (nullable)
+    int32_t* head;                     // workspace: [0] go, [1] copies, [2] pages in use
+    int32_t* a;                        // resize: first new page's rank per row; compact: sources
+    int32_t* b;                        // resize: copy flags per row; compact: targets
+    int32_t* free_list;                // resize
+    int32_t* owner;                    // resize: per page, the first row growing in it
+    int32_t* count;                    // resize: per page, the rows growing in it; compact: new place
+    int32_t* items;                    // resize: per copy the source, the target's rank, the positions filled
+    int32_t* snapshot;                 // fork: the table, then the lengths
+};
+
+// Block-wide exclusive prefix sum over 1024 threads; total in *total.
+__device__ __forceinline__ int plan_scan(int v, int* wave_sum, int* total)
+{
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int y = __shfl_up(incl, o, kWave);
+        if (lane >= o) incl += y;
+    }
+    __syncthreads();                   // wave_sum's last readers
+    if (lane == kWave - 1) wave_sum[wave] = incl;
+    __syncthreads();
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        before += w < wave ? wave_sum[w] : 0;
+        sum += wave_sum[w];
+    }
+    *total = sum;
+    return before + incl - v;
+}
+
+// What hq_pages_resize does to one row.
+struct ResizeRow {
+    int old_len, new_len;
+    int old_entries, new_entries;      // table entries the two lengths need
+    int source;                        // page the growth goes on writing to, or -1
+    bool hole;                         // that page is missing
+    bool bad;
+};
+
+__device__ __forceinline__ ResizeRow resize_row(const PagesParams& p, int r)
+{
+    ResizeRow d;
+    const int ps = p.c.page_size;
+    d.old_len = p.c.lengths[r];
+    const int want = p.want[r];
+    d.new_len = want < 0 ? d.old_len : want;
+    d.bad = d.old_len < 0 || int64_t(d.old_len) > int64_t(p.c.max_pages) * ps;
+    d.old_entries = int((int64_t(d.old_len) + ps - 1) >> p.shift);
+    d.new_entries = int((int64_t(d.new_len) + ps - 1) >> p.shift);
+    d.source = -1;
+    d.hole = false;
+    if (!d.bad && d.new_len > d.old_len && (d.old_len & (ps - 1))) {
+        const int e = d.old_len >> p.shift;
+        const int page = p.c.table[size_t(r) * p.c.max_pages + e];
+        if (page >= 0 && page < p.c.pages) d.source = page;
+        else d.hole = true;
+    }
+    return d;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PagesParams p)
+{
+    __shared__ int wave_sum[kPlanWaves];
+    __shared__ int refuse, copies;
+    const int t = threadIdx.x;
+    const int rows = p.c.sequences;
+    if (t == 0) refuse = copies = 0;
+    __syncthreads();
+    for (int r = t; r < rows; r += kPlanThreads) {
+        const ResizeRow d = resize_row(p, r);
+        if (d.bad) atomicOr(&refuse, HQ_PAGES_BAD);
+        else if (d.new_entries > p.c.max_pages) atomicOr(&refuse, HQ_PAGES_FULL);
+        if (d.source >= 0) {
+            publish_i(p.count + d.source, 0);
+            publish_i(p.owner + d.source, 0x7fffffff);
+        }
+    }
+    wait_all_memory();
+    __syncthreads();
+    if (refuse) {
+        if (t == 0) {
+            atomicOr(p.c.status, refuse);
+            p.head[0] = 0;
+        }
+        return;
+    }
+    for (int r = t; r < rows; r += kPlanThreads) {
+        const ResizeRow d = resize_row(p, r);
+        if (d.source >= 0) {
+            atomicAdd(p.count + d.source, 1);
+            atomicMin(p.owner + d.source, r);
+        }
+    }
+    wait_all_memory();
+    __syncthreads();
+    // new pages of each row, in the order of the table's entries
+    int need = 0;
+    for (int base = 0; base < rows; base += kPlanThreads) {
+        const int r = base + t;
+        int mine = 0;
+        bool copied = false;
+        ResizeRow d{};
+        if (r < rows) {
+            d = resize_row(p, r);
+            if (d.source >= 0) {
+                const int held = p.c.refs[d.source];
+                copied = held > 1 && !(read_i(p.owner + d.source) == r && read_i(p.count + d.source) == held);
+            }
+            mine = max(0, d.new_entries - d.old_entries) + (d.hole || copied ? 1 : 0);
+            p.b[r] = copied;
+        }
+        int total;
+        const int rank = plan_scan(mine, wave_sum, &total);
+        if (r < rows) p.a[r] = need + rank;
+        if (copied) {
+            int32_t* item = p.items + 3 * atomicAdd(&copies, 1);
+            item[0] = d.source;
+            item[1] = need + rank;
+            item[2] = d.old_len & (p.c.page_size - 1);
+        }
+        // (rows x entries fits the table; past the pool the call is refused)
+        need = need > p.c.pages ? need : need + total;
+    }
+    // the first `need` free pages: a wave looks at 1024 pages a round
+    const int lane = t & (kWave - 1), wave = t / kWave;
+    int found = 0;
+    for (int64_t base = 0; base < p.c.pages && found < need; base += int64_t(kPlanThreads) * kPlanStep) {
+        const int64_t at = base + int64_t(wave) * kWave * kPlanStep + lane;
+        uint64_t is_free[kPlanStep];
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) {
+            const int64_t page = at + k * kWave;
+            is_free[k] = __ballot(page < p.c.pages && p.c.refs[page < p.c.pages ? page : 0] == 0);
+            n += __popcll(is_free[k]);
+        }
+        int total;
+        int rank = found + plan_scan(lane == 0 ? n : 0, wave_sum, &total);
+        rank = __builtin_amdgcn_readfirstlane(rank);
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) {
+            const int mine = rank + __popcll(is_free[k] & ((uint64_t(1) << lane) - 1));
+            if (((is_free[k] >> lane) & 1) && mine < need) p.free_list[mine] = int(at + k * kWave);
+            rank += __popcll(is_free[k]);
+        }
+        found += total;
+    }
+    if (t == 0) {
+        const bool go = found >= need;
+        if (!go) atomicOr(p.c.status, HQ_PAGES_FULL);
+        p.head[0] = go;
+        p.head[1] = copies;
+    }
+}
+
+// Copy the first `fill` positions of page `src` to page `dst`, one kv head of
+// K or V of one layer a wave: segment s of layers * 2 * kv_heads.
+__device__ __forceinline__ void copy_segment(const hq_pages& c, int src, int dst, int fill, int s)
+{
+    const int h = s % c.kv_heads;
+    const int lw = s / c.kv_heads;
+    uint16_t* pool = (lw & 1) ? c.values : c.keys;
+    const size_t layer = size_t(lw >> 1) * c.pages;
+    const size_t head = size_t(c.page_size) * c.head_dim;
+    const uint4* from = reinterpret_cast<const uint4*>(pool + ((layer + src) * c.kv_heads + h) * head);
+    uint4* to = reinterpret_cast<uint4*>(pool + ((layer + dst) * c.kv_heads + h) * head);
+    const int n = fill * c.head_dim / 8;             // 16-byte pieces (head_dim is a multiple of 16)
+    const int lane = threadIdx.x & (kWave - 1);
+    for (int i = lane; i < n; i += kWave) to[i] = from[i];
+}
+
+__global__ __launch_bounds__(kBlock) void resize_apply_kernel(PagesParams p)
+{
+    if (p.head[0] == 0) return;
+    const hq_pages& c = p.c;
+    for (int r = blockIdx.x; r < c.sequences; r += gridDim.x) {
+        const ResizeRow d = resize_row(p, r);
+        const int rank = p.a[r];
+        const bool fresh_source = d.hole || p.b[r] != 0;
+        const int e0 = d.old_len >> p.shift;             // the partly filled page's entry
+        // positions no query from here on sees: [sinks, low)
+        const int64_t low = p.window > 0 ? int64_t(min(d.old_len, d.new_len)) - p.window + 1 : 0;
+        __syncthreads();                                 // every thread has read the row
+        for (int e = threadIdx.x; e < c.max_pages; e += kBlock) {
+            int32_t* entry = c.table + size_t(r) * c.max_pages + e;
+            const int page = *entry;
+            const bool held = page >= 0 && page < c.pages;
+            const bool replaced = fresh_source && e == e0;
+            const bool added = e >= d.old_entries && e < d.new_entries;
+            int now = page;
+            if (replaced) now = p.free_list[rank];
+            else if (added) now = p.free_list[rank + (fresh_source ? 1 : 0) + e - d.old_entries];
+            else if (e >= d.new_entries) now = -1;
+            else if ((int64_t(e) + 1) << p.shift <= low && int64_t(e) << p.shift >= p.sinks) now = -1;
+            if (now != page) {
+                if (held) atomicSub(c.refs + page, 1);
+                if (replaced || added) atomicAdd(c.refs + now, 1);
+                *entry = now;
+            }
+        }
+        if (threadIdx.x == 0) c.lengths[r] = d.new_len;
+    }
+    // page copies, spread over all the launch's waves
+    const int waves = gridDim.x * (kBlock / kWave);
+    const int segments = c.layers * 2 * c.kv_heads;
+    const int64_t all = int64_t(p.head[1]) * segments;
+    for (int64_t s = int64_t(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave; s < all; s += waves) {
+        const int32_t* item = p.items + 3 * (s / segments);
+        copy_segment(c, item[0], p.free_list[item[1]], item[2], int(s % segments));
+    }
+}
+
+// ------------------------------------------------------------------ forks
+__device__ __forceinline__ bool parents_ok(const PagesParams& p)
+{
+    // every block looks at all of them: all or nothing
+    int bad = 0;
+    for (int r = threadIdx.x; r < p.c.sequences; r += kBlock) bad |= p.want[r] >= p.c.sequences;
+    return !__syncthreads_or(bad);
+}
+
+__global__ __launch_bounds__(kBlock) void fork_snapshot_kernel(PagesParams p)
+{
+    const int r = blockIdx.x;
+    const size_t row = size_t(r) * p.c.max_pages;
+    for (int e = threadIdx.x; e < p.c.max_pages; e += kBlock) p.snapshot[row + e] = p.c.table[row + e];
+    if (threadIdx.x == 0) p.snapshot[size_t(p.c.sequences) * p.c.max_pages + r] = p.c.lengths[r];
+}
+
+__global__ __launch_bounds__(kBlock) void fork_rows_kernel(PagesParams p)
+{
+    const hq_pages& c = p.c;
+    const int r = blockIdx.x;
+    if (!parents_ok(p)) {
+        if (r == 0 && threadIdx.x == 0) atomicOr(c.status, HQ_PAGES_BAD);
+        return;
+    }
+    const int parent = p.want[r];
+    if (parent < 0 || parent == r) return;
+    const size_t row = size_t(r) * c.max_pages, from = size_t(parent) * c.max_pages;
+    for (int e = threadIdx.x; e < c.max_pages; e += kBlock) {
+        const int was = p.snapshot[row + e], now = p.snapshot[from + e];
+        if (was == now) continue;
+        if (was >= 0 && was < c.pages) atomicSub(c.refs + was, 1);
+        if (now >= 0 && now < c.pages) atomicAdd(c.refs + now, 1);
+        c.table[row + e] = now;
+    }
+    if (threadIdx.x == 0) c.lengths[r] = p.snapshot[size_t(c.sequences) * c.max_pages + parent];
+}
+
+// ------------------------------------------------------------- compaction
+__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagesParams p)
+{
+    __shared__ int wave_sum[kPlanWaves];
+    const int t = threadIdx.x;
+    const int lane = t & (kWave - 1), wave = t / kWave;
+    const int64_t pages = p.c.pages;
+    int n = 0;
+    for (int64_t page = t; page < pages; page += kPlanThreads) n += p.c.refs[page] > 0;
+    int live;
+    plan_scan(n, wave_sum, &live);
+    int sources = 0, targets = 0;
+    for (int64_t base = 0; base < pages; base += int64_t(kPlanThreads) * kPlanStep) {
+        const int64_t at = base + int64_t(wave) * kWave * kPlanStep + lane;
+        uint64_t moves[kPlanStep];         // at and above `live`: pages in use; below: free ones
+        int above = 0, below = 0;
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) {
+            const int64_t page = at + k * kWave;
+            const bool used = page < pages && p.c.refs[page < pages ? page : 0] > 0;
+            moves[k] = __ballot(page < pages && used == (page >= live));
+            const uint64_t high = __ballot(page >= live);
+            above += __popcll(moves[k] & high);
+            below += __popcll(moves[k] & ~high);
+            if (page < pages && page >= live) p.count[page] = int(page);   // (overwritten below where it moves)
+        }
+        int total_above, total_below;
+        int rank_above = sources + plan_scan(lane == 0 ? above : 0, wave_sum, &total_above);
+        int rank_below = targets + plan_scan(lane == 0 ? below : 0, wave_sum, &total_below);
+        rank_above = __builtin_amdgcn_readfirstlane(rank_above);
+        rank_below = __builtin_amdgcn_readfirstlane(rank_below);
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) {
+            const int64_t page = at + k * kWave;
+            const uint64_t high = __ballot(page >= live);
+            const uint64_t up = moves[k] & high, down = moves[k] & ~high;
+            const uint64_t under = (uint64_t(1) << lane) - 1;
+            if ((up >> lane) & 1) p.a[rank_above + __popcll(up & under)] = int(page);
+            if ((down >> lane) & 1) p.b[rank_below + __popcll(down & under)] = int(page);
+            rank_above += __popcll(up);
+            rank_below += __popcll(down);
+        }
+        sources += total_above;
+        targets += total_below;
+    }
+    wait_all_memory();
+    __syncthreads();
+    for (int i = t; i < sources; i += kPlanThreads) p.count[p.a[i]] = p.b[i];
+    if (t == 0) {
+        p.head[1] = sources;
+        p.head[2] = live;
+        if (p.live) *p.live = live;
+    }
+}
+
+__global__ __launch_bounds__(kBlock) void compact_apply_kernel(PagesParams p)
+{
+    const hq_pages& c = p.c;
+    const int moves = p.head[1], live = p.head[2];
+    if (moves == 0) return;
+    const int64_t threads = int64_t(gridDim.x) * kBlock;
+    const int64_t first = int64_t(blockIdx.x) * kBlock + threadIdx.x;
+    for (int64_t i = first; i < int64_t(c.sequences) * c.max_pages; i += threads) {
+        const int page = c.table[i];
+        if (page >= live && page < c.pages) c.table[i] = p.count[page];
+    }
+    for (int64_t i = first; i < moves; i += threads) {
+        c.refs[p.b[i]] = c.refs[p.a[i]];
+        c.refs[p.a[i]] = 0;
+    }
+    const int waves = gridDim.x * (kBlock / kWave);
+    const int segments = c.layers * 2 * c.kv_heads;
+    for (int64_t s = first / kWave; s < int64_t(moves) * segments; s += waves) {
+        const int i = int(s / segments);
+        copy_segment(c, p.a[i], p.b[i], c.page_size, int(s % segments));
+    }
+}
+
+// ------------------------------------------------------------------- host
+static size_t al256g(size_t v) { return (v + 255) & ~size_t(255); }
+
+static bool pages_shape_ok(const hq_pages* c)
+{
+    if (!c || c->layers < 1 || c->pages < 1 || c->kv_heads < 1 || c->sequences < 1 || c->max_pages < 1) return false;
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return false;
+    if (c->head_dim != 16 && c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return false;
+    // a length is an int, and so is a table's size
+    return int64_t(c->max_pages) * c->page_size <= 0x7fffffff && int64_t(c->sequences) * c->max_pages <= 0x7fffffff;
+}
+
+static PagesParams pages_params(const hq_pages* c, void* workspace)
+{
+    PagesParams p{};
+    p.c = *c;
+    p.shift = __builtin_ctz(unsigned(c->page_size));
+    char* at = static_cast<char*>(workspace);
+    auto take = [&](size_t ints) {
+        int32_t* here = reinterpret_cast<int32_t*>(at);
+        at += al256g(ints * 4);
+        return here;
+    };
+    const size_t wide = std::max(c->sequences, c->pages);
+    p.head = take(64);
+    p.a = take(wide);
+    p.b = take(wide);
+    p.count = take(c->pages);
+    p.owner = take(c->pages);
+    p.free_list = take(c->pages);
+    p.items = take(size_t(3) * c->sequences);
+    p.snapshot = take(size_t(c->sequences) * c->max_pages + c->sequences);
+    return p;
+}
+
+// blocks of 256 threads that keep the memory busy (8 a CU)
+constexpr int kCopyBlocks = 2048;
+
+}  // namespace hq
+
+using namespace hq;
+
+extern "C" size_t hq_pages_workspace_bytes(const hq_pages* cache)
+{
+    if (!pages_shape_ok(cache)) return 0;
+    const PagesParams p = pages_params(cache, nullptr);
+    return size_t(reinterpret_cast<uintptr_t>(p.snapshot)) +
+           al256g((size_t(cache->sequences) * cache->max_pages + cache->sequences) * 4);
+}
+
+extern "C" int hq_pages_resize(const hq_pages* cache, const int32_t* new_lengths, int window, int sinks,
+                               void* workspace, void* stream)
+{
+    if (!pages_shape_ok(cache) || !new_lengths || !workspace || window < 0 || sinks < 0) return HQ_ERR_ARG;
+    if (!cache->keys || !cache->values || !cache->table || !cache->lengths || !cache->refs || !cache->status)
+        return HQ_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) || (reinterpret_cast<uintptr_t>(cache->keys) & 15u) ||
+        (reinterpret_cast<uintptr_t>(cache->values) & 15u))
+        return HQ_ERR_ALIGN;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    PagesParams p = pages_params(cache, workspace);
+    p.want = new_lengths;
+    p.window = window;
+    p.sinks = sinks;
+    hipLaunchKernelGGL(resize_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
+    hipLaunchKernelGGL(resize_apply_kernel, dim3(kCopyBlocks), dim3(kBlock), 0, s, p);
+    return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
+}
+
+extern "C" int hq_pages_fork(const hq_pages* cache, const int32_t* parents, void* workspace, void* stream)
+{
+    if (!pages_shape_ok(cache) || !parents || !workspace) return HQ_ERR_ARG;
+    if (!cache->table || !cache->lengths || !cache->refs || !cache->status) return HQ_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return HQ_ERR_ALIGN;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    PagesParams p = pages_params(cache, workspace);
+    p.want = parents;
+    hipLaunchKernelGGL(fork_snapshot_kernel, dim3(cache->sequences), dim3(kBlock), 0, s, p);
+    hipLaunchKernelGGL(fork_rows_kernel, dim3(cache->sequences), dim3(kBlock), 0, s, p);
+    return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
+}
+
+extern "C" int hq_pages_compact(const hq_pages* cache, int32_t* live, void* workspace, void* stream)
+{
+    if (!pages_shape_ok(cache) || !workspace) return HQ_ERR_ARG;
+    if (!cache->keys || !cache->values || !cache->table || !cache->refs) return HQ_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) || (reinterpret_cast<uintptr_t>(cache->keys) & 15u) ||
+        (reinterpret_cast<uintptr_t>(cache->values) & 15u))
+        return HQ_ERR_ALIGN;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    PagesParams p = pages_params(cache, workspace);
+    p.live = live;
+    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
+    hipLaunchKernelGGL(compact_apply_kernel, dim3(kCopyBlocks), dim3(kBlock), 0, s, p);
+    return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
+}

@@ -177,6 +177,95 @@ int hq_quant_int4_gemm(const float* x, const uint8_t* weights, const float* scal
                        float* act_scales_out, int32_t* acc_out, void* workspace,
                        void* stream);
 
+/* ------------------------------------------------------- paged cache --
+ * An fp16 K/V cache of many sequences in pages of page_size positions that
+ * sequences may share.  No reference counterpart (the reference keeps one
+ * contiguous cache per session, cpu_lightspark.py:275-309).
+ * Row b of `table` holds the pages of sequence b in order (-1: none; entries
+ * past its length are -1), lengths[b] its positions, refs[p] the number of
+ * table entries that hold page p (0: the page is free).  A layer's page p is
+ * keys + ((layer*pages + p)*kv_heads + h)*page_size*head_dim for kv head h:
+ * one head's positions of a page are contiguous.  Everything lives on the
+ * device, so a captured graph of these calls is valid at every length.
+ * page_size: a power of two from 16 to 256; head_dim in {16, 32, 64, 128}.
+ * Entries, lengths, starts and parents outside their ranges are never
+ * followed: an entry counts as -1, and the calls that take a status report
+ * HQ_PAGES_BAD. */
+typedef struct hq_pages {
+    int32_t layers;       /* layers of keys and values (see each call) */
+    int32_t pages, page_size, kv_heads, head_dim;
+    int32_t sequences, max_pages;
+    int32_t reserved;
+    uint16_t* keys;       /* fp16 [layers, pages, kv_heads, page_size, head_dim] */
+    uint16_t* values;
+    int32_t* table;       /* [sequences, max_pages] */
+    int32_t* lengths;     /* [sequences] */
+    int32_t* refs;        /* [pages] */
+    int32_t* status;      /* [1] 0, or HQ_PAGES_* bits (sticky) */
+} hq_pages;
+
+#define HQ_PAGES_FULL 1   /* too few free pages, or a sequence past max_pages: that call changed nothing */
+#define HQ_PAGES_BAD 2    /* an entry, length, start or parent outside its range */
+
+/* Set the lengths: sequence b goes to new_lengths[b] positions (device int32
+ * [sequences]; negative: unchanged).  A growing sequence gets the pages it
+ * lacks, the lowest free ones in the order of the table's entries, and where
+ * the partly filled page that it goes on writing to is held by other entries
+ * too, a copy of that page's filled positions in every layer (if all its
+ * holders grow in this call, the first of them keeps the page).  A shrinking
+ * one releases the pages past its new length (0: all).  Pages released by a
+ * call are free for the next call, not for this one.  With window > 0 every
+ * sequence also releases the pages that no query from position min(old, new)
+ * on sees under that window and `sinks` (hq_paged_attention); their entries
+ * become -1.  All or nothing: HQ_PAGES_FULL or HQ_PAGES_BAD leave everything
+ * as it was.  `workspace`: hq_pages_workspace_bytes(cache) bytes, 256-byte
+ * aligned, of any contents. */
+size_t hq_pages_workspace_bytes(const hq_pages* cache);
+int hq_pages_resize(const hq_pages* cache, const int32_t* new_lengths, int window, int sinks, void* workspace,
+                    void* stream);
+/* Forks: every sequence b at once takes over the pages and the length of
+ * sequence parents[b] as they were before the call (device int32
+ * [sequences]; negative or b itself: unchanged), sharing them; what it held
+ * is released.  No K/V is moved (hq_pages_resize copies a shared page when it
+ * is written to next); keys and values are not used. */
+int hq_pages_fork(const hq_pages* cache, const int32_t* parents, void* workspace, void* stream);
+/* Move the pages in use to the lowest places: of the n pages in use, the ones
+ * at n and above go, in order, to the free places below n, in every layer;
+ * table and refs follow.  live (device int32 [1], nullable) receives n. */
+int hq_pages_compact(const hq_pages* cache, int32_t* live, void* workspace, void* stream);
+
+/* Append one layer's new tokens: qkv fp32 [tokens, (heads + 2*kv_heads) *
+ * head_dim] raw fused projection rows; per row the q/k head norms
+ * (x / sqrt(mean x^2 + eps)) * weight, RoPE at the token's position
+ * (rope_cos/rope_sin fp32 [rope_positions, head_dim/2]), q to query fp32
+ * [tokens, heads, head_dim], k and v as fp16 into their pages, with the
+ * arithmetic of hq_decode_step.  keys/values are the layer's pages (layers is
+ * not used), and lengths count the new tokens: the tokens of sequence b are
+ * rows starts[b] .. starts[b+1] - 1 (device int32 [sequences + 1], not
+ * falling; NULL: token b of sequence b, tokens = sequences) at positions
+ * lengths[b] - n_b .. lengths[b] - 1.  A row at a position outside the cache
+ * or the rope tables, or without a page, sets HQ_PAGES_BAD, writes no K/V
+ * and a query of zeros; rows of no sequence are not touched.  While status
+ * has HQ_PAGES_FULL set no K/V is written (the lengths did not grow, so the
+ * rows would land on earlier ones). */
+int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* starts, int tokens, int heads,
+                    const float* q_norm, const float* k_norm, float eps, const float* rope_cos,
+                    const float* rope_sin, int rope_positions, float* query, void* stream);
+
+/* Grouped-query attention of a batch's new tokens (rows as in
+ * hq_paged_append) over one layer's pages: the query at position p sees the
+ * positions j <= p that have a page, with window > 0 only those with
+ * j > p - window or j < sinks.  query, output fp32 [tokens, heads,
+ * head_dim], heads ordered [kv_head, group], groups = heads/kv_heads <= 8.
+ * A row that sees nothing gets zeros; rows of no sequence are not touched.
+ * Values at positions past a sequence's length are never used, whatever they
+ * hold.  status may be NULL.  `workspace`:
+ * hq_paged_attention_workspace_bytes(...) bytes, 256-byte aligned, of any
+ * contents. */
+size_t hq_paged_attention_workspace_bytes(int tokens, int sequences, int heads, int kv_heads, int head_dim);
+int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens, int heads,
+                       int window, int sinks, float* output, void* workspace, void* stream);
+
 /* ----------------------------------------------------- decode step --
  * One decode step of a Qwen3-shaped model, as LiteSparkQwen.forward_token
  * (cpu_lightspark.py:424-468): embedding row decode, per layer RMSNorm ->
