@@ -1,0 +1,994 @@
+// hq_paged_attn.hip - grouped-query attention of a batch's new tokens over the
+// paged K/V cache on gfx950 (hq_paged_attention).  No reference counterpart:
+// the reference attends one contiguous cache per session, token by token
+// (cpu_lightspark.py:389-422).
+//
+// For a query at position p and the positions j it sees:
+//   s_j = q.k_j / sqrt(D),  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
+// in one pass over the keys with the running maximum m and sum l.
+//
+// Precision: K and V are fp16, queries and outputs fp32, so the products run
+// on the fp16 matrix cores with the fp32 side in two parts.  A query row is
+// scaled by a power of two (its largest value into [2^9, 2^10)) and split
+// q = hi + lo, both fp16: 22 bits, and what small values lose is below 2^-34
+// of the row's largest.  The weights go as 2^14 e^(s-m) = hi + lo likewise.
+// K and V enter exactly; scores, m, l and outputs are fp32.  A product costs
+// two matrix instructions this way, against a rate of a sixteenth for the
+// fp32 ones.
+//
+// Tiles: the rows of a tile are (token, head of the group) pairs of one
+// sequence and kv head, so a K/V row is read once for all G heads.  Scores
+// are computed transposed, S^T = K Q^T: a lane then holds scores of one row
+// only, m and l are per lane, and the scores' registers are already the
+// operand of O^T = V^T P^T (the order of the keys inside a product is free as
+// long as V follows it).
+//   small  up to 16 rows (single tokens): 16x16x32 products, each of a block's
+//          4 waves on its own 32 keys, K and V straight to registers, the
+//          waves' parts joined in LDS.  Bound by HBM.
+//   large  128 rows, 32 a wave: 32x32x16 products over chunks of 64 keys that
+//          the block stages in LDS (K by direct copies, V transposed on the
+//          way), two buffers.  Bound by the matrix cores.
+//
+// Work: a tile's chunks are cut into pieces of about T = all work / kTarget
+// chunks (per sequence: the same number of pieces for all its tiles), each a
+// block; a tile of one piece writes its outputs, the others leave partial
+// results (m, l, O) that a second launch joins.  Every wave works the plan out
+// from starts and lengths, which live on the device.
+//
+// What matrix products cannot mask: 0 x NaN.  Values past a sequence's end are
+// zeroed on the way in; where a row's result is not finite for another reason
+// (an infinity or NaN in K or V, seen by it or by another row of the tile),
+// the row is computed again by paged_row, in fp32 from the visible positions
+// alone.
+#include "hq_device.h"
+#include "hq_internal.h"
+#include "hq_paged.h"
+
+namespace hq {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+constexpr int kChunkKeys = 64;
+constexpr int kSmallRows = 16;
+constexpr int kTileRows = 128;
+constexpr int kTarget = 1024;          // pieces aimed at
+constexpr int kSmallMin = 2;           // fewest chunks of a small piece: a step of 32 keys a wave
+constexpr int kLargeMin = 4;
+constexpr int kJoinThreads = 512;
+
+struct PagedAttnParams {
+    PagedBatch b;
+    const float* query;          // [tokens, heads, D]
+    float* out;
+    int window, sinks;           // window 0: none
+    int tile_tokens;             // tokens of a large tile
+    int part_rows;               // rows of partial results there is room for
+    int32_t* ordered;            // [1] starts never fall
+    int2* desc;                  // [tokens, kv_heads] 2 * pieces + small, first partial row
+    float* part_o;               // [part_rows, D]
+    float2* part_ml;             // [part_rows] m (of the scores times log2 e), l
+};
+
+// Whether the query at position `pos` sees position j (pages aside).
+__device__ __forceinline__ bool paged_visible(int pos, int j, int window, int sinks)
+{
+    return j <= pos && (window == 0 || j > pos - window || j < sinks);
+}
+
+constexpr float kLog2e = 0x1.715476p+0f;
+constexpr float kWeightScale = 16384.0f;           // 2^14
+
+// ------------------------------------------------------------- one row, fp32
+// One query row over positions [lo, hi) of sequence b, kv head h, in one wave:
+// a lane scores one position of 64 at a time and holds D/64 of the output's
+// values.  `seen`: whether anything was visible.
+template <int D>
+__device__ void paged_row(const PagedAttnParams& p, const float* q, int b, int h, int pos, int lo, int hi,
+                          float& m, float& l, float (&o)[2], bool& seen)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    const float scale = 1.0f / __builtin_sqrtf(float(D));
+    const size_t head = size_t(p.b.page_size) * D;
+    for (int base = lo; base < hi; base += kWave) {
+        const int j = base + lane;
+        const int page = j < hi ? paged_page(p.b, b, j) : -1;
+        const bool visible = page >= 0 && paged_visible(pos, j, p.window, p.sinks);
+        if (!__any(visible)) continue;
+        seen = true;
+        const size_t row = (size_t(max(page, 0)) * p.b.kv_heads + h) * head + size_t(j & (p.b.page_size - 1)) * D;
+        float s = -__builtin_inff();
+        if (visible) {
+            const uint4* k = reinterpret_cast<const uint4*>(p.b.keys + row);
+            float acc = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+                const uint4 v = k[c];
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc = __builtin_fmaf(q[8 * c + 2 * i], f16_to_f32(uint16_t(w[i])), acc);
+                    acc = __builtin_fmaf(q[8 * c + 2 * i + 1], f16_to_f32(uint16_t(w[i] >> 16)), acc);
+                }
+            }
+            s = acc * scale;
+        }
+        const float top = fmaxf(m, wave_max64_all(s));
+        const float alpha = m == top ? 1.0f : expf(m - top);
+        const float e = !visible || (top == -__builtin_inff() && s == top) ? 0.0f : expf(s - top);
+        l = l * alpha;
+        o[0] *= alpha;
+        o[1] *= alpha;
+        uint64_t left = __ballot(visible);
+        while (left) {
+            const int i = __builtin_ctzll(left);
+            left &= left - 1;
+            const float pi = __shfl(e, i, kWave);
+            const size_t vrow = (uint64_t(uint32_t(__shfl(int(row >> 32), i, kWave))) << 32) |
+                                uint32_t(__shfl(int(uint32_t(row)), i, kWave));
+            l += pi;
+            if (lane < D) o[0] = __builtin_fmaf(pi, f16_to_f32(p.b.values[vrow + lane]), o[0]);
+            if (D == 128) o[1] = __builtin_fmaf(pi, f16_to_f32(p.b.values[vrow + lane + 64]), o[1]);
+        }
+        m = top;
+    }
+}
+
+// ---------------------------------------------------------------------- plan
+// The chunks of 64 positions that a tile's queries, at positions pa .. pb,
+// see: chunks 0 .. sink - 1, then `first` and on, `count` in all.
+struct Span {
+    int sink, first, count;
+    __device__ __forceinline__ int chunk(int c) const { return c < sink ? c : first + (c - sink); }
+};
+
+__device__ __forceinline__ Span span_of(const PagedAttnParams& p, int pa, int pb)
+{
+    if (pb < 0) return Span{0, 0, 0};
+    const int64_t end = min(int64_t(pb) + 1, int64_t(p.b.max_pages) << p.b.shift);
+    const int last = int((end + kChunkKeys - 1) / kChunkKeys);
+    const int low = p.window > 0 ? int(max(int64_t(0), int64_t(pa) - p.window + 1)) : 0;
+    const int first = low / kChunkKeys;
+    const int sunk = min(p.sinks, low);
+    const int sink = min(min(first, last), sunk / kChunkKeys + (sunk % kChunkKeys != 0));
+    return Span{sink, first, sink + max(0, last - first)};
+}
+
+struct SequencePlan {
+    int first, n;                // rows
+    int length;
+    int tile_tokens, tiles, chunks;   // chunks of the last tile (no other has more)
+    bool small;
+    __device__ __forceinline__ int position(int i) const
+    {
+        return int(max(int64_t(length) - n + i, int64_t(-1)));
+    }
+};
+
+__device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, int b, bool* fall)
+{
+    SequencePlan s;
+    s.first = b;
+    s.n = 1;
+    if (p.b.starts) {
+        const int a = p.b.starts[b], z = p.b.starts[b + 1];
+        *fall |= a > z;
+        s.first = a;
+        s.n = a < 0 || a >= z || z > p.b.tokens ? 0 : z - a;
+    }
+    s.length = p.b.lengths[b];
+    s.small = int64_t(s.n) * p.b.groups <= kSmallRows;
+    s.tile_tokens = s.small ? max(1, s.n) : p.tile_tokens;
+    s.tiles = (s.n + s.tile_tokens - 1) / s.tile_tokens;
+    s.chunks = s.n ? span_of(p, s.position((s.tiles - 1) * s.tile_tokens), s.position(s.n - 1)).count : 0;
+    return s;
+}
+
+// A block's piece: one tile (rows of one sequence and kv head), some of its chunks.
+struct Piece {
+    int b, head;
+    int first, n;                // the tile's tokens
+    int pos;                     // position of its first token (may be -1: before the sequence; see row())
+    int64_t origin;              // lengths[b] - n_b + the tile's first token
+    int length;
+    int pieces, split, part;     // part: first partial row of this piece
+    bool small;
+    __device__ __forceinline__ int position(int i) const { return int(max(origin + i, int64_t(-1))); }
+};
+
+__device__ __forceinline__ int64_t wave_sum_i64(int64_t v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor((long long)v, o, kWave);
+    return v;
+}
+
+// The work of block `q`, the same in every wave; false: none.
+__device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piece& out)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    bool fall = false;
+    int64_t units = 0;
+    SequencePlan mine{};
+    for (int base = 0; base < p.b.sequences; base += kWave) {
+        if (base + lane < p.b.sequences) {
+            mine = sequence_plan(p, base + lane, &fall);
+            units += int64_t(mine.tiles) * mine.chunks;
+        }
+    }
+    const bool ordered = !__any(fall);
+    if (q == 0 && threadIdx.x == 0) *p.ordered = ordered;
+    if (!ordered) return false;
+    units = wave_sum_i64(units) * p.b.kv_heads;
+    const int target = int(min((units + kTarget - 1) / kTarget, int64_t(0x40000000)));
+    int64_t pieces = 0, rows = 0;
+    for (int base = 0; base < p.b.sequences; base += kWave) {
+        const bool in = base + lane < p.b.sequences;
+        if (p.b.sequences > kWave && in) mine = sequence_plan(p, base + lane, &fall);
+        if (!in) mine.tiles = 0;
+        const int most = max(target, mine.small ? kSmallMin : kLargeMin);
+        const int cuts = max(1, (mine.chunks + most - 1) / most);
+        const int64_t here = int64_t(mine.tiles) * cuts * p.b.kv_heads;
+        const int64_t part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
+        int64_t incl = here, part_incl = part;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int64_t y = __shfl_up((long long)incl, o, kWave), z = __shfl_up((long long)part_incl, o, kWave);
+            if (lane >= o) {
+                incl += y;
+                part_incl += z;
+            }
+        }
+        const uint64_t found = __ballot(q >= pieces + incl - here && q < pieces + incl);
+        if (found) {
+            const int src = __builtin_ctzll(found);
+            auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+            const int local = from(int(q - (pieces + incl - here)));
+            const int first_part = from(int(rows + part_incl - part));
+            out.pieces = from(cuts);
+            out.small = from(mine.small);
+            out.length = from(mine.length);
+            const int n = from(mine.n), tokens = from(mine.tile_tokens), tiles = from(mine.tiles);
+            out.b = base + src;
+            out.head = local % p.b.kv_heads;
+            const int rest = local / p.b.kv_heads;
+            out.split = rest % out.pieces;
+            const int tile = tiles - 1 - rest / out.pieces;      // the longest first
+            out.first = from(mine.first) + tile * tokens;
+            out.n = min(tokens, n - tile * tokens);
+            out.origin = int64_t(out.length) - n + tile * tokens;
+            out.pos = out.position(0);
+            out.part = first_part + (((tile * p.b.kv_heads + out.head) * out.pieces) + out.split) *
+                                        (out.small ? kSmallRows : kTileRows);
+            return true;
+        }
+        pieces += __shfl((long long)incl, kWave - 1, kWave);
+        rows += __shfl((long long)part_incl, kWave - 1, kWave);
+    }
+    return false;
+}
+
+// ------------------------------------------------------------- query operands
+// Eight values of a row as fp16 parts hi + lo of 2^-e times them.
+__device__ __forceinline__ void split8(const float (&x)[8], int e, half8& hi, half8& lo)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float y = __builtin_ldexpf(x[i], -e);
+        hi[i] = _Float16(y);
+        lo[i] = _Float16(y - float(hi[i]));
+    }
+}
+
+// The exponent that takes values of at most `top` to below 2^10 (0 for a row of zeros or without a finite maximum).
+__device__ __forceinline__ int row_exponent(float top)
+{
+    if (!(top > 0.0f) || top == __builtin_inff()) return 0;
+    return max(-100, int(__builtin_amdgcn_frexp_expf(top)) - 10);   // (2^e / sqrt(D) stays a normal number)
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Weights p (of up to 2^14) as hi + lo.
+__device__ __forceinline__ void split_weights(const float (&w)[8], half8& hi, half8& lo)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2v x = {w[i], w[i + 1]};
+        const half2v h = __builtin_convertvector(x, half2v);
+        const float2v r = {w[i] - float(h[0]), w[i + 1] - float(h[1])};
+        const half2v g = __builtin_convertvector(r, half2v);
+        hi[i] = h[0];
+        hi[i + 1] = h[1];
+        lo[i] = g[0];
+        lo[i + 1] = g[1];
+    }
+}
+
+__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
+
+// The result of one row, by one wave in fp32 (see paged_row), as this piece's output or part.
+template <int D>
+__device__ void redo_row(const PagedAttnParams& p, const Piece& w, const Span& span, int c0, int c1, int r)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    const size_t row = size_t(w.first + r / p.b.groups) * p.b.heads + w.head * p.b.groups + r % p.b.groups;
+    float m = -__builtin_inff(), l = 0.0f, o[2] = {0.0f, 0.0f};
+    bool seen = false;
+    const int64_t end = int64_t(p.b.max_pages) << p.b.shift;
+    for (int c = c0; c < c1; ++c) {
+        const int at = span.chunk(c) * kChunkKeys;
+        paged_row<D>(p, p.query + row * D, w.b, w.head, w.position(r / p.b.groups), at,
+                     int(min(end, int64_t(at) + kChunkKeys)), m, l, o, seen);
+    }
+    if (w.pieces == 1) {
+        if (lane < D) p.out[row * D + lane] = seen ? o[0] / l : 0.0f;
+        if (D == 128) p.out[row * D + lane + 64] = seen ? o[1] / l : 0.0f;
+        return;
+    }
+    const size_t at = size_t(w.part + r);
+    if (lane < D) p.part_o[at * D + lane] = o[0];
+    if (D == 128) p.part_o[at * D + lane + 64] = o[1];
+    // (a row whose scores are all -inf has no softmax: the join finds the NaN where nothing else counts)
+    if (lane == 0) p.part_ml[at] = make_float2(m * kLog2e, seen && m == -__builtin_inff() ? __builtin_nanf("") : l);
+}
+
+// ---------------------------------------------------------------- small tiles
+template <int D>
+struct SmallShared {
+    float o[4][kSmallRows][D];
+    float m[4][kSmallRows], l[4][kSmallRows];
+    int bad[kSmallRows];
+};
+
+template <int D>
+__device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span& span, int c0, int c1,
+                           SmallShared<D>& S)
+{
+    constexpr int STEPS = (D + 31) / 32;       // products over the dims
+    constexpr int VEC = D / 16;                // dims a lane holds of a V row
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int n = lane & 15, g = lane >> 4;
+    const int G = p.b.groups;
+    const int rows = w.n * G;
+    const int ps = p.b.page_size;
+    const bool mine = n < rows;
+    // this lane's query row (n), dims 32 s + 8 g ..
+    half8 qhi[STEPS], qlo[STEPS];
+    float c;
+    {
+        const float* q = p.query + (size_t(w.first + (mine ? n / G : 0)) * p.b.heads + w.head * G + (mine ? n % G : 0)) * D;
+        float x[STEPS][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = 32 * s + 8 * g + i;
+                x[s][i] = mine && d < D ? q[d < D ? d : 0] : 0.0f;
+                top = fmaxf(top, __builtin_fabsf(x[s][i]));
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const int e = row_exponent(top);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) split8(x[s], e, qhi[s], qlo[s]);
+        c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
+    }
+    const int pos = w.position(mine ? n / G : 0);
+    const int pos_min = w.position(0), pos_max = w.position(w.n - 1);
+    float4v acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+    bool seen = false;
+
+    // this wave's steps of 32 keys: wave, wave + 4, ...; pages of 32 of them at a time, two a step, in a register
+    const int steps = 2 * (c1 - c0);
+    const size_t head_stride = size_t(ps) * D;
+    auto key_of = [&](int t) { return span.chunk(c0 + (t >> 1)) * kChunkKeys + (t & 1) * 32; };
+    auto pages_of = [&](int k) {                       // k: the wave's k-th step, first of 32
+        const int t = wave + 4 * (k + (lane >> 1));
+        return t < steps ? paged_page(p.b, w.b, key_of(t) + 16 * (lane & 1)) : -1;
+    };
+    half8 kf[2][STEPS];
+    uint32_t vf[8][VEC >= 2 ? VEC / 2 : 1];
+    auto base_of = [&](int page, int j) {
+        return (size_t(max(page, 0)) * p.b.kv_heads + w.head) * head_stride + size_t(j & (ps - 1)) * D;
+    };
+    auto load_k = [&](int pg0, int pg1, int j) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint16_t* k = p.b.keys + base_of(t ? pg1 : pg0, j + 16 * t);
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int d = 32 * s + 8 * g;
+                kf[t][s] = D >= 32 || d < D ? *reinterpret_cast<const half8*>(k + n * D + d) : half8{};
+            }
+        }
+    };
+    auto load_v = [&](int pg0, int pg1, int j) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint16_t* v = p.b.values + base_of(t ? pg1 : pg0, j + 16 * t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t* a = v + (4 * g + i) * D + VEC * n;
+                if constexpr (VEC == 8) {
+                    const uint4v x = *reinterpret_cast<const uint4v*>(a);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) vf[4 * t + i][d] = x[d];
+                } else if constexpr (VEC == 4) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(a);
+                    vf[4 * t + i][0] = x.x;
+                    vf[4 * t + i][1] = x.y;
+                } else if constexpr (VEC == 2) {
+                    vf[4 * t + i][0] = *reinterpret_cast<const uint32_t*>(a);
+                } else {
+                    vf[4 * t + i][0] = *a;
+                }
+            }
+        }
+    };
+    const int own = steps > wave ? (steps - wave + 3) / 4 : 0;
+    int pg = own ? pages_of(0) : -1;
+    int pg0 = __builtin_amdgcn_readlane(pg, 0), pg1 = __builtin_amdgcn_readlane(pg, 1);
+    int j0 = own ? key_of(wave) : 0;
+    if (own) {
+        load_k(pg0, pg1, j0);
+        load_v(pg0, pg1, j0);
+    }
+    for (int k = 0; k < own; ++k) {
+        // the next step's pages
+        const int kn = k + 1;
+        int next0 = -1, next1 = -1, nj = 0;
+        if (kn < own) {
+            if ((kn & 31) == 0) pg = pages_of(kn);
+            next0 = __builtin_amdgcn_readlane(pg, 2 * (kn & 31));
+            next1 = __builtin_amdgcn_readlane(pg, 2 * (kn & 31) + 1);
+            nj = key_of(wave + 4 * kn);
+        }
+        float4v s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int d = 0; d < STEPS; ++d) {
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qlo[d], s[t], 0, 0, 0);
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qhi[d], s[t], 0, 0, 0);
+            }
+        }
+        if (kn < own) load_k(next0, next1, nj);
+        // lane (n, g): row n, keys j0 + 16 t + 4 g + i
+        const bool all = pg0 >= 0 && pg1 >= 0 && j0 + 31 <= pos_min &&
+                         (p.window == 0 || j0 > pos_max - p.window || j0 + 32 <= p.sinks);
+        if (!all) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + 16 * t + 4 * g + i;
+                    const bool there = (t ? pg1 : pg0) >= 0;
+                    const bool visible = there && paged_visible(pos, j, p.window, p.sinks);
+                    s[t][i] = visible ? s[t][i] : -__builtin_inff();
+                    seen |= visible;
+                    if (!there || j >= w.length)
+#pragma unroll
+                        for (auto& x : vf[4 * t + i]) x = 0;
+                }
+        } else {
+            seen = true;
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = fmaxf(m, top);
+        const float safe = top == -__builtin_inff() ? 0.0f : top;
+        if (__any(top > m)) {
+            const float alpha = exp2_fast((m - safe) * c);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] *= alpha;
+            m = top;
+        }
+        const float shift = 14.0f - safe * c;
+        float e[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[4 * t + i] = exp2_fast(__builtin_fmaf(s[t][i], c, shift));
+                l += e[4 * t + i];
+            }
+        half8 hi, lo;
+        split_weights(e, hi, lo);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            // dims VEC n + i: half (i & 1) of word i / 2 of each key
+            uint4v a;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+                a[d] = __builtin_amdgcn_perm(vf[2 * d + 1][i / 2], vf[2 * d][i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
+            const half8 v = __builtin_bit_cast(half8, a);
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, acc[i], 0, 0, 0);
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, acc[i], 0, 0, 0);
+        }
+        if (kn < own) load_v(next0, next1, nj);
+        pg0 = next0;
+        pg1 = next1;
+        j0 = nj;
+    }
+    l += __shfl_xor(l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+    // join the four waves: lane (n, g) holds row n, dims VEC (4 g + i) + v
+    if (g == 0) {
+        S.m[wave][n] = m * c;
+        S.l[wave][n] = l;
+    }
+    if (threadIdx.x < kSmallRows) S.bad[threadIdx.x] = 0;
+    const uint64_t any_seen = __ballot(seen);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S.o[wave][n][VEC * (4 * g + i) + v] = acc[v][i];
+    // rows of which this wave saw something: bit n (of any g)
+    const uint32_t rows_seen = uint32_t(any_seen | (any_seen >> 16) | (any_seen >> 32) | (any_seen >> 48)) & 0xFFFFu;
+    __syncthreads();
+    if (lane < kSmallRows && ((rows_seen >> lane) & 1)) atomicOr(&S.bad[lane], 2);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * D; i += kBlock) {
+        const int r = i / D, d = i % D;
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int v = 0; v < 4; ++v) top = fmaxf(top, S.m[v][r]);
+        float sum = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const float f = S.m[v][r] == -__builtin_inff() ? 0.0f : exp2_fast(S.m[v][r] - top);
+            sum += S.l[v][r] * f;
+            o += S.o[v][r][d] * f;
+        }
+        const bool none = (S.bad[r] & 2) == 0;
+        const bool bad = !none && (!finite(sum) || !finite(o) || sum == 0.0f);
+        if (bad) atomicOr(&S.bad[r], 1);
+        const size_t row = size_t(w.first + r / p.b.groups) * p.b.heads + w.head * p.b.groups + r % p.b.groups;
+        if (w.pieces == 1) {
+            p.out[row * D + d] = none ? 0.0f : o / sum;
+        } else {
+            p.part_o[size_t(w.part + r) * D + d] = none ? 0.0f : o * (1.0f / kWeightScale);
+            if (d == 0) p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f)
+                                                     : make_float2(top, sum * (1.0f / kWeightScale));
+        }
+    }
+    __syncthreads();
+    for (int r = wave; r < rows; r += 4)
+        if (S.bad[r] & 1) redo_row<D>(p, w, span, c0, c1, r);
+}
+
+// ---------------------------------------------------------------- large tiles
+template <int D>
+struct LargeShared {
+    static constexpr int VROWS = D < 32 ? 32 : D;
+    alignas(16) uint16_t k[2][kChunkKeys * D];         // [key][dim], 16-byte pieces of a row permuted by the key
+    alignas(16) uint16_t v[2][VROWS * kChunkKeys];     // [dim][key], keys in the products' order
+};
+
+// Permutation of the 16-byte pieces of V^T row `dim` in LDS: 16 rows that a
+// product reads together lie in 16 different places of the 64 banks, and the
+// writes of 4-row groups in 8 of 16.
+__device__ __forceinline__ int v_swizzle(int dim) { return ((dim >> 1) ^ (dim >> 3)) & 7; }
+
+template <int D>
+__device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span& span, int c0, int c1,
+                           LargeShared<D>& S)
+{
+    constexpr int STEPS = D / 16;
+    constexpr int DT = D < 32 ? 1 : D / 32;
+    constexpr int PIECES = D / 8;              // 16-byte pieces of a K row
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int n = lane & 31, g = lane >> 5;
+    const int G = p.b.groups;
+    const int ps = p.b.page_size;
+    const int rows = w.n * G;
+    const int r = 32 * wave + n;               // this lane's row
+    const bool mine = r < rows;
+    const int token = mine ? r / G : 0;
+    const size_t out_row = size_t(w.first + token) * p.b.heads + w.head * G + (mine ? r % G : 0);
+    half8 qhi[STEPS], qlo[STEPS];
+    float c;
+    {
+        const float* q = p.query + out_row * D;
+        float top = 0.0f;
+        float x[STEPS][8];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const float4v a = *reinterpret_cast<const float4v*>(q + 16 * s + 8 * g);
+            const float4v b = *reinterpret_cast<const float4v*>(q + 16 * s + 8 * g + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[s][i] = mine ? a[i] : 0.0f;
+                x[s][4 + i] = mine ? b[i] : 0.0f;
+                top = fmaxf(top, fmaxf(__builtin_fabsf(x[s][i]), __builtin_fabsf(x[s][4 + i])));
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const int e = row_exponent(top);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) split8(x[s], e, qhi[s], qlo[s]);
+        c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
+    }
+    const int pos = w.position(token);
+    const bool active = 32 * wave < rows;      // (wave-uniform)
+    const int pos_min = w.position(min(32 * wave, rows - 1) / G);
+    const int pos_max = w.position(min(32 * wave + 31, rows - 1) / G);
+
+    float16v acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[i][k] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+    bool seen = false;
+
+    const size_t head_stride = size_t(ps) * D;
+    auto base_of = [&](int page, int j) {
+        return (size_t(max(page, 0)) * p.b.kv_heads + w.head) * head_stride + size_t(j & (ps - 1)) * D;
+    };
+    // pages of 16 chunks at a time, 4 parts of 16 keys each, in a register
+    auto pages_of = [&](int cc) {
+        const int at = cc + (lane >> 2);
+        return at < c1 ? paged_page(p.b, w.b, span.chunk(at) * kChunkKeys + 16 * (lane & 3)) : -1;
+    };
+    // V on its way to LDS: thread (piece pc of 8 keys, 4 dims)
+    const int pc = threadIdx.x / (D / 4), dg = threadIdx.x % (D / 4);
+    const bool stages = pc < 8;
+    uint2 vr[8];
+    auto fetch = [&](int pg, int first, int cc) {
+        const int j0 = span.chunk(cc) * kChunkKeys;
+        const int lane0 = 4 * (cc - first);
+        const int sub = pc >> 1;
+        const int vpage = __shfl(pg, lane0 + (sub & 3), kWave);   // (every lane takes part)
+        if (stages) {
+            const int page = vpage;
+            const uint16_t* v = p.b.values + base_of(page, j0 + 16 * sub) + 4 * dg;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                vr[i] = *reinterpret_cast<const uint2*>(v + (8 * (i >> 2) + 4 * (pc & 1) + (i & 3)) * D);
+            if (page < 0 || j0 + kChunkKeys > w.length) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = j0 + 16 * sub + 8 * (i >> 2) + 4 * (pc & 1) + (i & 3);
+                    if (page < 0 || j >= w.length) vr[i] = make_uint2(0, 0);
+                }
+            }
+        }
+        // K rows 16 wave .. + 15, contiguous in their page
+        const int page = __builtin_amdgcn_readlane(pg, lane0 + wave);
+        const uint16_t* k = p.b.keys + base_of(page, j0 + 16 * wave);
+        const uint32_t to = lds_addr(&S.k[cc & 1][16 * wave * D]);
+#pragma unroll
+        for (int i = 0; i < (PIECES + 3) / 4; ++i) {
+            const int u = 64 * i + lane;
+            const int row = u / PIECES, at = u % PIECES;
+            const uint32_t off = uint32_t(row * PIECES + (at ^ (row & (PIECES - 1)))) * 16;
+            if (D >= 32 || lane < 16 * PIECES) dma16(k, off, to + 1024 * i);
+        }
+    };
+    auto store_v = [&](int buf) {
+        if (!stages) return;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            uint4v x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a = d < 2 ? vr[2 * i].x : vr[2 * i].y, b = d < 2 ? vr[2 * i + 1].x : vr[2 * i + 1].y;
+                x[i] = __builtin_amdgcn_perm(b, a, (d & 1) ? 0x07060302u : 0x05040100u);
+            }
+            const int dim = 4 * dg + d;
+            *reinterpret_cast<uint4v*>(&S.v[buf][dim * kChunkKeys + (pc ^ v_swizzle(dim)) * 8]) = x;
+        }
+    };
+    int pg = pages_of(c0), pg_first = c0;
+    if (c0 < c1) {
+        fetch(pg, pg_first, c0);
+        store_v(c0 & 1);
+    }
+    wait_all_memory();
+    __syncthreads();
+    for (int cc = c0; cc < c1; ++cc) {
+        const int buf = cc & 1;
+        const int j0 = span.chunk(cc) * kChunkKeys;
+        const uint32_t there = uint32_t(__ballot(pg >= 0) >> (4 * (cc - pg_first))) & 15u;   // parts with a page
+        if (cc + 1 < c1) {
+            if (cc + 1 - pg_first == 16) {
+                pg_first = cc + 1;
+                pg = pages_of(pg_first);
+            }
+            fetch(pg, pg_first, cc + 1);
+        }
+        const bool work = active && j0 <= pos_max;
+        float16v s[2];
+        half8 hi[4], lo[4];
+        if (work) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+                const int key = 32 * t + n;
+#pragma unroll
+                for (int d = 0; d < STEPS; ++d) {
+                    const half8 a = *reinterpret_cast<const half8*>(
+                        &S.k[buf][key * D + ((2 * d + g) ^ (key & (PIECES - 1))) * 8]);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qlo[d], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qhi[d], s[t], 0, 0, 0);
+                }
+            }
+            // lane (n, g): row n, keys j0 + 32 t + 8 (i / 4) + 4 g + i % 4
+            const bool all = there == 15u && j0 + kChunkKeys - 1 <= pos_min &&
+                             (p.window == 0 || j0 > pos_max - p.window || j0 + kChunkKeys <= p.sinks);
+            if (!all) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = 32 * t + 8 * (i >> 2) + 4 * g + (i & 3);
+                        const bool visible = ((there >> (2 * t + (i >> 3))) & 1) &&
+                                             paged_visible(pos, j0 + at, p.window, p.sinks);
+                        s[t][i] = visible ? s[t][i] : -__builtin_inff();
+                        seen |= visible;
+                    }
+            } else {
+                seen = true;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            top = fmaxf(m, top);
+            const float safe = top == -__builtin_inff() ? 0.0f : top;
+            if (__any(top > m)) {
+                const float alpha = exp2_fast((m - safe) * c);
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+                m = top;
+            }
+            const float shift = 14.0f - safe * c;
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = exp2_fast(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, shift));
+                    l += e[i];
+                }
+                split_weights(e, hi[st], lo[st]);
+            }
+        }
+        if (cc + 1 < c1) store_v(buf ^ 1);
+        if (work) {
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const int dim = 32 * dt + n;
+                    const half8 a = *reinterpret_cast<const half8*>(
+                        &S.v[buf][dim * kChunkKeys + ((2 * st + g) ^ v_swizzle(dim)) * 8]);
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, lo[st], acc[dt], 0, 0, 0);
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, hi[st], acc[dt], 0, 0, 0);
+                }
+        }
+        wait_all_memory();
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32, kWave);
+    // lane (n, g): row n, dims 32 dt + 8 (i / 4) + 4 g + i % 4
+    bool ok = finite(l) && l != 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (32 * dt + 8 * (i >> 2) < D) ok &= finite(acc[dt][i]);
+    const uint64_t was_seen = __ballot(seen);
+    const bool none = (((was_seen | (was_seen >> 32)) >> n) & 1) == 0;
+    const uint64_t wrong = __ballot(mine && !none && !ok);
+    const uint32_t again = uint32_t(wrong | (wrong >> 32));
+    if (mine && ((again >> n) & 1) == 0) {
+        const bool direct = w.pieces == 1;
+        float* to = direct ? p.out + out_row * D : p.part_o + size_t(w.part + r) * D;
+        const float f = none ? 0.0f : direct ? 1.0f / l : 1.0f / kWeightScale;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int dim = 32 * dt + 8 * i + 4 * g;
+                if (dim < D) {
+                    float4v x;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = none ? 0.0f : acc[dt][4 * i + k] * f;
+                    *reinterpret_cast<float4v*>(to + dim) = x;
+                }
+            }
+        if (!direct && g == 0)
+            p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f)
+                                         : make_float2(m * c, l * (1.0f / kWeightScale));
+    }
+    for (uint32_t left = again; left; left &= left - 1)
+        redo_row<D>(p, w, span, c0, c1, 32 * wave + __builtin_ctz(left));
+}
+
+template <int D, bool LARGE>
+struct AttnShared {
+    SmallShared<D> small;
+};
+template <int D>
+struct AttnShared<D, true> {
+    union {
+        SmallShared<D> small;
+        LargeShared<D> large;
+    };
+};
+
+template <int D, bool LARGE>
+__global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnParams p)
+{
+    __shared__ AttnShared<D, LARGE> S;
+    Piece w;
+    if (!plan_piece(p, blockIdx.x, w)) return;
+    // the join's directory: which rows have parts, and where
+    if (w.split == 0)
+        for (int i = threadIdx.x; i < w.n; i += kBlock)
+            p.desc[size_t(w.first + i) * p.b.kv_heads + w.head] =
+                make_int2(2 * w.pieces + (w.small ? 1 : 0), w.part + i * p.b.groups);
+    const Span span = span_of(p, w.pos, w.position(w.n - 1));
+    const int c0 = int(int64_t(span.count) * w.split / w.pieces);
+    const int c1 = int(int64_t(span.count) * (w.split + 1) / w.pieces);
+    if (w.small) small_tile<D>(p, w, span, c0, c1, S.small);
+    else if constexpr (LARGE) large_tile<D>(p, w, span, c0, c1, S.large);
+}
+
+// Join the parts of one token's heads of one kv head: thread (group of
+// parts, pair of values).
+template <int D>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParams p)
+{
+    __shared__ float so[kJoinThreads][2], sl[kJoinThreads], sm[kJoinThreads];
+    const int t = blockIdx.x, h = blockIdx.y;
+    if (*p.ordered == 0) return;
+    int first = 0, count = 0;
+    if (paged_sequence(p.b, t, &first, &count) < 0) return;
+    const int2 d = p.desc[size_t(t) * p.b.kv_heads + h];
+    const int pieces = d.x >> 1, stride = (d.x & 1) ? kSmallRows : kTileRows;
+    if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) return;
+    const int pairs = p.b.groups * D / 2;                 // at most 512
+    const int sets = kJoinThreads / pairs;
+    const int set = threadIdx.x / pairs, pair = threadIdx.x % pairs;
+    const int r = pair / (D / 2);
+    float m = -__builtin_inff(), l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    float lost = 0.0f;                                    // NaN where a part saw only scores of -inf
+    if (set < sets) {
+        for (int i = set; i < pieces; i += sets) {
+            const size_t row = size_t(d.y) + size_t(i) * stride + r;
+            const float2 ml = p.part_ml[row];
+            const float2 x = reinterpret_cast<const float2*>(p.part_o + row * D)[pair % (D / 2)];
+            if (ml.x == -__builtin_inff()) {
+                lost += ml.y;
+                continue;
+            }
+            const float top = fmaxf(m, ml.x);
+            const float a = exp2_fast(m - top), b = exp2_fast(ml.x - top);
+            l = l * a + ml.y * b;
+            o0 = o0 * a + x.x * b;
+            o1 = o1 * a + x.y * b;
+            m = top;
+        }
+    }
+    sm[threadIdx.x] = m;
+    sl[threadIdx.x] = m == -__builtin_inff() ? lost : l;
+    so[threadIdx.x][0] = o0;
+    so[threadIdx.x][1] = o1;
+    __syncthreads();
+    if (set != 0) return;
+    for (int k = 1; k < sets; ++k) {
+        const int i = k * pairs + pair;
+        if (sm[i] == -__builtin_inff()) {
+            lost += sl[i];
+            continue;
+        }
+        const float top = fmaxf(m, sm[i]);
+        const float a = exp2_fast(m - top), b = exp2_fast(sm[i] - top);
+        l = l * a + sl[i] * b;
+        o0 = o0 * a + so[i][0] * b;
+        o1 = o1 * a + so[i][1] * b;
+        m = top;
+    }
+    float2 y = make_float2(o0 / l, o1 / l);
+    if (m == -__builtin_inff()) y = make_float2(lost, lost);   // nothing seen: 0; only scores of -inf: NaN
+    const size_t row = size_t(t) * p.b.heads + h * p.b.groups + r;
+    reinterpret_cast<float2*>(p.out + row * D)[pair % (D / 2)] = y;
+}
+
+// -------------------------------------------------------------------- host
+struct AttnLayout {
+    size_t desc, ml, o, total;
+    int part_rows;
+};
+
+// Rows of partial results: a sequence cut in S > 1 pieces a tile has more
+// than T chunks a tile, so S < 2 chunks / T, and over all of them fewer than
+// 2 work / T <= 2 kTarget pieces.
+static AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large)
+{
+    AttnLayout L;
+    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    L.part_rows = 2 * kTarget * (large ? kTileRows : kSmallRows);
+    L.desc = 256;
+    L.ml = L.desc + up(size_t(tokens) * kv_heads * sizeof(int2));
+    L.o = L.ml + up(size_t(L.part_rows) * sizeof(float2));
+    L.total = L.o + up(size_t(L.part_rows) * head_dim * sizeof(float));
+    return L;
+}
+
+}  // namespace hq
+
+using namespace hq;
+
+// Whether a batch may hold a tile of more than 16 rows.
+static bool attn_large(int tokens, int groups, bool single) { return !single && int64_t(tokens) * groups > kSmallRows; }
+
+extern "C" size_t hq_paged_attention_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim, int single)
+{
+    if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1) return 0;
+    return attn_layout(tokens, kv_heads, head_dim, attn_large(tokens, heads / kv_heads, single != 0)).total;
+}
+
+template <int D>
+static void launch_attention(const PagedAttnParams& p, bool large, int64_t blocks, hipStream_t s)
+{
+    if (large) hipLaunchKernelGGL((paged_attention_kernel<D, true>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
+    else hipLaunchKernelGGL((paged_attention_kernel<D, false>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
+    hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.b.tokens, p.b.kv_heads), dim3(kJoinThreads), 0, s, p);
+}
+
+extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens,
+                                  int heads, int window, int sinks, float* output, void* workspace, void* stream)
+{
+    PagedAttnParams p;
+    const int err = paged_check(cache, query, starts, tokens, heads, output, &p.b);
+    if (err) return err;
+    if (window < 0 || sinks < 0 || !workspace) return HQ_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return HQ_ERR_ALIGN;
+    if (tokens == 0) return HQ_OK;
+    p.query = query;
+    p.out = output;
+    p.window = window;
+    p.sinks = sinks;
+    p.tile_tokens = kTileRows / p.b.groups;
+    const bool large = attn_large(tokens, p.b.groups, starts == nullptr);
+    const AttnLayout L = attn_layout(tokens, p.b.kv_heads, cache->head_dim, large);
+    char* ws = static_cast<char*>(workspace);
+    p.part_rows = L.part_rows;
+    p.ordered = reinterpret_cast<int32_t*>(ws);
+    p.desc = reinterpret_cast<int2*>(ws + L.desc);
+    p.part_ml = reinterpret_cast<float2*>(ws + L.ml);
+    p.part_o = reinterpret_cast<float*>(ws + L.o);
+    // at most kTarget pieces and one a tile and kv head; a block without one ends at once
+    const int64_t tiles = int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences);
+    const int64_t blocks = kTarget + tiles * p.b.kv_heads;
+    if (blocks > 0x7fffffff) return HQ_ERR_ARG;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (cache->head_dim) {
+    case 16: launch_attention<16>(p, large, blocks, s); break;
+    case 32: launch_attention<32>(p, large, blocks, s); break;
+    case 64: launch_attention<64>(p, large, blocks, s); break;
+    default: launch_attention<128>(p, large, blocks, s); break;
+    }
+    return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
+}

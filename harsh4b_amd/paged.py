@@ -176,8 +176,8 @@ def paged_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace_bytes(tokens: int, sequences: int, heads: int, kv_heads: int, head_dim: int) -> int:
-    return _native.lib().hq_paged_attention_workspace_bytes(tokens, sequences, heads, kv_heads, head_dim)
+def _attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head_dim: int, single: bool) -> int:
+    return _native.lib().hq_paged_attention_workspace_bytes(tokens, heads, kv_heads, head_dim, single)
 
 
 def paged_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
@@ -209,7 +209,7 @@ def paged_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tenso
     lib = _native.lib()
     _launch(lambda ws, s: lib.hq_paged_attention(
         ctypes.byref(cache), query.data_ptr(), first, tokens, heads, window, sinks, out.data_ptr(), ws, s),
-        _attention_workspace_bytes(tokens, cache.sequences, heads, kv, d), device, stream,
+        _attention_workspace_bytes(tokens, heads, kv, d, starts is None), device, stream,
         (query, keys, values, table, lengths, starts, out), "hq_paged_attention")
     return out
 

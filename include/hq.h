@@ -260,9 +260,9 @@ int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* star
  * A row that sees nothing gets zeros; rows of no sequence are not touched.
  * Values at positions past a sequence's length are never used, whatever they
  * hold.  status may be NULL.  `workspace`:
- * hq_paged_attention_workspace_bytes(...) bytes, 256-byte aligned, of any
- * contents. */
-size_t hq_paged_attention_workspace_bytes(int tokens, int sequences, int heads, int kv_heads, int head_dim);
+ * hq_paged_attention_workspace_bytes(...) bytes (single: nonzero where starts
+ * is NULL), 256-byte aligned, of any contents. */
+size_t hq_paged_attention_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim, int single);
 int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens, int heads,
                        int window, int sinks, float* output, void* workspace, void* stream);
 

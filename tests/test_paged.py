@@ -89,8 +89,8 @@ def test_c_entries_refuse_bad_arguments():
         assert lib.hq_pages_compact(ctypes.byref(u), None, p, None) == 2
     assert lib.hq_pages_resize(c, None, 0, 0, p, None) == 1 and lib.hq_pages_resize(c, p, -1, 0, p, None) == 1
     assert lib.hq_pages_resize(c, p, 0, 0, p + 64, None) == 2 and lib.hq_pages_fork(c, p, p + 4, None) == 2
-    assert lib.hq_paged_attention_workspace_bytes(3, 0, 4, 2, 32) == 0
-    assert lib.hq_paged_attention_workspace_bytes(3, 3, 4, 2, 32) > 0
+    assert lib.hq_paged_attention_workspace_bytes(3, 5, 2, 32, 0) == 0
+    assert lib.hq_paged_attention_workspace_bytes(3, 4, 2, 32, 1) > 0
     # the plan's lists: two of a page or sequence, three of a page, three ints a copy, the table and the lengths
     assert lib.hq_pages_workspace_bytes(c) >= 4 * (2 * 8 + 3 * 8 + 3 * 3 + 12 + 3)
 
