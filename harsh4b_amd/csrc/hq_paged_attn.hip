@@ -26,8 +26,8 @@
 //          4 waves on its own 32 keys, K and V straight to registers, the
 //          waves' parts joined in LDS.  Bound by HBM.
 //   large  128 rows, 32 a wave: 32x32x16 products over chunks of 64 keys that
-//          the block stages in LDS (K by direct copies, V transposed on the
-//          way), two buffers.  Bound by the matrix cores.
+//          the block copies straight to LDS (V is transposed by the reads),
+//          two buffers.  Bound by the matrix cores.
 //
 // Work: a tile's chunks are cut into pieces of about T = all work / kTarget
 // chunks (per sequence: the same number of pieces for all its tiles), each a
@@ -40,6 +40,8 @@
 // (an infinity or NaN in K or V, seen by it or by another row of the tile),
 // the row is computed again by paged_row, in fp32 from the visible positions
 // alone.
+#include <algorithm>
+
 #include "hq_device.h"
 #include "hq_internal.h"
 #include "hq_paged.h"
@@ -56,7 +58,14 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int kChunkKeys = 64;
 constexpr int kSmallRows = 16;
 constexpr int kTileRows = 128;
-constexpr int kTarget = 1024;          // pieces aimed at
+#ifndef TSMALL
+#define TSMALL 512
+#endif
+#ifndef TLARGE
+#define TLARGE 512
+#endif
+constexpr int kTargetSmall = TSMALL;     // pieces aimed at: batches of small tiles only
+constexpr int kTargetLarge = TLARGE;      // others
 constexpr int kSmallMin = 2;           // fewest chunks of a small piece: a step of 32 keys a wave
 constexpr int kLargeMin = 4;
 constexpr int kJoinThreads = 512;
@@ -67,6 +76,7 @@ struct PagedAttnParams {
     float* out;
     int window, sinks;           // window 0: none
     int tile_tokens;             // tokens of a large tile
+    int target;                  // pieces aimed at
     int part_rows;               // rows of partial results there is room for
     int32_t* ordered;            // [1] starts never fall
     int2* desc;                  // [tokens, kv_heads] 2 * pieces + small, first partial row
@@ -82,6 +92,9 @@ __device__ __forceinline__ bool paged_visible(int pos, int j, int window, int si
 
 constexpr float kLog2e = 0x1.715476p+0f;
 constexpr float kWeightScale = 16384.0f;           // 2^14
+// Large tiles keep an old maximum until a score passes it by 2^8: their
+// weights are 2^6 e^(s-m), up to 2^14.
+constexpr float kLargeShift = 6.0f, kLargeScale = 64.0f, kLargeSlack = 8.0f;
 
 // ------------------------------------------------------------- one row, fp32
 // One query row over positions [lo, hi) of sequence b, kv head h, in one wave:
@@ -200,11 +213,24 @@ struct Piece {
     __device__ __forceinline__ int position(int i) const { return int(max(origin + i, int64_t(-1))); }
 };
 
-__device__ __forceinline__ int64_t wave_sum_i64(int64_t v)
+// Inclusive prefix sum over the wave (every lane active): row shifts, then the
+// row totals broadcast to the rows above.
+__device__ __forceinline__ int wave_prefix(int v)
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor((long long)v, o, kWave);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast 31 into rows 2 and 3
     return v;
+}
+
+// Pieces a sequence's tiles are cut in for pieces of about `target` chunks.
+__device__ __forceinline__ int cuts_of(const SequencePlan& s, int target)
+{
+    const int size = max(target, s.small ? kSmallMin : kLargeMin);
+    return max(1, int(float(s.chunks) / float(size) + 0.5f));
 }
 
 // The work of block `q`, the same in every wave; false: none.
@@ -223,41 +249,43 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     const bool ordered = !__any(fall);
     if (q == 0 && threadIdx.x == 0) *p.ordered = ordered;
     if (!ordered) return false;
-    units = wave_sum_i64(units) * p.b.kv_heads;
-    const int target = int(min((units + kTarget - 1) / kTarget, int64_t(0x40000000)));
-    int64_t pieces = 0, rows = 0;
+    // (the sum of 64 in two parts that fit an int each)
+    const int low = __builtin_amdgcn_readfirstlane(wave_isum64(int(units & 0xFFFFFF)));
+    const int high = __builtin_amdgcn_readfirstlane(wave_isum64(int(min(units >> 24, int64_t(0xFFFFFF)))));
+    units = ((int64_t(high) << 24) + low) * p.b.kv_heads;
+    const int target = int(min((units + p.target - 1) / p.target, int64_t(0x40000000)));
+    int pieces = 0, rows = 0;
     for (int base = 0; base < p.b.sequences; base += kWave) {
         const bool in = base + lane < p.b.sequences;
         if (p.b.sequences > kWave && in) mine = sequence_plan(p, base + lane, &fall);
         if (!in) mine.tiles = 0;
-        const int most = max(target, mine.small ? kSmallMin : kLargeMin);
-        const int cuts = max(1, (mine.chunks + most - 1) / most);
-        const int64_t here = int64_t(mine.tiles) * cuts * p.b.kv_heads;
-        const int64_t part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
-        int64_t incl = here, part_incl = part;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int64_t y = __shfl_up((long long)incl, o, kWave), z = __shfl_up((long long)part_incl, o, kWave);
-            if (lane >= o) {
-                incl += y;
-                part_incl += z;
-            }
-        }
+        const int cuts = cuts_of(mine, target);
+        const int here = mine.tiles * cuts * p.b.kv_heads;
+        const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
+        const int incl = wave_prefix(here), part_incl = wave_prefix(part);
         const uint64_t found = __ballot(q >= pieces + incl - here && q < pieces + incl);
         if (found) {
             const int src = __builtin_ctzll(found);
             auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
-            const int local = from(int(q - (pieces + incl - here)));
-            const int first_part = from(int(rows + part_incl - part));
+            const int local = q - from(pieces + incl - here);
+            const int first_part = from(rows + part_incl - part);
             out.pieces = from(cuts);
             out.small = from(mine.small);
             out.length = from(mine.length);
             const int n = from(mine.n), tokens = from(mine.tile_tokens), tiles = from(mine.tiles);
             out.b = base + src;
-            out.head = local % p.b.kv_heads;
-            const int rest = local / p.b.kv_heads;
-            out.split = rest % out.pieces;
-            const int tile = tiles - 1 - rest / out.pieces;      // the longest first
+            int rest, tile;
+            if (out.small) {                                         // (one tile)
+                rest = unsigned(local) / unsigned(p.b.kv_heads);
+                out.split = rest;
+                tile = 0;
+            } else {
+                rest = unsigned(local) / unsigned(p.b.kv_heads);
+                const int done = unsigned(rest) / unsigned(out.pieces);
+                out.split = rest - done * out.pieces;
+                tile = tiles - 1 - done;                             // the longest first
+            }
+            out.head = local - rest * p.b.kv_heads;
             out.first = from(mine.first) + tile * tokens;
             out.n = min(tokens, n - tile * tokens);
             out.origin = int64_t(out.length) - n + tile * tokens;
@@ -266,8 +294,8 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
                                         (out.small ? kSmallRows : kTileRows);
             return true;
         }
-        pieces += __shfl((long long)incl, kWave - 1, kWave);
-        rows += __shfl((long long)part_incl, kWave - 1, kWave);
+        pieces += __builtin_amdgcn_readlane(incl, kWave - 1);
+        rows += __builtin_amdgcn_readlane(part_incl, kWave - 1);
     }
     return false;
 }
@@ -296,17 +324,17 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // Weights p (of up to 2^14) as hi + lo.
 __device__ __forceinline__ void split_weights(const float (&w)[8], half8& hi, half8& lo)
 {
+    uint4v a, b;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const float2v x = {w[i], w[i + 1]};
+    for (int i = 0; i < 4; ++i) {
+        const float2v x = {w[2 * i], w[2 * i + 1]};
         const half2v h = __builtin_convertvector(x, half2v);
-        const float2v r = {w[i] - float(h[0]), w[i + 1] - float(h[1])};
-        const half2v g = __builtin_convertvector(r, half2v);
-        hi[i] = h[0];
-        hi[i + 1] = h[1];
-        lo[i] = g[0];
-        lo[i + 1] = g[1];
+        const float2v rest = {x[0] - float(h[0]), x[1] - float(h[1])};
+        a[i] = __builtin_bit_cast(uint32_t, h);
+        b[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, half2v));
     }
+    hi = __builtin_bit_cast(half8, a);
+    lo = __builtin_bit_cast(half8, b);
 }
 
 __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
@@ -351,7 +379,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
 {
     constexpr int STEPS = (D + 31) / 32;       // products over the dims
     constexpr int VEC = D / 16;                // dims a lane holds of a V row
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n = lane & 15, g = lane >> 4;
     const int G = p.b.groups;
     const int rows = w.n * G;
@@ -573,15 +601,20 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
 // ---------------------------------------------------------------- large tiles
 template <int D>
 struct LargeShared {
-    static constexpr int VROWS = D < 32 ? 32 : D;
-    alignas(16) uint16_t k[2][kChunkKeys * D];         // [key][dim], 16-byte pieces of a row permuted by the key
-    alignas(16) uint16_t v[2][VROWS * kChunkKeys];     // [dim][key], keys in the products' order
+    // [key][dim], the 16-byte pieces of a row permuted by the key: piece i of K in place i ^ (key & 15), of V in
+    // i ^ 2 (key & 7) (both within the row), so that the rows a product reads together lie in different banks
+    alignas(256) uint16_t k[2][kChunkKeys * D];
+    alignas(256) uint16_t v[2][kChunkKeys * D];
 };
 
-// Permutation of the 16-byte pieces of V^T row `dim` in LDS: 16 rows that a
-// product reads together lie in 16 different places of the 64 banks, and the
-// writes of 4-row groups in 8 of 16.
-__device__ __forceinline__ int v_swizzle(int dim) { return ((dim >> 1) ^ (dim >> 3)) & 7; }
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// Four keys of one dim a lane from V rows in LDS: lane i of 16 gives the
+// address of row i / 4, dims 4 (i % 4) .. + 3 and receives dim i of the four.
+__device__ __forceinline__ short4v read_transposed(uint32_t lds)
+{
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(uintptr_t(lds)));
+}
 
 template <int D>
 __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span& span, int c0, int c1,
@@ -590,7 +623,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     constexpr int STEPS = D / 16;
     constexpr int DT = D < 32 ? 1 : D / 32;
     constexpr int PIECES = D / 8;              // 16-byte pieces of a K row
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n = lane & 31, g = lane >> 5;
     const int G = p.b.groups;
     const int ps = p.b.page_size;
@@ -623,6 +656,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
     }
     const int pos = w.position(token);
+    const int low = p.window > 0 ? max(0, pos - p.window + 1) : 0;     // first position of the row's window
     const bool active = 32 * wave < rows;      // (wave-uniform)
     const int pos_min = w.position(min(32 * wave, rows - 1) / G);
     const int pos_max = w.position(min(32 * wave + 31, rows - 1) / G);
@@ -632,161 +666,229 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int k = 0; k < 16; ++k) acc[i][k] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f, shift = kLargeShift;
     bool seen = false;
 
     const size_t head_stride = size_t(ps) * D;
     auto base_of = [&](int page, int j) {
         return (size_t(max(page, 0)) * p.b.kv_heads + w.head) * head_stride + size_t(j & (ps - 1)) * D;
     };
-    // pages of 16 chunks at a time, 4 parts of 16 keys each, in a register
+    // pages of 16 chunks at a time, 4 parts of 16 keys each, in a register:
+    // of chunks pg_first ..; a chunk's are taken when its values are fetched
+    int pg = -1, pg_first = c0;
     auto pages_of = [&](int cc) {
         const int at = cc + (lane >> 2);
         return at < c1 ? paged_page(p.b, w.b, span.chunk(at) * kChunkKeys + 16 * (lane & 3)) : -1;
     };
-    // V on its way to LDS: thread (piece pc of 8 keys, 4 dims)
-    const int pc = threadIdx.x / (D / 4), dg = threadIdx.x % (D / 4);
-    const bool stages = pc < 8;
-    uint2 vr[8];
-    auto fetch = [&](int pg, int first, int cc) {
-        const int j0 = span.chunk(cc) * kChunkKeys;
-        const int lane0 = 4 * (cc - first);
-        const int sub = pc >> 1;
-        const int vpage = __shfl(pg, lane0 + (sub & 3), kWave);   // (every lane takes part)
-        if (stages) {
-            const int page = vpage;
-            const uint16_t* v = p.b.values + base_of(page, j0 + 16 * sub) + 4 * dg;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                vr[i] = *reinterpret_cast<const uint2*>(v + (8 * (i >> 2) + 4 * (pc & 1) + (i & 3)) * D);
-            if (page < 0 || j0 + kChunkKeys > w.length) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = j0 + 16 * sub + 8 * (i >> 2) + 4 * (pc & 1) + (i & 3);
-                    if (page < 0 || j >= w.length) vr[i] = make_uint2(0, 0);
-                }
-            }
-        }
-        // K rows 16 wave .. + 15, contiguous in their page
-        const int page = __builtin_amdgcn_readlane(pg, lane0 + wave);
-        const uint16_t* k = p.b.keys + base_of(page, j0 + 16 * wave);
+    auto opaque = [](uint32_t v) {             // (the compiler would keep everything made from it in registers)
+        asm volatile("" : "+v"(v));
+        return v;
+    };
+    // Rows 16 wave .. + 15 of chunk cc, contiguous in their page, to LDS: copy
+    // i takes PER rows, lane (row, place) the piece that belongs in that place.
+    // The permutations work bit by bit, so copy i's piece is copy 0's with
+    // bits of the row 16 i / COPIES flipped.
+    constexpr int PER = 64 / PIECES < 16 ? 64 / PIECES : 16, COPIES = 16 / PER;
+    const int copy_row = lane / PIECES, place = lane % PIECES;
+    const uint32_t k_copy = uint32_t(copy_row * PIECES + (place ^ (copy_row & (PIECES - 1)))) * 16;
+    const uint32_t v_copy = uint32_t(copy_row * PIECES + (place ^ ((2 * copy_row) & (PIECES - 1)))) * 16;
+    auto copy_k = [&](int page, int cc) {
+        const uint16_t* k = p.b.keys + base_of(page, span.chunk(cc) * kChunkKeys + 16 * wave);
         const uint32_t to = lds_addr(&S.k[cc & 1][16 * wave * D]);
+        const uint32_t from = opaque(k_copy);
 #pragma unroll
-        for (int i = 0; i < (PIECES + 3) / 4; ++i) {
-            const int u = 64 * i + lane;
-            const int row = u / PIECES, at = u % PIECES;
-            const uint32_t off = uint32_t(row * PIECES + (at ^ (row & (PIECES - 1)))) * 16;
-            if (D >= 32 || lane < 16 * PIECES) dma16(k, off, to + 1024 * i);
+        for (int i = 0; i < COPIES; ++i)
+            if (D >= 32 || copy_row < 16)
+                dma16(k, (from ^ (16 * ((i * PER) & (PIECES - 1)))) + 1024 * i, to + 1024 * i);
+    };
+    auto copy_v = [&](int page, int cc) {
+        const int j0 = span.chunk(cc) * kChunkKeys + 16 * wave;
+        const uint16_t* v = p.b.values + base_of(page, j0);
+        uint16_t* to = &S.v[cc & 1][16 * wave * D];
+        const int there = page < 0 ? 0 : min(w.length - j0, 16);         // rows; the others are zeros
+        const uint32_t from = opaque(v_copy);
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            if (D < 32 && copy_row >= 16) continue;
+            if (copy_row < there - i * PER)
+                dma16(v, (from ^ (16 * ((2 * i * PER) & (PIECES - 1)))) + 1024 * i, lds_addr(to) + 1024 * i);
+            else
+                *reinterpret_cast<uint4v*>(to + 512 * i + 8 * lane) = uint4v{0, 0, 0, 0};
         }
     };
-    auto store_v = [&](int buf) {
-        if (!stages) return;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            uint4v x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a = d < 2 ? vr[2 * i].x : vr[2 * i].y, b = d < 2 ? vr[2 * i + 1].x : vr[2 * i + 1].y;
-                x[i] = __builtin_amdgcn_perm(b, a, (d & 1) ? 0x07060302u : 0x05040100u);
-            }
-            const int dim = 4 * dg + d;
-            *reinterpret_cast<uint4v*>(&S.v[buf][dim * kChunkKeys + (pc ^ v_swizzle(dim)) * 8]) = x;
-        }
+    // Operands from LDS: unit i of the scores of half t (dims 16 i ..), unit i
+    // of the products with V of half t (16 keys and 32 dims).  The addresses
+    // are a lane's base with bits of the piece flipped; the bases are made
+    // anew for every step (opaque to the compiler, which would keep all of
+    // them in registers).
+    typedef __attribute__((address_space(3))) const half8* lds_half8;
+    constexpr uint32_t kBufBytes = kChunkKeys * D * 2;
+    const int lane16 = lane & 15;
+    const uint32_t k_lane = lds_addr(&S.k[0][0]) + n * 2 * D + ((g ^ (n & (PIECES - 1))) & (PIECES - 1)) * 16;
+    const int v_key = 4 * g + (lane16 >> 2);
+    const uint32_t v_lane = lds_addr(&S.v[0][0]) + v_key * 2 * D + 8 * (lane16 & 1) +
+                            (((2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ (2 * v_key)) & (PIECES - 1)) * 16;
+    auto k_unit = [&](uint32_t base, int i) { return *lds_half8(uintptr_t(base ^ (32 * i))); };
+    auto v_unit = [&](uint32_t base, int i) {
+        const uint32_t at = (base ^ ((64 * (i % DT)) & (2 * D - 1))) + (i / DT) * 32 * D;
+        // (the rows 8 keys on have the same permutation)
+        struct { short4v a, b; } both = {read_transposed(at), read_transposed(at + 16 * D)};
+        return __builtin_bit_cast(half8, both);
     };
-    int pg = pages_of(c0), pg_first = c0;
-    if (c0 < c1) {
-        fetch(pg, pg_first, c0);
-        store_v(c0 & 1);
-    }
-    wait_all_memory();
-    __syncthreads();
-    for (int cc = c0; cc < c1; ++cc) {
-        const int buf = cc & 1;
-        const int j0 = span.chunk(cc) * kChunkKeys;
-        const uint32_t there = uint32_t(__ballot(pg >= 0) >> (4 * (cc - pg_first))) & 15u;   // parts with a page
-        if (cc + 1 < c1) {
-            if (cc + 1 - pg_first == 16) {
-                pg_first = cc + 1;
-                pg = pages_of(pg_first);
-            }
-            fetch(pg, pg_first, cc + 1);
+    struct Weights {
+        uint4v hi[2], lo[2];                   // [16 keys], two fp16 a word
+    };
+    // The weights `now` of the scores `cur` side by side with the scores
+    // `next` of half kt in K buffer kbuf (matrix instructions of one and the
+    // arithmetic of the other overlap only where they alternate in the
+    // program), then O += V P of half vt in buffer vbuf.  Lane (n, g) of the
+    // scores: row n, keys 32 t + 8 (i / 4) + 4 g + i % 4.
+    constexpr int VUNITS = 2 * DT;
+    auto weigh = [&](const float16v& cur, int pair, Weights& now) {
+        const int at = 2 * pair;
+        const float2v e = {exp2_fast(__builtin_fmaf(cur[at], c, shift)),
+                           exp2_fast(__builtin_fmaf(cur[at + 1], c, shift))};
+        l += e[0];
+        l += e[1];
+        const half2v h = __builtin_convertvector(e, half2v);
+        const float2v rest = {e[0] - float(h[0]), e[1] - float(h[1])};
+        const half2v f = __builtin_convertvector(rest, half2v);
+        now.hi[at / 8][at % 8 / 2] = __builtin_bit_cast(uint32_t, h);
+        now.lo[at / 8][at % 8 / 2] = __builtin_bit_cast(uint32_t, f);
+    };
+    auto step = [&](auto with_scores, int kbuf, int kt, float16v& next, auto with_weights, const float16v& cur,
+                    int vbuf, int vt) {
+        constexpr bool SC = decltype(with_scores)::value, WE = decltype(with_weights)::value;
+        constexpr int UNITS = SC ? STEPS : 1;
+        constexpr int PAIRS = 8 / UNITS;
+        Weights now{};
+        half8 ka{};
+        uint32_t kb = 0;
+        if constexpr (SC) {
+            kb = opaque(k_lane + kbuf * kBufBytes + kt * 64 * D);
+            ka = k_unit(kb, 0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) next[i] = 0.0f;
         }
-        const bool work = active && j0 <= pos_max;
-        float16v s[2];
-        half8 hi[4], lo[4];
-        if (work) {
+        unrolled<UNITS>([&](auto u) {
+            constexpr int i = decltype(u)::value;
+            const half8 k = ka;
+            if constexpr (SC) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (SC && i + 1 < UNITS) ka = k_unit(kb, i + 1);
+            if constexpr (SC) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], next, 0, 0, 0);
+            if constexpr (WE)
+                unrolled<PAIRS>([&](auto q) {
+                    if constexpr (2 * decltype(q)::value < PAIRS) weigh(cur, i * PAIRS + decltype(q)::value, now);
+                });
+            if constexpr (SC) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qhi[i], next, 0, 0, 0);
+            if constexpr (WE)
+                unrolled<PAIRS>([&](auto q) {
+                    if constexpr (2 * decltype(q)::value >= PAIRS) weigh(cur, i * PAIRS + decltype(q)::value, now);
+                });
+        });
+        if constexpr (WE) {
+            const uint32_t vb = opaque(v_lane + vbuf * kBufBytes + vt * 64 * D);
+            half8 va = v_unit(vb, 0);
+            unrolled<VUNITS>([&](auto u) {
+                constexpr int i = decltype(u)::value;
+                const half8 v = va;
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (i + 1 < VUNITS) va = v_unit(vb, i + 1);
+                acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8, now.lo[i / DT]), acc[i % DT], 0, 0, 0);
+                acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8, now.hi[i / DT]), acc[i % DT], 0, 0, 0);
+            });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    // masks, and a new maximum where the old one is left too far behind
+    auto settle = [&](int cc, int t, uint32_t there, float16v& s) {
+        const int j0 = span.chunk(cc) * kChunkKeys + 32 * t;
+        const uint32_t both = (there >> (2 * t)) & 3u;
+        const bool all = both == 3u && j0 + 31 <= pos_min &&
+                         (p.window == 0 || j0 > pos_max - p.window || j0 + 32 <= p.sinks);
+        if (!all) {
+            // of the lane's first key; its others lie 8 (i / 4) + i % 4 further
+            const int to_pos = int(opaque(pos - j0 - 4 * g)), to_low = int(opaque(low - j0 - 4 * g));
+            const int to_sinks = int(opaque(p.sinks - j0 - 4 * g));
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
-                const int key = 32 * t + n;
-#pragma unroll
-                for (int d = 0; d < STEPS; ++d) {
-                    const half8 a = *reinterpret_cast<const half8*>(
-                        &S.k[buf][key * D + ((2 * d + g) ^ (key & (PIECES - 1))) * 8]);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qlo[d], s[t], 0, 0, 0);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qhi[d], s[t], 0, 0, 0);
-                }
+            for (int i = 0; i < 16; ++i) {
+                const int at = 8 * (i >> 2) + (i & 3);
+                const bool visible = ((both >> (i >> 3)) & 1u) & (at <= to_pos) & ((at >= to_low) | (at < to_sinks));
+                s[i] = visible ? s[i] : -__builtin_inff();
+                seen |= visible;
             }
-            // lane (n, g): row n, keys j0 + 32 t + 8 (i / 4) + 4 g + i % 4
-            const bool all = there == 15u && j0 + kChunkKeys - 1 <= pos_min &&
-                             (p.window == 0 || j0 > pos_max - p.window || j0 + kChunkKeys <= p.sinks);
-            if (!all) {
+        } else {
+            seen = true;
+        }
+        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int at = 32 * t + 8 * (i >> 2) + 4 * g + (i & 3);
-                        const bool visible = ((there >> (2 * t + (i >> 3))) & 1) &&
-                                             paged_visible(pos, j0 + at, p.window, p.sinks);
-                        s[t][i] = visible ? s[t][i] : -__builtin_inff();
-                        seen |= visible;
-                    }
-            } else {
-                seen = true;
-            }
-            float top = s[0][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+        top = fmaxf(top, s[15]);
+        unsigned a = __builtin_bit_cast(unsigned, top), b = a;
+        swap32(a, b);
+        top = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+        // (m = -inf: the first that is seen; both -inf: NaN, not taken)
+        if (__any((top - m) * c > kLargeSlack)) {
             top = fmaxf(m, top);
             const float safe = top == -__builtin_inff() ? 0.0f : top;
-            if (__any(top > m)) {
-                const float alpha = exp2_fast((m - safe) * c);
-                l *= alpha;
+            const float alpha = exp2_fast((m - safe) * c);
+            l *= alpha;
 #pragma unroll
-                for (int i = 0; i < DT; ++i) acc[i] *= alpha;
-                m = top;
-            }
-            const float shift = 14.0f - safe * c;
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = exp2_fast(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, shift));
-                    l += e[i];
-                }
-                split_weights(e, hi[st], lo[st]);
-            }
+            for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+            m = top;
+            shift = kLargeShift - safe * c;
         }
-        if (cc + 1 < c1) store_v(buf ^ 1);
-        if (work) {
-#pragma unroll
-            for (int st = 0; st < 4; ++st)
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const int dim = 32 * dt + n;
-                    const half8 a = *reinterpret_cast<const half8*>(
-                        &S.v[buf][dim * kChunkKeys + ((2 * st + g) ^ v_swizzle(dim)) * 8]);
-                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, lo[st], acc[dt], 0, 0, 0);
-                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, hi[st], acc[dt], 0, 0, 0);
-                }
-        }
+    };
+    auto there_of = [&](int cc) { return uint32_t(__ballot(pg >= 0) >> (4 * (cc - pg_first))) & 15u; };
+
+    if (c0 < c1) {
+        // The scores run half a chunk (32 keys) ahead of the weights.  Two
+        // barriers a chunk: one lets K of chunk cc + 2 take cc's place, one V.
+        pg = pages_of(c0);
+        uint32_t there = there_of(c0);
+        int page = __builtin_amdgcn_readlane(pg, wave);        // of chunk c0, then of cc + 1
+        copy_k(page, c0);
+        copy_v(page, c0);
+        page = __builtin_amdgcn_readlane(pg, 4 + wave);
+        if (c0 + 1 < c1) copy_k(page, c0 + 1);
         wait_all_memory();
-        __syncthreads();
+        lds_sync();
+        float16v sa{}, sb{};
+        if (active) {
+            step(yes, c0 & 1, 0, sa, no, sb, 0, 0);
+            settle(c0, 0, there, sa);
+        }
+        for (int cc = c0;; ++cc) {
+            // here: sa the scores of cc's first half; K of cc and cc + 1, V of cc in LDS
+            const bool more = cc + 1 < c1;
+            if (more) copy_v(page, cc + 1);
+            if (active) {
+                step(yes, cc & 1, 1, sb, yes, sa, cc & 1, 0);
+                settle(cc, 1, there, sb);
+            }
+            if (!more) {
+                if (active) step(no, 0, 0, sa, yes, sb, cc & 1, 1);
+                break;
+            }
+            lds_sync();
+            there = there_of(cc + 1);
+            if (cc + 2 < c1) {
+                if (cc + 2 - pg_first == 16) {
+                    pg_first = cc + 2;
+                    pg = pages_of(pg_first);
+                }
+                page = __builtin_amdgcn_readlane(pg, 4 * (cc + 2 - pg_first) + wave);
+                copy_k(page, cc + 2);
+            }
+            if (active) {
+                step(yes, (cc + 1) & 1, 0, sa, yes, sb, cc & 1, 1);
+                settle(cc + 1, 0, there, sa);
+            }
+            wait_all_memory();
+            lds_sync();
+        }
     }
     l += __shfl_xor(l, 32, kWave);
     // lane (n, g): row n, dims 32 dt + 8 (i / 4) + 4 g + i % 4
@@ -803,7 +905,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     if (mine && ((again >> n) & 1) == 0) {
         const bool direct = w.pieces == 1;
         float* to = direct ? p.out + out_row * D : p.part_o + size_t(w.part + r) * D;
-        const float f = none ? 0.0f : direct ? 1.0f / l : 1.0f / kWeightScale;
+        const float f = none ? 0.0f : direct ? 1.0f / l : 1.0f / kLargeScale;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -818,7 +920,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             }
         if (!direct && g == 0)
             p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f)
-                                         : make_float2(m * c, l * (1.0f / kWeightScale));
+                                         : make_float2(m * c, l * (1.0f / kLargeScale));
     }
     for (uint32_t left = again; left; left &= left - 1)
         redo_row<D>(p, w, span, c0, c1, 32 * wave + __builtin_ctz(left));
@@ -861,10 +963,10 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 {
     __shared__ float so[kJoinThreads][2], sl[kJoinThreads], sm[kJoinThreads];
     const int t = blockIdx.x, h = blockIdx.y;
-    if (*p.ordered == 0) return;
+    const int2 d = p.desc[size_t(t) * p.b.kv_heads + h];   // (of any contents where the row is nobody's)
+    const int ordered = *p.ordered;
     int first = 0, count = 0;
-    if (paged_sequence(p.b, t, &first, &count) < 0) return;
-    const int2 d = p.desc[size_t(t) * p.b.kv_heads + h];
+    if (paged_sequence(p.b, t, &first, &count) < 0 || ordered == 0) return;
     const int pieces = d.x >> 1, stride = (d.x & 1) ? kSmallRows : kTileRows;
     if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) return;
     const int pairs = p.b.groups * D / 2;                 // at most 512
@@ -921,14 +1023,14 @@ struct AttnLayout {
     int part_rows;
 };
 
-// Rows of partial results: a sequence cut in S > 1 pieces a tile has more
-// than T chunks a tile, so S < 2 chunks / T, and over all of them fewer than
-// 2 work / T <= 2 kTarget pieces.
+// Rows of partial results: pieces are of T >= work / target chunks, and a
+// sequence of S > 1 pieces a tile has at least 1.5 T chunks a tile, so S <=
+// chunks / T + 1/2 < 2 chunks / T, and over all of them fewer than 2 target.
 static AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large)
 {
     AttnLayout L;
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
-    L.part_rows = 2 * kTarget * (large ? kTileRows : kSmallRows);
+    L.part_rows = large ? 2 * kTargetLarge * kTileRows : 2 * kTargetSmall * kSmallRows;
     L.desc = 256;
     L.ml = L.desc + up(size_t(tokens) * kv_heads * sizeof(int2));
     L.o = L.ml + up(size_t(L.part_rows) * sizeof(float2));
@@ -979,9 +1081,14 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     p.desc = reinterpret_cast<int2*>(ws + L.desc);
     p.part_ml = reinterpret_cast<float2*>(ws + L.ml);
     p.part_o = reinterpret_cast<float*>(ws + L.o);
-    // at most kTarget pieces and one a tile and kv head; a block without one ends at once
-    const int64_t tiles = int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences);
-    const int64_t blocks = kTarget + tiles * p.b.kv_heads;
+    p.target = large ? kTargetLarge : kTargetSmall;
+    // chunks / T + 1 pieces a tile and kv head at most, so `target` and one of each in all; nor more than the
+    // table's width allows.  A block without a piece ends at once.
+    const int64_t tiles = large ? int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences)
+                                : std::min(tokens, p.b.sequences);
+    const int64_t widest = (int64_t(cache->max_pages) * cache->page_size + kChunkKeys - 1) / kChunkKeys;
+    const int64_t blocks = std::min(p.target + tiles * p.b.kv_heads,
+                                    tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
     if (blocks > 0x7fffffff) return HQ_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {
