@@ -61,6 +61,12 @@ constexpr int kTileRows = 128;
 #ifndef TSMALL
 #define TSMALL 512
 #endif
+#ifndef KAHEAD
+#define KAHEAD 1
+#endif
+#ifndef VAHEAD
+#define VAHEAD 3
+#endif
 #ifndef TLARGE
 #define TLARGE 512
 #endif
@@ -321,6 +327,21 @@ __device__ __forceinline__ int row_exponent(float top)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// What an fp16 pair leaves of the two values it was rounded from: a - h.lo and
+// b - h.hi, one v_fma_mix_f32 each (it reads an fp16 half; the compiler makes
+// a conversion and a subtraction).
+__device__ __forceinline__ float2v residual(float a, float b, half2v h)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, h);
+    float2v r;
+    float x, y;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x) : "v"(u), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y) : "v"(u), "v"(b));
+    r[0] = x;
+    r[1] = y;
+    return r;
+}
+
 // Weights p (of up to 2^14) as hi + lo.
 __device__ __forceinline__ void split_weights(const float (&w)[8], half8& hi, half8& lo)
 {
@@ -329,7 +350,7 @@ __device__ __forceinline__ void split_weights(const float (&w)[8], half8& hi, ha
     for (int i = 0; i < 4; ++i) {
         const float2v x = {w[2 * i], w[2 * i + 1]};
         const half2v h = __builtin_convertvector(x, half2v);
-        const float2v rest = {x[0] - float(h[0]), x[1] - float(h[1])};
+        const float2v rest = residual(x[0], x[1], h);
         a[i] = __builtin_bit_cast(uint32_t, h);
         b[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, half2v));
     }
@@ -750,8 +771,9 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
                            exp2_fast(__builtin_fmaf(cur[at + 1], c, shift))};
         l += e[0];
         l += e[1];
+        asm volatile("" : "+v"(l));            // (summed here: the compiler would keep all of e for later)
         const half2v h = __builtin_convertvector(e, half2v);
-        const float2v rest = {e[0] - float(h[0]), e[1] - float(h[1])};
+        const float2v rest = residual(e[0], e[1], h);
         const half2v f = __builtin_convertvector(rest, half2v);
         now.hi[at / 8][at % 8 / 2] = __builtin_bit_cast(uint32_t, h);
         now.lo[at / 8][at % 8 / 2] = __builtin_bit_cast(uint32_t, f);
@@ -761,20 +783,25 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         constexpr bool SC = decltype(with_scores)::value, WE = decltype(with_weights)::value;
         constexpr int UNITS = SC ? STEPS : 1;
         constexpr int PAIRS = 8 / UNITS;
+        constexpr int AHEAD = KAHEAD, VSET = VAHEAD + 1;
         Weights now{};
-        half8 ka{};
-        uint32_t kb = 0;
+        half8 ka[AHEAD + 1], va[VSET];
+        uint32_t kb = 0, vb = 0;
         if constexpr (SC) {
             kb = opaque(k_lane + kbuf * kBufBytes + kt * 64 * D);
-            ka = k_unit(kb, 0);
+            unrolled<(AHEAD < UNITS ? AHEAD : UNITS)>([&](auto u) { ka[decltype(u)::value] = k_unit(kb, decltype(u)::value); });
 #pragma unroll
             for (int i = 0; i < 16; ++i) next[i] = 0.0f;
         }
         unrolled<UNITS>([&](auto u) {
             constexpr int i = decltype(u)::value;
-            const half8 k = ka;
             if constexpr (SC) __builtin_amdgcn_sched_barrier(0);
-            if constexpr (SC && i + 1 < UNITS) ka = k_unit(kb, i + 1);
+            if constexpr (SC && i + AHEAD < UNITS) ka[(i + AHEAD) % (AHEAD + 1)] = k_unit(kb, i + AHEAD);
+            if constexpr (WE && i == UNITS - 1) {
+                vb = opaque(v_lane + vbuf * kBufBytes + vt * 64 * D);
+                unrolled<(VAHEAD < VUNITS ? VAHEAD : VUNITS)>([&](auto q) { va[decltype(q)::value] = v_unit(vb, decltype(q)::value); });
+            }
+            const half8 k = ka[i % (AHEAD + 1)];
             if constexpr (SC) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], next, 0, 0, 0);
             if constexpr (WE)
                 unrolled<PAIRS>([&](auto q) {
@@ -787,13 +814,11 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 });
         });
         if constexpr (WE) {
-            const uint32_t vb = opaque(v_lane + vbuf * kBufBytes + vt * 64 * D);
-            half8 va = v_unit(vb, 0);
             unrolled<VUNITS>([&](auto u) {
                 constexpr int i = decltype(u)::value;
-                const half8 v = va;
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (i + 1 < VUNITS) va = v_unit(vb, i + 1);
+                if constexpr (i + VAHEAD < VUNITS) va[(i + VAHEAD) % VSET] = v_unit(vb, i + VAHEAD);
+                const half8 v = va[i % VSET];
                 acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8, now.lo[i / DT]), acc[i % DT], 0, 0, 0);
                 acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8, now.hi[i / DT]), acc[i % DT], 0, 0, 0);
             });
