@@ -81,14 +81,14 @@ _SIGNATURES = {
     "hq_gemm_workspace_bytes": ([c_int, c_int, c_int], c_size),
     "hq_int4_i8_gemm": ([vp, vp, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp], c_int),
     "hq_quant_int4_gemm": ([vp, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp, vp, vp], c_int),
-    "hq_pages_workspace_bytes": ([ctypes.POINTER(HqPages)], c_size),
-    "hq_pages_resize": ([ctypes.POINTER(HqPages), vp, c_int, c_int, vp, vp], c_int),
-    "hq_pages_fork": ([ctypes.POINTER(HqPages), vp, vp, vp], c_int),
-    "hq_pages_compact": ([ctypes.POINTER(HqPages), vp, vp, vp], c_int),
-    "hq_paged_append": ([ctypes.POINTER(HqPages), vp, vp, c_int, c_int, vp, vp, c_float, vp, vp, c_int, vp, vp],
+    "hq_pages_workspace_bytes": ([vp], c_size),
+    "hq_pages_resize": ([vp, vp, c_int, c_int, vp, vp], c_int),
+    "hq_pages_fork": ([vp, vp, vp, vp], c_int),
+    "hq_pages_compact": ([vp, vp, vp, vp], c_int),
+    "hq_paged_append": ([vp, vp, vp, c_int, c_int, vp, vp, c_float, vp, vp, c_int, vp, vp],
                         c_int),
     "hq_paged_attention_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int], c_size),
-    "hq_paged_attention": ([ctypes.POINTER(HqPages), vp, vp, c_int, c_int, c_int, c_int, vp, vp, vp], c_int),
+    "hq_paged_attention": ([vp, vp, vp, c_int, c_int, c_int, c_int, vp, vp, vp], c_int),
     "hq_step_layer_blocks": ([ctypes.POINTER(HqModel)], c_int),
     "hq_step_workspace_bytes": ([ctypes.POINTER(HqModel), c_int], c_size),
     "hq_decode_step": ([ctypes.POINTER(HqModel), ctypes.POINTER(HqState), vp], c_int),

@@ -67,6 +67,9 @@ constexpr int kTileRows = 128;
 #ifndef VAHEAD
 #define VAHEAD 3
 #endif
+#ifndef OCC
+#define OCC 2
+#endif
 #ifndef TLARGE
 #define TLARGE 512
 #endif
@@ -168,9 +171,9 @@ struct Span {
 __device__ __forceinline__ Span span_of(const PagedAttnParams& p, int pa, int pb)
 {
     if (pb < 0) return Span{0, 0, 0};
-    const int64_t end = min(int64_t(pb) + 1, int64_t(p.b.max_pages) << p.b.shift);
-    const int last = int((end + kChunkKeys - 1) / kChunkKeys);
-    const int low = p.window > 0 ? int(max(int64_t(0), int64_t(pa) - p.window + 1)) : 0;
+    const int end = min(pb + 1, p.b.max_pages << p.b.shift);
+    const int last = (end - 1) / kChunkKeys + 1;
+    const int low = p.window > 0 && pa >= p.window ? pa - p.window + 1 : 0;
     const int first = low / kChunkKeys;
     const int sunk = min(p.sinks, low);
     const int sink = min(min(first, last), sunk / kChunkKeys + (sunk % kChunkKeys != 0));
@@ -179,13 +182,9 @@ __device__ __forceinline__ Span span_of(const PagedAttnParams& p, int pa, int pb
 
 struct SequencePlan {
     int first, n;                // rows
-    int length;
+    int length;                  // (a negative one counts as 0)
     int tile_tokens, tiles, chunks;   // chunks of the last tile (no other has more)
     bool small;
-    __device__ __forceinline__ int position(int i) const
-    {
-        return int(max(int64_t(length) - n + i, int64_t(-1)));
-    }
 };
 
 __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, int b, bool* fall)
@@ -193,17 +192,20 @@ __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, 
     SequencePlan s;
     s.first = b;
     s.n = 1;
+    s.small = true;
+    s.tile_tokens = s.tiles = 1;
+    s.length = max(0, p.b.lengths[b]);
     if (p.b.starts) {
         const int a = p.b.starts[b], z = p.b.starts[b + 1];
         *fall |= a > z;
         s.first = a;
         s.n = a < 0 || a >= z || z > p.b.tokens ? 0 : z - a;
+        s.small = s.n <= kSmallRows / p.b.groups;
+        s.tile_tokens = s.small ? max(1, s.n) : p.tile_tokens;
+        s.tiles = int(unsigned(s.n + s.tile_tokens - 1) / unsigned(s.tile_tokens));
     }
-    s.length = p.b.lengths[b];
-    s.small = int64_t(s.n) * p.b.groups <= kSmallRows;
-    s.tile_tokens = s.small ? max(1, s.n) : p.tile_tokens;
-    s.tiles = (s.n + s.tile_tokens - 1) / s.tile_tokens;
-    s.chunks = s.n ? span_of(p, s.position((s.tiles - 1) * s.tile_tokens), s.position(s.n - 1)).count : 0;
+    const int origin = s.length - s.n;
+    s.chunks = s.n ? span_of(p, origin + (s.tiles - 1) * s.tile_tokens, s.length - 1).count : 0;
     return s;
 }
 
@@ -211,12 +213,11 @@ __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, 
 struct Piece {
     int b, head;
     int first, n;                // the tile's tokens
-    int pos;                     // position of its first token (may be -1: before the sequence; see row())
-    int64_t origin;              // lengths[b] - n_b + the tile's first token
+    int pos;                     // position of its first token (negative: before the sequence)
     int length;
     int pieces, split, part;     // part: first partial row of this piece
     bool small;
-    __device__ __forceinline__ int position(int i) const { return int(max(origin + i, int64_t(-1))); }
+    __device__ __forceinline__ int position(int i) const { return max(pos + i, -1); }
 };
 
 // Inclusive prefix sum over the wave (every lane active): row shifts, then the
@@ -294,8 +295,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
             out.head = local - rest * p.b.kv_heads;
             out.first = from(mine.first) + tile * tokens;
             out.n = min(tokens, n - tile * tokens);
-            out.origin = int64_t(out.length) - n + tile * tokens;
-            out.pos = out.position(0);
+            out.pos = out.length - n + tile * tokens;
             out.part = first_part + (((tile * p.b.kv_heads + out.head) * out.pieces) + out.split) *
                                         (out.small ? kSmallRows : kTileRows);
             return true;
@@ -389,7 +389,7 @@ __device__ void redo_row(const PagedAttnParams& p, const Piece& w, const Span& s
 // ---------------------------------------------------------------- small tiles
 template <int D>
 struct SmallShared {
-    float o[4][kSmallRows][D];
+    float o[4][kSmallRows][D + 4];             // (+ 4: the rows start in different banks)
     float m[4][kSmallRows], l[4][kSmallRows];
     int bad[kSmallRows];
 };
@@ -406,28 +406,6 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const int rows = w.n * G;
     const int ps = p.b.page_size;
     const bool mine = n < rows;
-    // this lane's query row (n), dims 32 s + 8 g ..
-    half8 qhi[STEPS], qlo[STEPS];
-    float c;
-    {
-        const float* q = p.query + (size_t(w.first + (mine ? n / G : 0)) * p.b.heads + w.head * G + (mine ? n % G : 0)) * D;
-        float x[STEPS][8];
-        float top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int d = 32 * s + 8 * g + i;
-                x[s][i] = mine && d < D ? q[d < D ? d : 0] : 0.0f;
-                top = fmaxf(top, __builtin_fabsf(x[s][i]));
-            }
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const int e = row_exponent(top);
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) split8(x[s], e, qhi[s], qlo[s]);
-        c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
-    }
     const int pos = w.position(mine ? n / G : 0);
     const int pos_min = w.position(0), pos_max = w.position(w.n - 1);
     float4v acc[VEC];
@@ -484,12 +462,44 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         }
     };
     const int own = steps > wave ? (steps - wave + 3) / 4 : 0;
+    // This lane's query row (n), dims 32 s + 8 g ..: its loads, the page
+    // table's and then the first step's of K and V are under way together.
+    float4v x[STEPS][2];
+    {
+        const float* q = p.query + (size_t(w.first + (mine ? n / G : 0)) * p.b.heads + w.head * G + (mine ? n % G : 0)) * D;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int d = D >= 32 ? 32 * s + 8 * g : 8 * (g & 1);
+            x[s][0] = *reinterpret_cast<const float4v*>(q + d);
+            x[s][1] = *reinterpret_cast<const float4v*>(q + d + 4);
+        }
+    }
     int pg = own ? pages_of(0) : -1;
     int pg0 = __builtin_amdgcn_readlane(pg, 0), pg1 = __builtin_amdgcn_readlane(pg, 1);
     int j0 = own ? key_of(wave) : 0;
     if (own) {
         load_k(pg0, pg1, j0);
         load_v(pg0, pg1, j0);
+    }
+    half8 qhi[STEPS], qlo[STEPS];
+    float c;
+    {
+        const bool used = mine && (D >= 32 || g < 2);
+        float top = 0.0f;
+        float y[STEPS][8];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[s][i] = used ? x[s][i >> 2][i & 3] : 0.0f;
+                top = fmaxf(top, __builtin_fabsf(y[s][i]));
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const int e = row_exponent(top);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) split8(y[s], e, qhi[s], qlo[s]);
+        c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
     }
     for (int k = 0; k < own; ++k) {
         // the next step's pages
@@ -575,48 +585,69 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
     // join the four waves: lane (n, g) holds row n, dims VEC (4 g + i) + v
+    const uint64_t any_seen = __ballot(seen);
+    const bool row_seen = ((any_seen | (any_seen >> 16) | (any_seen >> 32) | (any_seen >> 48)) >> n) & 1;
     if (g == 0) {
         S.m[wave][n] = m * c;
-        S.l[wave][n] = l;
+        S.l[wave][n] = row_seen ? l : -1.0f;               // (-1: this wave saw nothing of the row)
+        if (wave == 0) S.bad[n] = 0;
     }
-    if (threadIdx.x < kSmallRows) S.bad[threadIdx.x] = 0;
-    const uint64_t any_seen = __ballot(seen);
+    if (mine) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v)
+        for (int i = 0; i < 4; ++i) {
+            float* to = &S.o[wave][n][VEC * (4 * g + i)];
+            if constexpr (VEC >= 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S.o[wave][n][VEC * (4 * g + i) + v] = acc[v][i];
-    // rows of which this wave saw something: bit n (of any g)
-    const uint32_t rows_seen = uint32_t(any_seen | (any_seen >> 16) | (any_seen >> 32) | (any_seen >> 48)) & 0xFFFFu;
-    __syncthreads();
-    if (lane < kSmallRows && ((rows_seen >> lane) & 1)) atomicOr(&S.bad[lane], 2);
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * D; i += kBlock) {
-        const int r = i / D, d = i % D;
-        float top = -__builtin_inff();
+                for (int v = 0; v < VEC; v += 4)
+                    *reinterpret_cast<float4v*>(to + v) = float4v{acc[v][i], acc[v + 1][i], acc[v + 2][i], acc[v + 3][i]};
+            } else {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) top = fmaxf(top, S.m[v][r]);
-        float sum = 0.0f, o = 0.0f;
+                for (int v = 0; v < VEC; ++v) to[v] = acc[v][i];
+            }
+        }
+    }
+    lds_sync();
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kBlock) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float sm[4], sl[4];
+        float4v so[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-            const float f = S.m[v][r] == -__builtin_inff() ? 0.0f : exp2_fast(S.m[v][r] - top);
-            sum += S.l[v][r] * f;
-            o += S.o[v][r][d] * f;
+            sm[v] = S.m[v][r];
+            sl[v] = S.l[v][r];
+            so[v] = *reinterpret_cast<const float4v*>(&S.o[v][r][d]);
         }
-        const bool none = (S.bad[r] & 2) == 0;
-        const bool bad = !none && (!finite(sum) || !finite(o) || sum == 0.0f);
-        if (bad) atomicOr(&S.bad[r], 1);
-        const size_t row = size_t(w.first + r / p.b.groups) * p.b.heads + w.head * p.b.groups + r % p.b.groups;
+        const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+        float sum = 0.0f;
+        float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+        bool none = true;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const float f = sm[v] == -__builtin_inff() ? 0.0f : exp2_fast(sm[v] - top);
+            if (sl[v] != -1.0f) {
+                none = false;
+                sum += sl[v] * f;
+            }
+            o += so[v] * f;
+        }
+        const bool bad = !none && (!finite(sum) || sum == 0.0f || !finite(o[0]) || !finite(o[1]) || !finite(o[2]) ||
+                                   !finite(o[3]));
+        if (bad) S.bad[r] = 1;
+        const float f = none ? 0.0f : w.pieces == 1 ? 1.0f / sum : 1.0f / kWeightScale;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = none ? 0.0f : o[k] * f;
+        const size_t row = size_t(w.first + r / G) * p.b.heads + w.head * G + r % G;
         if (w.pieces == 1) {
-            p.out[row * D + d] = none ? 0.0f : o / sum;
+            *reinterpret_cast<float4v*>(p.out + row * D + d) = o;
         } else {
-            p.part_o[size_t(w.part + r) * D + d] = none ? 0.0f : o * (1.0f / kWeightScale);
-            if (d == 0) p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f)
-                                                     : make_float2(top, sum * (1.0f / kWeightScale));
+            *reinterpret_cast<float4v*>(p.part_o + size_t(w.part + r) * D + d) = o;
+            if (d == 0) p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f) : make_float2(top, sum * f);
         }
     }
+    wait_all_memory();                         // (a row done again is stored again, by another wave)
     __syncthreads();
     for (int r = wave; r < rows; r += 4)
-        if (S.bad[r] & 1) redo_row<D>(p, w, span, c0, c1, r);
+        if (S.bad[r]) redo_row<D>(p, w, span, c0, c1, r);
 }
 
 // ---------------------------------------------------------------- large tiles
@@ -964,7 +995,7 @@ struct AttnShared<D, true> {
 };
 
 template <int D, bool LARGE>
-__global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnParams p)
+__global__ __launch_bounds__(kBlock, LARGE ? 2 : OCC) void paged_attention_kernel(PagedAttnParams p)
 {
     __shared__ AttnShared<D, LARGE> S;
     Piece w;

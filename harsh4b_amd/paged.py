@@ -23,13 +23,13 @@ session, cpu_lightspark.py:275-309).  There is no host fallback.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
+import struct
 
 import torch
 
 from . import _native
-from ._native import HqPages, check
+from ._native import check
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (16, 32, 64, 128)
@@ -37,23 +37,44 @@ MAX_GROUPS = 8
 
 
 # --------------------------------------------------------------------------- checks
-def _tensor(t, name: str, dtype, dims: int, device=None) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != dims or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} device tensor of {dims} dimensions")
-    if device is not None and t.device != device:
+# (the host's time is most of a small call's: one attribute at a time, and the
+# C struct packed as bytes)
+_I32, _F32, _F16 = torch.int32, torch.float32, torch.float16
+_pack = struct.Struct("8i6P").pack
+
+
+def _is(t, dtype, index: int) -> bool:
+    """Whether t is a contiguous tensor of that type on that GPU."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous())
+
+
+def _refuse(name: str, t, dtype, index: int, what: str):
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.get_device() != index:
         raise ValueError(f"{name} is on another device")
+    raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} device tensor {what}")
 
 
-def _cache(keys, values, table, lengths, refs, status, dims: int, pools: bool = True) -> HqPages:
-    """The tables' C struct, checked; keys/values [layers, pages, kv_heads,
-    page_size, head_dim] (dims 5) or one layer of them (dims 4)."""
-    _tensor(table, "table", torch.int32, 2)
-    device = table.device
-    layers, kv_heads, page_size, head_dim = 1, 1, PAGE_SIZES[0], HEAD_DIMS[0]
+def _index(table) -> int:
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise ValueError("table must be a contiguous int32 device tensor [sequences, max_pages]")
+    return table.get_device()
+
+
+def _cache(index: int, keys, values, table, lengths, refs, status, dims: int, pools: bool = True):
+    """The tables' C struct (hq_pages) as bytes, after its checks, and the
+    sizes the callers need; keys/values [layers, pages, kv_heads, page_size,
+    head_dim] (dims 5) or one layer of them (dims 4)."""
+    layers, kv_heads, page_size, head_dim = 1, 1, 16, 16
+    key_ptr = value_ptr = 0
     if pools:
-        _tensor(keys, "keys", torch.float16, dims, device)
-        _tensor(values, "values", torch.float16, dims, device)
+        if not _is(keys, _F16, index):
+            _refuse("keys", keys, _F16, index, "of pages")
+        if not _is(values, _F16, index):
+            _refuse("values", values, _F16, index, "of pages")
         shape = keys.shape
+        if len(shape) != dims:
+            raise ValueError("keys must be [pages, kv_heads, page_size, head_dim]" if dims == 4 else
+                             "keys must be [layers, pages, kv_heads, page_size, head_dim]")
         if values.shape != shape:
             raise ValueError("keys and values must have the same shape")
         if dims == 5:
@@ -65,69 +86,83 @@ def _cache(keys, values, table, lengths, refs, status, dims: int, pools: bool = 
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
         if layers == 0 or pages == 0 or kv_heads == 0:
             raise ValueError("keys/values hold no pages")
+        key_ptr, value_ptr = keys.data_ptr(), values.data_ptr()
     else:
         pages = refs.shape[0] if isinstance(refs, torch.Tensor) and refs.dim() == 1 else 0
+    if not _is(table, _I32, index) or table.dim() != 2:
+        _refuse("table", table, _I32, index, "[sequences, max_pages]")
     sequences, max_pages = table.shape
     if sequences == 0 or max_pages == 0 or max_pages * page_size > 0x7FFFFFFF or sequences * max_pages > 0x7FFFFFFF:
         raise ValueError("table must be [sequences, max_pages] with fewer than 2^31 entries and positions a row")
+    length_ptr = ref_ptr = status_ptr = 0
     if lengths is not None:
-        _tensor(lengths, "lengths", torch.int32, 1, device)
-        if lengths.shape[0] != sequences:
-            raise ValueError("lengths must be [sequences]")
+        if not _is(lengths, _I32, index) or lengths.dim() != 1 or lengths.shape[0] != sequences:
+            _refuse("lengths", lengths, _I32, index, "[sequences]")
+        length_ptr = lengths.data_ptr()
     if refs is not None:
-        _tensor(refs, "refs", torch.int32, 1, device)
-        if refs.shape[0] != pages or pages == 0:
-            raise ValueError("refs must be [pages]")
+        if not _is(refs, _I32, index) or refs.dim() != 1 or refs.shape[0] != pages or pages == 0:
+            _refuse("refs", refs, _I32, index, "[pages]")
+        ref_ptr = refs.data_ptr()
     if status is not None:
-        _tensor(status, "status", torch.int32, 1, device)
-        if status.shape[0] != 1:
-            raise ValueError("status must hold one int32")
-    return HqPages(layers, pages, page_size, kv_heads, head_dim, sequences, max_pages, 0,
-                   keys.data_ptr() if pools else None, values.data_ptr() if pools else None, table.data_ptr(),
-                   None if lengths is None else lengths.data_ptr(), None if refs is None else refs.data_ptr(),
-                   None if status is None else status.data_ptr())
+        if not _is(status, _I32, index) or status.numel() != 1:
+            _refuse("status", status, _I32, index, "[1]")
+        status_ptr = status.data_ptr()
+    return (_pack(layers, pages, page_size, kv_heads, head_dim, sequences, max_pages, 0, key_ptr, value_ptr,
+                  table.data_ptr(), length_ptr, ref_ptr, status_ptr), sequences, kv_heads, head_dim)
 
 
-def _per_sequence(t, name: str, table) -> None:
-    _tensor(t, name, torch.int32, 1, table.device)
-    if t.shape[0] != table.shape[0]:
-        raise ValueError(f"{name} must be [sequences]")
+def _per_sequence(t, name: str, sequences: int, index: int) -> None:
+    if not _is(t, _I32, index) or t.dim() != 1 or t.shape[0] != sequences:
+        _refuse(name, t, _I32, index, "[sequences]")
 
 
-def _starts(starts, table, tokens: int) -> int | None:
+def _starts(starts, sequences: int, tokens: int, index: int) -> int | None:
     if starts is None:
-        if tokens != table.shape[0]:
+        if tokens != sequences:
             raise ValueError("without starts a batch has one row for every sequence")
         return None
-    _tensor(starts, "starts", torch.int32, 1, table.device)
-    if starts.shape[0] != table.shape[0] + 1:
-        raise ValueError("starts must be [sequences + 1]")
+    if not _is(starts, _I32, index) or starts.dim() != 1 or starts.shape[0] != sequences + 1:
+        _refuse("starts", starts, _I32, index, "[sequences + 1]")
     return starts.data_ptr()
 
 
-def _launch(call, nbytes: int, device, stream, tensors, what: str) -> None:
-    """call(workspace pointer, stream handle) on `stream` (None: the current
-    one of `device`) with a workspace of this call alone: memory of any
+def _launch(entry, args: tuple, nbytes: int, index: int, stream, tensors, what: str) -> None:
+    """entry(*args[, workspace], stream handle) on `stream` (None: the current
+    one of the tensors' GPU) with a workspace of this call alone: memory of any
     contents from torch's allocator, which hands it out in the stream's order
     and inside a capture from the graph's own pool."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _launch(call, nbytes, device, stream, tensors, what)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(entry, args, nbytes, index, stream, tensors, what)
     if stream is None:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        check(call(None if ws is None else ws.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)), what)
-        return
-    if stream.device != device:
-        raise ValueError("the stream belongs to another device than the tensors")
-    # the stream waits for what the caller's has enqueued, and the tensors'
-    # memory is not reused before the stream is done with them
-    stream.wait_stream(torch.cuda.current_stream(device))
-    with torch.cuda.stream(stream):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
-    check(call(None if ws is None else ws.data_ptr(), stream.cuda_stream), what)
+        handle = torch._C._cuda_getCurrentRawStream(index)
+        if nbytes:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=_device_of(index))
+            status = entry(*args, workspace.data_ptr(), handle)
+        else:
+            status = entry(*args, handle)
+    else:
+        if stream.device.index != index:
+            raise ValueError("the stream belongs to another device than the tensors")
+        # the stream waits for what the caller's has enqueued, and the tensors'
+        # memory is not reused before the stream is done with them
+        stream.wait_stream(torch.cuda.current_stream(index))
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+        if nbytes:
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=_device_of(index))
+            status = entry(*args, workspace.data_ptr(), stream.cuda_stream)
+        else:
+            status = entry(*args, stream.cuda_stream)
+    if status:
+        check(status, what)
+
+
+@functools.lru_cache(maxsize=None)
+def _device_of(index: int) -> torch.device:
+    return torch.device("cuda", index)
 
 
 # --------------------------------------------------------------------------- append, attention
@@ -140,38 +175,36 @@ def paged_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     float32 [tokens, heads, head_dim].  qkv: raw projection rows float32
     [tokens, (heads + 2 kv_heads) * head_dim]; `lengths` count the new tokens
     already (pages_resize)."""
-    cache = _cache(keys, values, table, lengths, None, status, 4)
-    device, d, kv = table.device, cache.head_dim, cache.kv_heads
-    if status is None:
-        raise ValueError("paged_append needs the cache's status")
-    _tensor(qkv, "qkv", torch.float32, 2, device)
+    if status is None or lengths is None:
+        raise ValueError("paged_append needs the cache's lengths and status")
+    index = _index(table)
+    cache, sequences, kv, d = _cache(index, keys, values, table, lengths, None, status, 4)
+    if not _is(qkv, _F32, index) or qkv.dim() != 2:
+        _refuse("qkv", qkv, _F32, index, "[tokens, (heads + 2 kv_heads) * head_dim]")
     tokens, width = qkv.shape
     heads = width // d - 2 * kv
     if width % d or heads < 1 or heads % kv or heads // kv > MAX_GROUPS:
         raise ValueError("qkv must be [tokens, (heads + 2 kv_heads) * head_dim] with 1 to 8 heads a kv head")
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _tensor(t, name, torch.float32, 1, device)
-        if t.shape[0] != d:
-            raise ValueError(f"{name} must be [head_dim]")
-    for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        _tensor(t, name, torch.float32, 2, device)
-    if rope_cos.shape != rope_sin.shape or rope_cos.shape[1] != d // 2 or rope_cos.shape[0] < 1:
+    if not _is(q_norm, _F32, index) or q_norm.dim() != 1 or q_norm.shape[0] != d:
+        _refuse("q_norm", q_norm, _F32, index, "[head_dim]")
+    if not _is(k_norm, _F32, index) or k_norm.dim() != 1 or k_norm.shape[0] != d:
+        _refuse("k_norm", k_norm, _F32, index, "[head_dim]")
+    if not _is(rope_cos, _F32, index) or not _is(rope_sin, _F32, index) or rope_cos.dim() != 2:
+        raise ValueError("rope_cos and rope_sin must be contiguous float32 device tensors of the cache's GPU")
+    positions, half = rope_cos.shape
+    if rope_sin.shape != (positions, half) or 2 * half != d or positions < 1:
         raise ValueError("rope_cos and rope_sin must be [positions, head_dim / 2]")
-    first = _starts(starts, table, tokens)
+    first = _starts(starts, sequences, tokens, index)
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=torch.float32, device=device)
-    else:
-        _tensor(out, "out", torch.float32, 3, device)
-        if out.shape != (tokens, heads, d):
-            raise ValueError("out must be [tokens, heads, head_dim]")
-    if tokens == 0:
-        return out
-    lib = _native.lib()
-    _launch(lambda ws, s: lib.hq_paged_append(
-        ctypes.byref(cache), qkv.data_ptr(), first, tokens, heads, q_norm.data_ptr(), k_norm.data_ptr(), float(eps),
-        rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], out.data_ptr(), s), 0, device, stream,
-        (qkv, q_norm, k_norm, rope_cos, rope_sin, keys, values, table, lengths, status, starts, out),
-        "hq_paged_append")
+        out = torch.empty((tokens, heads, d), dtype=_F32, device=qkv.device)
+    elif not _is(out, _F32, index) or out.shape != (tokens, heads, d):
+        _refuse("out", out, _F32, index, "[tokens, heads, head_dim]")
+    if tokens:
+        _launch(_native.lib().hq_paged_append,
+                (cache, qkv.data_ptr(), first, tokens, heads, q_norm.data_ptr(), k_norm.data_ptr(), eps,
+                 rope_cos.data_ptr(), rope_sin.data_ptr(), positions, out.data_ptr()), 0, index, stream,
+                (qkv, q_norm, k_norm, rope_cos, rope_sin, keys, values, table, lengths, status, starts, out),
+                "hq_paged_append")
     return out
 
 
@@ -189,34 +222,35 @@ def paged_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tenso
     `window` > 0 the last `window` of them and the first `sinks` positions.  A
     token that sees nothing gets zeros; rows past the last sequence's are not
     touched."""
-    cache = _cache(keys, values, table, lengths, None, None, 4)
-    device, d, kv = table.device, cache.head_dim, cache.kv_heads
-    _tensor(query, "query", torch.float32, 3, device)
-    tokens, heads, width = query.shape
+    if lengths is None:
+        raise ValueError("paged_attention needs the cache's lengths")
+    index = _index(table)
+    cache, sequences, kv, d = _cache(index, keys, values, table, lengths, None, None, 4)
+    if not _is(query, _F32, index) or query.dim() != 3:
+        _refuse("query", query, _F32, index, "[tokens, heads, head_dim]")
+    tokens, heads, width = shape = query.shape
     if width != d or heads < 1 or heads % kv or heads // kv > MAX_GROUPS:
         raise ValueError("query must be [tokens, heads, head_dim] with 1 to 8 heads a kv head")
     if not 0 <= window <= 0x7FFFFFFF or not 0 <= sinks <= 0x7FFFFFFF:
         raise ValueError("window and sinks must not be negative")
-    first = _starts(starts, table, tokens)
+    first = _starts(starts, sequences, tokens, index)
     if out is None:
         out = torch.empty_like(query)
-    else:
-        _tensor(out, "out", torch.float32, 3, device)
-        if out.shape != query.shape:
-            raise ValueError("out must be like query")
-    if tokens == 0:
-        return out
-    lib = _native.lib()
-    _launch(lambda ws, s: lib.hq_paged_attention(
-        ctypes.byref(cache), query.data_ptr(), first, tokens, heads, window, sinks, out.data_ptr(), ws, s),
-        _attention_workspace_bytes(tokens, heads, kv, d, starts is None), device, stream,
-        (query, keys, values, table, lengths, starts, out), "hq_paged_attention")
+    elif not _is(out, _F32, index) or out.shape != shape:
+        _refuse("out", out, _F32, index, "like query")
+    if tokens:
+        _launch(_native.lib().hq_paged_attention,
+                (cache, query.data_ptr(), first, tokens, heads, window, sinks, out.data_ptr()),
+                _attention_workspace_bytes(tokens, heads, kv, d, first is None), index, stream,
+                (query, keys, values, table, lengths, starts, out), "hq_paged_attention")
     return out
 
 
 # --------------------------------------------------------------------------- page management
-def _pages_workspace(cache: HqPages) -> int:
-    return _native.lib().hq_pages_workspace_bytes(ctypes.byref(cache))
+@functools.lru_cache(maxsize=1024)
+def _pages_workspace_bytes(pages: int, sequences: int, max_pages: int) -> int:
+    cache = _pack(1, pages, 16, 1, 16, sequences, max_pages, 0, 0, 0, 0, 0, 0, 0)
+    return _native.lib().hq_pages_workspace_bytes(cache)
 
 
 def pages_resize(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -228,15 +262,15 @@ def pages_resize(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
     others hold it too; shrinking releases pages, and `window` > 0 those that
     no later query sees.  Too few free pages, or a length past the table, set
     HQ_PAGES_FULL in `status` and change nothing."""
-    cache = _cache(keys, values, table, lengths, refs, status, 5)
     if lengths is None or refs is None or status is None:
         raise ValueError("pages_resize needs lengths, refs and status")
-    _per_sequence(new_lengths, "new_lengths", table)
+    index = _index(table)
+    cache, sequences, _, _ = _cache(index, keys, values, table, lengths, refs, status, 5)
+    _per_sequence(new_lengths, "new_lengths", sequences, index)
     if not 0 <= window <= 0x7FFFFFFF or not 0 <= sinks <= 0x7FFFFFFF:
         raise ValueError("window and sinks must not be negative")
-    lib = _native.lib()
-    _launch(lambda ws, s: lib.hq_pages_resize(ctypes.byref(cache), new_lengths.data_ptr(), window, sinks, ws, s),
-            _pages_workspace(cache), table.device, stream,
+    _launch(_native.lib().hq_pages_resize, (cache, new_lengths.data_ptr(), window, sinks),
+            _pages_workspace_bytes(refs.shape[0], sequences, table.shape[1]), index, stream,
             (keys, values, table, lengths, refs, status, new_lengths), "hq_pages_resize")
 
 
@@ -247,11 +281,12 @@ def pages_fork(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, s
     call, sharing all its pages (hq_pages_fork); what it held is released."""
     if lengths is None or refs is None or status is None:
         raise ValueError("pages_fork needs lengths, refs and status")
-    cache = _cache(None, None, table, lengths, refs, status, 5, pools=False)
-    _per_sequence(parents, "parents", table)
-    lib = _native.lib()
-    _launch(lambda ws, s: lib.hq_pages_fork(ctypes.byref(cache), parents.data_ptr(), ws, s), _pages_workspace(cache),
-            table.device, stream, (table, lengths, refs, status, parents), "hq_pages_fork")
+    index = _index(table)
+    cache, sequences, _, _ = _cache(index, None, None, table, lengths, refs, status, 5, pools=False)
+    _per_sequence(parents, "parents", sequences, index)
+    _launch(_native.lib().hq_pages_fork, (cache, parents.data_ptr()),
+            _pages_workspace_bytes(refs.shape[0], sequences, table.shape[1]), index, stream,
+            (table, lengths, refs, status, parents), "hq_pages_fork")
 
 
 def pages_compact(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, refs: torch.Tensor,
@@ -260,16 +295,15 @@ def pages_compact(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
     and refs with them; returns their number, int32 [1] on the device."""
     if refs is None:
         raise ValueError("pages_compact needs refs")
-    cache = _cache(keys, values, table, None, refs, None, 5)
+    index = _index(table)
+    cache, sequences, _, _ = _cache(index, keys, values, table, None, refs, None, 5)
     if live is None:
-        live = torch.empty(1, dtype=torch.int32, device=table.device)
-    else:
-        _tensor(live, "live", torch.int32, 1, table.device)
-        if live.shape[0] != 1:
-            raise ValueError("live must hold one int32")
-    lib = _native.lib()
-    _launch(lambda ws, s: lib.hq_pages_compact(ctypes.byref(cache), live.data_ptr(), ws, s), _pages_workspace(cache),
-            table.device, stream, (keys, values, table, refs, live), "hq_pages_compact")
+        live = torch.empty(1, dtype=_I32, device=table.device)
+    elif not _is(live, _I32, index) or live.numel() != 1:
+        _refuse("live", live, _I32, index, "[1]")
+    _launch(_native.lib().hq_pages_compact, (cache, live.data_ptr()),
+            _pages_workspace_bytes(refs.shape[0], sequences, table.shape[1]), index, stream,
+            (keys, values, table, refs, live), "hq_pages_compact")
     return live
 
 
