@@ -651,10 +651,18 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
 }
 
 // ---------------------------------------------------------------- large tiles
+// Two groups of 16 lanes read four pieces of four rows of V at a time: 16 of
+// the 16 places of 256 bytes (a row of D = 128, two of D = 64, ...).
+template <int D>
+__host__ __device__ constexpr int v_flip(int key)
+{
+    return D == 128 ? 4 * (key & 3) : D == 64 ? 4 * ((key >> 1) & 1) : 0;
+}
+
 template <int D>
 struct LargeShared {
     // [key][dim], the 16-byte pieces of a row permuted by the key: piece i of K in place i ^ (key & 15), of V in
-    // i ^ 2 (key & 7) (both within the row), so that the rows a product reads together lie in different banks
+    // i ^ v_flip(key) (both within the row), so that the rows a product reads together lie in different banks
     alignas(256) uint16_t k[2][kChunkKeys * D];
     alignas(256) uint16_t v[2][kChunkKeys * D];
 };
@@ -743,7 +751,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     constexpr int PER = 64 / PIECES < 16 ? 64 / PIECES : 16, COPIES = 16 / PER;
     const int copy_row = lane / PIECES, place = lane % PIECES;
     const uint32_t k_copy = uint32_t(copy_row * PIECES + (place ^ (copy_row & (PIECES - 1)))) * 16;
-    const uint32_t v_copy = uint32_t(copy_row * PIECES + (place ^ ((2 * copy_row) & (PIECES - 1)))) * 16;
+    const uint32_t v_copy = uint32_t(copy_row * PIECES + (place ^ v_flip<D>(copy_row))) * 16;
     auto copy_k = [&](int page, int cc) {
         const uint16_t* k = p.b.keys + base_of(page, span.chunk(cc) * kChunkKeys + 16 * wave);
         const uint32_t to = lds_addr(&S.k[cc & 1][16 * wave * D]);
@@ -763,7 +771,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         for (int i = 0; i < COPIES; ++i) {
             if (D < 32 && copy_row >= 16) continue;
             if (copy_row < there - i * PER)
-                dma16(v, (from ^ (16 * ((2 * i * PER) & (PIECES - 1)))) + 1024 * i, lds_addr(to) + 1024 * i);
+                dma16(v, (from ^ (16 * v_flip<D>(i * PER))) + 1024 * i, lds_addr(to) + 1024 * i);
             else
                 *reinterpret_cast<uint4v*>(to + 512 * i + 8 * lane) = uint4v{0, 0, 0, 0};
         }
@@ -779,7 +787,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const uint32_t k_lane = lds_addr(&S.k[0][0]) + n * 2 * D + ((g ^ (n & (PIECES - 1))) & (PIECES - 1)) * 16;
     const int v_key = 4 * g + (lane16 >> 2);
     const uint32_t v_lane = lds_addr(&S.v[0][0]) + v_key * 2 * D + 8 * (lane16 & 1) +
-                            (((2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ (2 * v_key)) & (PIECES - 1)) * 16;
+                            (((2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) & (PIECES - 1)) ^ v_flip<D>(v_key)) * 16;
     auto k_unit = [&](uint32_t base, int i) { return *lds_half8(uintptr_t(base ^ (32 * i))); };
     auto v_unit = [&](uint32_t base, int i) {
         const uint32_t at = (base ^ ((64 * (i % DT)) & (2 * D - 1))) + (i / DT) * 32 * D;
