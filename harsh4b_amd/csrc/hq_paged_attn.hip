@@ -822,6 +822,9 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         constexpr bool SC = decltype(with_scores)::value, WE = decltype(with_weights)::value;
         constexpr int UNITS = SC ? STEPS : 1;
         constexpr int PAIRS = 8 / UNITS;
+        // (a wave at its matrix instructions goes before one at its masks and
+        // maxima: the SIMD's two waves then fall out of step, and overlap)
+        __builtin_amdgcn_s_setprio(1);
         constexpr int AHEAD = KAHEAD, VSET = VAHEAD + 1;
         Weights now{};
         half8 ka[AHEAD + 1], va[VSET];
@@ -863,6 +866,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             });
         }
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
     };
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
@@ -936,7 +940,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 if (active) step(no, 0, 0, sa, yes, sb, cc & 1, 1);
                 break;
             }
-            lds_sync();
+            lds_sync();                        // K of cc is read
             there = there_of(cc + 1);
             if (cc + 2 < c1) {
                 if (cc + 2 - pg_first == 16) {
@@ -950,6 +954,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 step(yes, (cc + 1) & 1, 0, sa, yes, sb, cc & 1, 1);
                 settle(cc + 1, 0, there, sa);
             }
+            // (waiting for V of cc + 1 alone, with K of cc + 2 on its way, gained nothing)
             wait_all_memory();
             lds_sync();
         }
