@@ -62,7 +62,7 @@ constexpr int kTileRows = 128;
 #define TSMALL 512
 #endif
 #ifndef KAHEAD
-#define KAHEAD 1
+#define KAHEAD 2
 #endif
 #ifndef VAHEAD
 #define VAHEAD 3
@@ -86,12 +86,16 @@ struct PagedAttnParams {
     int window, sinks;           // window 0: none
     int tile_tokens;             // tokens of a large tile
     int target;                  // pieces aimed at
+    int by_group;                // 65536 / groups + 1, for row_token
     int part_rows;               // rows of partial results there is room for
     int32_t* ordered;            // [1] starts never fall
     int2* desc;                  // [tokens, kv_heads] 2 * pieces + small, first partial row
     float* part_o;               // [part_rows, D]
     float2* part_ml;             // [part_rows] m (of the scores times log2 e), l
 };
+
+// The token of a tile's row: r / groups (exact: r < 128, groups <= 8).
+__device__ __forceinline__ int row_token(const PagedAttnParams& p, int r) { return (r * p.by_group) >> 16; }
 
 // Whether the query at position `pos` sees position j (pages aside).
 __device__ __forceinline__ bool paged_visible(int pos, int j, int window, int sinks)
@@ -220,6 +224,8 @@ struct Piece {
     __device__ __forceinline__ int position(int i) const { return max(pos + i, -1); }
 };
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Inclusive prefix sum over the wave (every lane active): row shifts, then the
 // row totals broadcast to the rows above.
 __device__ __forceinline__ int wave_prefix(int v)
@@ -292,7 +298,9 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
                 out.split = rest - done * out.pieces;
                 tile = tiles - 1 - done;                             // the longest first
             }
-            out.head = local - rest * p.b.kv_heads;
+            tile = uniform(tile);
+            out.split = uniform(out.split);
+            out.head = uniform(local - rest * p.b.kv_heads);
             out.first = from(mine.first) + tile * tokens;
             out.n = min(tokens, n - tile * tokens);
             out.pos = out.length - n + tile * tokens;
@@ -365,13 +373,14 @@ template <int D>
 __device__ void redo_row(const PagedAttnParams& p, const Piece& w, const Span& span, int c0, int c1, int r)
 {
     const int lane = threadIdx.x & (kWave - 1);
-    const size_t row = size_t(w.first + r / p.b.groups) * p.b.heads + w.head * p.b.groups + r % p.b.groups;
+    const int token = row_token(p, r);
+    const size_t row = size_t(w.first + token) * p.b.heads + w.head * p.b.groups + (r - token * p.b.groups);
     float m = -__builtin_inff(), l = 0.0f, o[2] = {0.0f, 0.0f};
     bool seen = false;
     const int64_t end = int64_t(p.b.max_pages) << p.b.shift;
     for (int c = c0; c < c1; ++c) {
         const int at = span.chunk(c) * kChunkKeys;
-        paged_row<D>(p, p.query + row * D, w.b, w.head, w.position(r / p.b.groups), at,
+        paged_row<D>(p, p.query + row * D, w.b, w.head, w.position(token), at,
                      int(min(end, int64_t(at) + kChunkKeys)), m, l, o, seen);
     }
     if (w.pieces == 1) {
@@ -406,7 +415,8 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const int rows = w.n * G;
     const int ps = p.b.page_size;
     const bool mine = n < rows;
-    const int pos = w.position(mine ? n / G : 0);
+    const int token = mine ? row_token(p, n) : 0;
+    const int pos = w.position(token);
     const int pos_min = w.position(0), pos_max = w.position(w.n - 1);
     float4v acc[VEC];
 #pragma unroll
@@ -466,7 +476,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     // table's and then the first step's of K and V are under way together.
     float4v x[STEPS][2];
     {
-        const float* q = p.query + (size_t(w.first + (mine ? n / G : 0)) * p.b.heads + w.head * G + (mine ? n % G : 0)) * D;
+        const float* q = p.query + (size_t(w.first + token) * p.b.heads + w.head * G + (mine ? n - token * G : 0)) * D;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int d = D >= 32 ? 32 * s + 8 * g : 8 * (g & 1);
@@ -636,7 +646,8 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         const float f = none ? 0.0f : w.pieces == 1 ? 1.0f / sum : 1.0f / kWeightScale;
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = none ? 0.0f : o[k] * f;
-        const size_t row = size_t(w.first + r / G) * p.b.heads + w.head * G + r % G;
+        const int of = row_token(p, r);
+        const size_t row = size_t(w.first + of) * p.b.heads + w.head * G + (r - of * G);
         if (w.pieces == 1) {
             *reinterpret_cast<float4v*>(p.out + row * D + d) = o;
         } else {
@@ -690,8 +701,8 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const int rows = w.n * G;
     const int r = 32 * wave + n;               // this lane's row
     const bool mine = r < rows;
-    const int token = mine ? r / G : 0;
-    const size_t out_row = size_t(w.first + token) * p.b.heads + w.head * G + (mine ? r % G : 0);
+    const int token = mine ? row_token(p, r) : 0;
+    const size_t out_row = size_t(w.first + token) * p.b.heads + w.head * G + (mine ? r - token * G : 0);
     half8 qhi[STEPS], qlo[STEPS];
     float c;
     {
@@ -715,11 +726,9 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         for (int s = 0; s < STEPS; ++s) split8(x[s], e, qhi[s], qlo[s]);
         c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
     }
-    const int pos = w.position(token);
-    const int low = p.window > 0 ? max(0, pos - p.window + 1) : 0;     // first position of the row's window
     const bool active = 32 * wave < rows;      // (wave-uniform)
-    const int pos_min = w.position(min(32 * wave, rows - 1) / G);
-    const int pos_max = w.position(min(32 * wave + 31, rows - 1) / G);
+    const int pos_min = uniform(w.position(row_token(p, min(32 * wave, rows - 1))));
+    const int pos_max = uniform(w.position(row_token(p, min(32 * wave + 31, rows - 1))));
 
     float16v acc[DT];
 #pragma unroll
@@ -744,36 +753,44 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         asm volatile("" : "+v"(v));
         return v;
     };
-    // Rows 16 wave .. + 15 of chunk cc, contiguous in their page, to LDS: copy
+    // Rows 16 wave .. + 15 of chunk cc (from position `at`), contiguous in their page, to LDS: copy
     // i takes PER rows, lane (row, place) the piece that belongs in that place.
     // The permutations work bit by bit, so copy i's piece is copy 0's with
     // bits of the row 16 i / COPIES flipped.
     constexpr int PER = 64 / PIECES < 16 ? 64 / PIECES : 16, COPIES = 16 / PER;
-    const int copy_row = lane / PIECES, place = lane % PIECES;
-    const uint32_t k_copy = uint32_t(copy_row * PIECES + (place ^ (copy_row & (PIECES - 1)))) * 16;
-    const uint32_t v_copy = uint32_t(copy_row * PIECES + (place ^ v_flip<D>(copy_row))) * 16;
-    auto copy_k = [&](int page, int cc) {
-        const uint16_t* k = p.b.keys + base_of(page, span.chunk(cc) * kChunkKeys + 16 * wave);
+    auto copy_k = [&](int page, int at, int cc) {
+        const uint16_t* k = p.b.keys + base_of(page, at + 16 * wave);
         const uint32_t to = lds_addr(&S.k[cc & 1][16 * wave * D]);
-        const uint32_t from = opaque(k_copy);
+        const uint32_t x = opaque(lane), row = x / PIECES, place = x % PIECES;
+        const uint32_t from = (row * PIECES + (place ^ (row & (PIECES - 1)))) * 16;
 #pragma unroll
         for (int i = 0; i < COPIES; ++i)
-            if (D >= 32 || copy_row < 16)
+            if (D >= 32 || row < 16)
                 dma16(k, (from ^ (16 * ((i * PER) & (PIECES - 1)))) + 1024 * i, to + 1024 * i);
     };
-    auto copy_v = [&](int page, int cc) {
-        const int j0 = span.chunk(cc) * kChunkKeys + 16 * wave;
+    auto copy_v = [&](int page, int at, int cc) {
+        const int j0 = at + 16 * wave;
         const uint16_t* v = p.b.values + base_of(page, j0);
         uint16_t* to = &S.v[cc & 1][16 * wave * D];
-        const int there = page < 0 ? 0 : min(w.length - j0, 16);         // rows; the others are zeros
-        const uint32_t from = opaque(v_copy);
+        const int there = page < 0 ? 0 : w.length - j0;                  // rows of the 16; the others are zeros
+        const uint32_t x = opaque(lane), copy_row = x / PIECES;
+        const uint32_t from = (copy_row * PIECES + ((x % PIECES) ^ v_flip<D>(copy_row))) * 16;
+        if (there >= 16) {
 #pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-            if (D < 32 && copy_row >= 16) continue;
-            if (copy_row < there - i * PER)
-                dma16(v, (from ^ (16 * v_flip<D>(i * PER))) + 1024 * i, lds_addr(to) + 1024 * i);
-            else
-                *reinterpret_cast<uint4v*>(to + 512 * i + 8 * lane) = uint4v{0, 0, 0, 0};
+            for (int i = 0; i < COPIES; ++i)
+                if (D >= 32 || copy_row < 16)
+                    dma16(v, (from ^ (16 * v_flip<D>(i * PER))) + 1024 * i, lds_addr(to) + 1024 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+                if (D < 32 && copy_row >= 16) continue;
+                if (int(copy_row) < there - i * PER) {
+                    dma16(v, (from ^ (16 * v_flip<D>(i * PER))) + 1024 * i, lds_addr(to) + 1024 * i);
+                } else {
+                    const uint32_t z = opaque(0);
+                    *reinterpret_cast<uint4v*>(to + 512 * i + 8 * lane) = uint4v{z, z, z, z};
+                }
+            }
         }
     };
     // Operands from LDS: unit i of the scores of half t (dims 16 i ..), unit i
@@ -871,13 +888,17 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
     // masks, and a new maximum where the old one is left too far behind
-    auto settle = [&](int cc, int t, uint32_t there, float16v& s) {
-        const int j0 = span.chunk(cc) * kChunkKeys + 32 * t;
+    auto settle = [&](int at, int t, uint32_t there, float16v& s) {
+        const int j0 = at + 32 * t;
         const uint32_t both = (there >> (2 * t)) & 3u;
         const bool all = both == 3u && j0 + 31 <= pos_min &&
                          (p.window == 0 || j0 > pos_max - p.window || j0 + 32 <= p.sinks);
         if (!all) {
             // of the lane's first key; its others lie 8 (i / 4) + i % 4 further
+            const int x = int(opaque(lane)), g = x >> 5;
+            const int row = 32 * wave + (x & 31);
+            const int pos = w.position(row < rows ? row_token(p, row) : 0);
+            const int low = p.window > 0 ? max(0, pos - p.window + 1) : 0;     // first position of the row's window
             const int to_pos = int(opaque(pos - j0 - 4 * g)), to_low = int(opaque(low - j0 - 4 * g));
             const int to_sinks = int(opaque(p.sinks - j0 - 4 * g));
 #pragma unroll
@@ -917,50 +938,66 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         pg = pages_of(c0);
         uint32_t there = there_of(c0);
         int page = __builtin_amdgcn_readlane(pg, wave);        // of chunk c0, then of cc + 1
-        copy_k(page, c0);
-        copy_v(page, c0);
+        // positions of chunks cc and cc + 1
+        int at = span.chunk(c0) * kChunkKeys, at_next = span.chunk(c0 + 1) * kChunkKeys;
+        copy_k(page, at, c0);
+        copy_v(page, at, c0);
         page = __builtin_amdgcn_readlane(pg, 4 + wave);
-        if (c0 + 1 < c1) copy_k(page, c0 + 1);
+        if (c0 + 1 < c1) copy_k(page, at_next, c0 + 1);
         wait_all_memory();
         lds_sync();
-        float16v sa{}, sb{};
-        if (active) {
-            step(yes, c0 & 1, 0, sa, no, sb, 0, 0);
-            settle(c0, 0, there, sa);
-        }
-        for (int cc = c0;; ++cc) {
-            // here: sa the scores of cc's first half; K of cc and cc + 1, V of cc in LDS
-            const bool more = cc + 1 < c1;
-            if (more) copy_v(page, cc + 1);
-            if (active) {
-                step(yes, cc & 1, 1, sb, yes, sa, cc & 1, 0);
-                settle(cc, 1, there, sb);
-            }
-            if (!more) {
-                if (active) step(no, 0, 0, sa, yes, sb, cc & 1, 1);
-                break;
-            }
+        // copies of chunk cc + 1's V, and (once K of cc is read) of cc + 2's K
+        auto stage_v = [&](int cc) { copy_v(page, at_next, cc + 1); };
+        auto stage_k = [&](int cc) {
             lds_sync();                        // K of cc is read
             there = there_of(cc + 1);
+            at = at_next;
+            at_next = span.chunk(cc + 2) * kChunkKeys;
             if (cc + 2 < c1) {
                 if (cc + 2 - pg_first == 16) {
                     pg_first = cc + 2;
                     pg = pages_of(pg_first);
                 }
                 page = __builtin_amdgcn_readlane(pg, 4 * (cc + 2 - pg_first) + wave);
-                copy_k(page, cc + 2);
+                copy_k(page, at_next, cc + 2);
             }
-            if (active) {
-                step(yes, (cc + 1) & 1, 0, sa, yes, sb, cc & 1, 1);
-                settle(cc + 1, 0, there, sa);
-            }
+        };
+        auto arrived = [&] {
             // (waiting for V of cc + 1 alone, with K of cc + 2 on its way, gained nothing)
             wait_all_memory();
             lds_sync();
+        };
+        if (active) {
+            float16v sa, sb;
+            step(yes, c0 & 1, 0, sa, no, sa, 0, 0);
+            settle(at, 0, there, sa);
+            for (int cc = c0; cc < c1 - 1; ++cc) {
+                // here: sa the scores of cc's first half; K of cc and cc + 1, V of cc in LDS
+                stage_v(cc);
+                step(yes, cc & 1, 1, sb, yes, sa, cc & 1, 0);
+                settle(at, 1, there, sb);
+                stage_k(cc);
+                step(yes, (cc + 1) & 1, 0, sa, yes, sb, cc & 1, 1);
+                settle(at, 0, there, sa);
+                arrived();
+            }
+            step(yes, (c1 - 1) & 1, 1, sb, yes, sa, (c1 - 1) & 1, 0);
+            settle(at, 1, there, sb);
+            step(no, 0, 0, sa, yes, sb, (c1 - 1) & 1, 1);
+        } else {                               // rows of no token: only the wave's share of the copies
+            for (int cc = c0; cc < c1 - 1; ++cc) {
+                stage_v(cc);
+                stage_k(cc);
+                arrived();
+            }
         }
     }
     l += __shfl_xor(l, 32, kWave);
     // lane (n, g): row n, dims 32 dt + 8 (i / 4) + 4 g + i % 4
+    const int x = int(opaque(lane)), n_end = x & 31, g_end = x >> 5, r_end = 32 * wave + n_end;
+    const bool mine_end = r_end < rows;
+    const int token_end = mine_end ? row_token(p, r_end) : 0;
+    const size_t row_end = size_t(w.first + token_end) * p.b.heads + w.head * G + (mine_end ? r_end - token_end * G : 0);
     bool ok = finite(l) && l != 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -968,18 +1005,18 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         for (int i = 0; i < 16; ++i)
             if (32 * dt + 8 * (i >> 2) < D) ok &= finite(acc[dt][i]);
     const uint64_t was_seen = __ballot(seen);
-    const bool none = (((was_seen | (was_seen >> 32)) >> n) & 1) == 0;
-    const uint64_t wrong = __ballot(mine && !none && !ok);
+    const bool none = (((was_seen | (was_seen >> 32)) >> n_end) & 1) == 0;
+    const uint64_t wrong = __ballot(mine_end && !none && !ok);
     const uint32_t again = uint32_t(wrong | (wrong >> 32));
-    if (mine && ((again >> n) & 1) == 0) {
+    if (mine_end && ((again >> n_end) & 1) == 0) {
         const bool direct = w.pieces == 1;
-        float* to = direct ? p.out + out_row * D : p.part_o + size_t(w.part + r) * D;
+        float* to = direct ? p.out + row_end * D : p.part_o + size_t(w.part + r_end) * D;
         const float f = none ? 0.0f : direct ? 1.0f / l : 1.0f / kLargeScale;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int dim = 32 * dt + 8 * i + 4 * g;
+                const int dim = 32 * dt + 8 * i + 4 * g_end;
                 if (dim < D) {
                     float4v x;
 #pragma unroll
@@ -987,8 +1024,8 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
                     *reinterpret_cast<float4v*>(to + dim) = x;
                 }
             }
-        if (!direct && g == 0)
-            p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f)
+        if (!direct && g_end == 0)
+            p.part_ml[w.part + r_end] = none ? make_float2(-__builtin_inff(), 0.0f)
                                          : make_float2(m * c, l * (1.0f / kLargeScale));
     }
     for (uint32_t left = again; left; left &= left - 1)
@@ -1018,9 +1055,12 @@ __global__ __launch_bounds__(kBlock, LARGE ? 2 : OCC) void paged_attention_kerne
         for (int i = threadIdx.x; i < w.n; i += kBlock)
             p.desc[size_t(w.first + i) * p.b.kv_heads + w.head] =
                 make_int2(2 * w.pieces + (w.small ? 1 : 0), w.part + i * p.b.groups);
-    const Span span = span_of(p, w.pos, w.position(w.n - 1));
-    const int c0 = int(int64_t(span.count) * w.split / w.pieces);
-    const int c1 = int(int64_t(span.count) * (w.split + 1) / w.pieces);
+    Span span = span_of(p, w.pos, w.position(w.n - 1));
+    // (the same in every lane: kept where the compiler knows it)
+    span.sink = uniform(span.sink);
+    span.first = uniform(span.first);
+    const int c0 = uniform(int(int64_t(span.count) * w.split / w.pieces));
+    const int c1 = uniform(int(int64_t(span.count) * (w.split + 1) / w.pieces));
     if (w.small) small_tile<D>(p, w, span, c0, c1, S.small);
     else if constexpr (LARGE) large_tile<D>(p, w, span, c0, c1, S.large);
 }
@@ -1142,6 +1182,7 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     p.window = window;
     p.sinks = sinks;
     p.tile_tokens = kTileRows / p.b.groups;
+    p.by_group = 65536 / p.b.groups + 1;
     const bool large = attn_large(tokens, p.b.groups, starts == nullptr);
     const AttnLayout L = attn_layout(tokens, p.b.kv_heads, cache->head_dim, large);
     char* ws = static_cast<char*>(workspace);
