@@ -77,7 +77,10 @@ constexpr int kTargetSmall = TSMALL;     // pieces aimed at: batches of small ti
 constexpr int kTargetLarge = TLARGE;      // others
 constexpr int kSmallMin = 2;           // fewest chunks of a small piece: a step of 32 keys a wave
 constexpr int kLargeMin = 4;
-constexpr int kJoinThreads = 512;
+#ifndef JT
+#define JT 256
+#endif
+constexpr int kJoinThreads = JT;
 
 struct PagedAttnParams {
     PagedBatch b;
@@ -1065,12 +1068,13 @@ __global__ __launch_bounds__(kBlock, LARGE ? 2 : OCC) void paged_attention_kerne
     else if constexpr (LARGE) large_tile<D>(p, w, span, c0, c1, S.large);
 }
 
-// Join the parts of one token's heads of one kv head: thread (group of
-// parts, pair of values).
+// Join the parts of one token's heads of one kv head: thread (set of parts,
+// four values), the parts' loads four at a time ahead of their use.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParams p)
 {
-    __shared__ float so[kJoinThreads][2], sl[kJoinThreads], sm[kJoinThreads];
+    __shared__ float4v so[kJoinThreads];
+    __shared__ float sl[kJoinThreads], sm[kJoinThreads];
     const int t = blockIdx.x, h = blockIdx.y;
     const int2 d = p.desc[size_t(t) * p.b.kv_heads + h];   // (of any contents where the row is nobody's)
     const int ordered = *p.ordered;
@@ -1078,52 +1082,53 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
     if (paged_sequence(p.b, t, &first, &count) < 0 || ordered == 0) return;
     const int pieces = d.x >> 1, stride = (d.x & 1) ? kSmallRows : kTileRows;
     if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) return;
-    const int pairs = p.b.groups * D / 2;                 // at most 512
-    const int sets = kJoinThreads / pairs;
-    const int set = threadIdx.x / pairs, pair = threadIdx.x % pairs;
-    const int r = pair / (D / 2);
-    float m = -__builtin_inff(), l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    const int quads = p.b.groups * D / 4;                 // at most 256
+    const int sets = kJoinThreads / quads;
+    const int set = threadIdx.x / quads, quad = threadIdx.x % quads;
+    const int r = quad / (D / 4), at = quad % (D / 4);
+    float m = -__builtin_inff(), l = 0.0f;
+    float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
     float lost = 0.0f;                                    // NaN where a part saw only scores of -inf
-    if (set < sets) {
-        for (int i = set; i < pieces; i += sets) {
-            const size_t row = size_t(d.y) + size_t(i) * stride + r;
-            const float2 ml = p.part_ml[row];
-            const float2 x = reinterpret_cast<const float2*>(p.part_o + row * D)[pair % (D / 2)];
-            if (ml.x == -__builtin_inff()) {
-                lost += ml.y;
-                continue;
-            }
-            const float top = fmaxf(m, ml.x);
-            const float a = exp2_fast(m - top), b = exp2_fast(ml.x - top);
-            l = l * a + ml.y * b;
-            o0 = o0 * a + x.x * b;
-            o1 = o1 * a + x.y * b;
-            m = top;
+    auto add = [&](float pm, float pl, const float4v& po) {
+        if (pm == -__builtin_inff()) {
+            lost += pl;
+            return;
         }
-    }
-    sm[threadIdx.x] = m;
-    sl[threadIdx.x] = m == -__builtin_inff() ? lost : l;
-    so[threadIdx.x][0] = o0;
-    so[threadIdx.x][1] = o1;
-    __syncthreads();
-    if (set != 0) return;
-    for (int k = 1; k < sets; ++k) {
-        const int i = k * pairs + pair;
-        if (sm[i] == -__builtin_inff()) {
-            lost += sl[i];
-            continue;
-        }
-        const float top = fmaxf(m, sm[i]);
-        const float a = exp2_fast(m - top), b = exp2_fast(sm[i] - top);
-        l = l * a + sl[i] * b;
-        o0 = o0 * a + so[i][0] * b;
-        o1 = o1 * a + so[i][1] * b;
+        const float top = fmaxf(m, pm);
+        const float a = exp2_fast(m - top), b = exp2_fast(pm - top);
+        l = l * a + pl * b;
+        o = o * a + po * b;
         m = top;
+    };
+    if (set < sets) {
+        for (int i0 = set; i0 < pieces; i0 += 4 * sets) {
+            float2 ml[4];
+            float4v x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * sets;
+                const size_t row = size_t(d.y) + size_t(i < pieces ? i : i0) * stride + r;
+                ml[k] = p.part_ml[row];
+                x[k] = reinterpret_cast<const float4v*>(p.part_o + row * D)[at];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i0 + k * sets < pieces) add(ml[k].x, ml[k].y, x[k]);
+        }
     }
-    float2 y = make_float2(o0 / l, o1 / l);
-    if (m == -__builtin_inff()) y = make_float2(lost, lost);   // nothing seen: 0; only scores of -inf: NaN
+    if (sets > 1) {
+        sm[threadIdx.x] = m;
+        sl[threadIdx.x] = m == -__builtin_inff() ? lost : l;
+        so[threadIdx.x] = o;
+        __syncthreads();
+        if (set != 0) return;
+        for (int k = 1; k < sets; ++k) add(sm[k * quads + quad], sl[k * quads + quad], so[k * quads + quad]);
+    }
+    const float f = 1.0f / l;
+    float4v y = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+    if (m == -__builtin_inff()) y = float4v{lost, lost, lost, lost};   // nothing seen: 0; only scores of -inf: NaN
     const size_t row = size_t(t) * p.b.heads + h * p.b.groups + r;
-    reinterpret_cast<float2*>(p.out + row * D)[pair % (D / 2)] = y;
+    reinterpret_cast<float4v*>(p.out + row * D)[at] = y;
 }
 
 // -------------------------------------------------------------------- host
