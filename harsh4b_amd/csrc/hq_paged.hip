@@ -20,76 +20,108 @@ struct AppendParams {
     float* query;                // [tokens, heads, D]
 };
 
-// One head's row of one token a wave, as prefill_qk_kernel: the spec's norm
-// (64 fmaf partials, halving tree) and rotation, so that K, V and q have the
-// decode step's bits.  Bound by HBM (a prompt) or latency (a token a sequence).
+// A token's heads (q, k, v) over the waves of gridDim.y blocks, PER at a time:
+// their loads together, then the spec's norm (64 fmaf partials, halving tree)
+// and rotation as the decode step's, so that K, V and q have its bits.  Bound
+// by HBM (a prompt) or latency (a token a sequence).
+#ifndef APP
+#define APP 4
+#endif
+#ifndef APT
+#define APT 1024
+#endif
+#ifndef APY
+#define APY 1
+#endif
+constexpr int kAppendPer = APP;
+
 template <int D>
 __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
 {
-    constexpr int PER = D == 128 ? 2 : 1;          // values a lane holds
+    constexpr int VALUES = D == 128 ? 2 : 1;       // a lane holds of a row
     const int t = blockIdx.x;
-    const int slot = blockIdx.y * (kBlock / kWave) + threadIdx.x / kWave;
     const int lane = threadIdx.x & (kWave - 1);
     const int heads = p.b.heads, kv_heads = p.b.kv_heads;
     const int total = heads + 2 * kv_heads;
-    if (slot >= total) return;
     const bool in = lane < D;
-    const float* src = p.qkv + (size_t(t) * total + slot) * D;
-    const float x0 = in ? src[lane] : 0.0f;
-    const float x1 = PER == 2 ? src[lane + 64] : 0.0f;
+    const int step = gridDim.y * (kBlock / kWave) * kAppendPer;
+    int slot0 = (blockIdx.y * (kBlock / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * kAppendPer;
+    if (slot0 >= total) return;
+    float x0[kAppendPer], x1[kAppendPer];
+    auto load = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < kAppendPer; ++i) {
+            const float* src = p.qkv + (size_t(t) * total + min(from + i, total - 1)) * D;
+            x0[i] = in ? src[lane] : 0.0f;
+            x1[i] = VALUES == 2 ? src[lane + 64] : 0.0f;
+        }
+    };
+    load(slot0);
     int first = 0, count = 0;
     const int b = paged_sequence(p.b, t, &first, &count);
     if (b < 0) return;
     const int pos = paged_position(p.b, b, count, t - first);
     const int page = paged_page(p.b, b, pos);
-    const bool is_q = slot < heads;
     const bool placed = pos >= 0 && pos < p.rope_positions && page >= 0;
-    if (!placed) {
-        if (lane == 0) atomicOr(p.b.status, HQ_PAGES_BAD);
-        if (is_q && in) {
-            float* qd = p.query + (size_t(t) * heads + slot) * D;
-            qd[lane] = 0.0f;
-            if (PER == 2) qd[lane + 64] = 0.0f;
-        }
-        return;
-    }
-    if (!is_q && (*p.b.status & HQ_PAGES_FULL)) return;
-    const size_t at = size_t(pos & (p.b.page_size - 1)) * D;
-    const size_t head = size_t(p.b.page_size) * D;
-    if (slot >= heads + kv_heads) {
-        uint16_t* vd = const_cast<uint16_t*>(p.b.values) +
-                       (size_t(page) * kv_heads + (slot - heads - kv_heads)) * head + at;
-        if (in) vd[lane] = f32_to_f16(x0);
-        if (PER == 2) vd[lane + 64] = f32_to_f16(x1);
-        return;
-    }
-    const float* w = is_q ? p.q_norm : p.k_norm;
-    float s = __builtin_fmaf(x0, x0, 0.0f);
-    if (PER == 2) s = __builtin_fmaf(x1, x1, s);
-    const float ss = wave_tree_sum64_all(s);
-    const float r = __builtin_sqrtf(ss / float(D) + p.eps);
+    const bool full = (*p.b.status & HQ_PAGES_FULL) != 0;
+    if (!placed && lane == 0) atomicOr(p.b.status, HQ_PAGES_BAD);
     // pairs (i, i + D/2): of D = 128 in one lane, else in lanes D/2 apart
-    const int i = PER == 2 ? lane : lane & (D / 2 - 1);
-    const float c0 = p.rope_cos[size_t(pos) * (D / 2) + i];
-    const float s0 = p.rope_sin[size_t(pos) * (D / 2) + i];
-    const float y0 = in ? (x0 / r) * w[lane] : 0.0f;
-    float a, b2 = 0.0f;
-    if (PER == 2) {
-        const float y1 = (x1 / r) * w[lane + 64];
-        a = y0 * c0 - y1 * s0;
-        b2 = y1 * c0 + y0 * s0;
-    } else {
-        const float other = __shfl_xor(y0, D / 2, kWave);
-        a = lane < D / 2 ? y0 * c0 - other * s0 : y0 * c0 + other * s0;
-    }
-    if (is_q) {
-        float* qd = p.query + (size_t(t) * heads + slot) * D;
-        if (in) qd[lane] = a;
-        if (PER == 2) qd[lane + 64] = b2;
-    } else {
-        uint16_t* kd = const_cast<uint16_t*>(p.b.keys) + (size_t(page) * kv_heads + (slot - heads)) * head + at;
-        if (in) kd[lane] = f32_to_f16(a);
-        if (PER == 2) kd[lane + 64] = f32_to_f16(b2);
+    const int pair = VALUES == 2 ? lane : lane & (D / 2 - 1);
+    const size_t rope = size_t(placed ? pos : 0) * (D / 2) + pair;
+    const float cos = p.rope_cos[rope], sin = p.rope_sin[rope];
+    const float qw0 = in ? p.q_norm[lane] : 0.0f, kw0 = in ? p.k_norm[lane] : 0.0f;
+    const float qw1 = VALUES == 2 ? p.q_norm[lane + 64] : 0.0f, kw1 = VALUES == 2 ? p.k_norm[lane + 64] : 0.0f;
+    // this position's K and V rows of kv head 0
+    const size_t head = size_t(p.b.page_size) * D;
+    const size_t at = size_t(max(page, 0)) * kv_heads * head + size_t(pos & (p.b.page_size - 1)) * D;
+    uint16_t* const krow = const_cast<uint16_t*>(p.b.keys) + at;
+    uint16_t* const vrow = const_cast<uint16_t*>(p.b.values) + at;
+    while (true) {
+        float y0[kAppendPer], y1[kAppendPer];
+#pragma unroll
+        for (int i = 0; i < kAppendPer; ++i) {
+            const int slot = slot0 + i;
+            if (slot >= heads + kv_heads) {        // v: as it is
+                y0[i] = x0[i];
+                y1[i] = x1[i];
+                continue;
+            }
+            const bool is_q = slot < heads;
+            float s = __builtin_fmaf(x0[i], x0[i], 0.0f);
+            if (VALUES == 2) s = __builtin_fmaf(x1[i], x1[i], s);
+            const float ss = wave_tree_sum64_all(s);
+            const float r = __builtin_sqrtf(ss / float(D) + p.eps);
+            const float a = (x0[i] / r) * (is_q ? qw0 : kw0);
+            if (VALUES == 2) {
+                const float c = (x1[i] / r) * (is_q ? qw1 : kw1);
+                y0[i] = a * cos - c * sin;
+                y1[i] = c * cos + a * sin;
+            } else {
+                const float z = in ? a : 0.0f;
+                const float other = __shfl_xor(z, D / 2, kWave);
+                y0[i] = lane < D / 2 ? z * cos - other * sin : z * cos + other * sin;
+                y1[i] = 0.0f;
+            }
+        }
+        const int done = slot0;
+        slot0 += step;
+        const bool more = slot0 < total;
+        if (more) load(slot0);
+#pragma unroll
+        for (int i = 0; i < kAppendPer; ++i) {
+            const int slot = done + i;
+            if (slot < heads) {
+                float* to = p.query + (size_t(t) * heads + slot) * D;
+                if (in) to[lane] = placed ? y0[i] : 0.0f;
+                if (VALUES == 2) to[lane + 64] = placed ? y1[i] : 0.0f;
+            } else if (slot < total && placed && !full) {
+                uint16_t* to = slot < heads + kv_heads ? krow + (slot - heads) * head
+                                                       : vrow + (slot - heads - kv_heads) * head;
+                if (in) to[lane] = f32_to_f16(y0[i]);
+                if (VALUES == 2) to[lane + 64] = f32_to_f16(y1[i]);
+            }
+        }
+        if (!more) return;
     }
 }
 
@@ -114,8 +146,10 @@ extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const in
     p.eps = eps;
     p.rope_positions = rope_positions;
     p.query = query;
+    // few tokens: kAppendPer heads a wave; from 4 tokens a CU on a block does a token
     const int slots = heads + 2 * cache->kv_heads;
-    const dim3 grid(tokens, (slots + 3) / 4);
+    const int per_block = kAppendPer * (kBlock / kWave);
+    const dim3 grid(tokens, tokens < APT ? (slots + per_block - 1) / per_block : APY);
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {
     case 16: hipLaunchKernelGGL(paged_append_kernel<16>, grid, dim3(kBlock), 0, s, p); break;

@@ -58,29 +58,16 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int kChunkKeys = 64;
 constexpr int kSmallRows = 16;
 constexpr int kTileRows = 128;
-#ifndef TSMALL
-#define TSMALL 512
-#endif
-#ifndef KAHEAD
-#define KAHEAD 2
-#endif
-#ifndef VAHEAD
-#define VAHEAD 3
-#endif
-#ifndef OCC
-#define OCC 2
-#endif
-#ifndef TLARGE
-#define TLARGE 512
-#endif
-constexpr int kTargetSmall = TSMALL;     // pieces aimed at: batches of small tiles only
-constexpr int kTargetLarge = TLARGE;      // others
+// Pieces aimed at: one for each place on the chip (two blocks a CU), all
+// started at once.  With twice as many, 16 windows of 1024 take 26.4 us
+// (22.2), 3 chats of 40960 101 (91), a question of 501 tokens 155 (143).
+constexpr int kTarget = 512;
 constexpr int kSmallMin = 2;           // fewest chunks of a small piece: a step of 32 keys a wave
 constexpr int kLargeMin = 4;
-#ifndef JT
-#define JT 256
-#endif
-constexpr int kJoinThreads = JT;
+// A chunk of a large tile counts as two of a small one: a step of 24 chats and
+// a prompt's 250 tokens takes 60.2 us so, 72.6 with 1, 74.1 with 3.
+constexpr int kLargeCost = 2;
+constexpr int kJoinThreads = 256;
 
 struct PagedAttnParams {
     PagedBatch b;
@@ -88,7 +75,6 @@ struct PagedAttnParams {
     float* out;
     int window, sinks;           // window 0: none
     int tile_tokens;             // tokens of a large tile
-    int target;                  // pieces aimed at
     int by_group;                // 65536 / groups + 1, for row_token
     int part_rows;               // rows of partial results there is room for
     int32_t* ordered;            // [1] starts never fall
@@ -192,6 +178,7 @@ struct SequencePlan {
     int length;                  // (a negative one counts as 0)
     int tile_tokens, tiles, chunks;   // chunks of the last tile (no other has more)
     bool small;
+    __device__ __forceinline__ int cost() const { return small ? 1 : kLargeCost; }   // of a chunk
 };
 
 __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, int b, bool* fall)
@@ -245,8 +232,8 @@ __device__ __forceinline__ int wave_prefix(int v)
 // Pieces a sequence's tiles are cut in for pieces of about `target` chunks.
 __device__ __forceinline__ int cuts_of(const SequencePlan& s, int target)
 {
-    const int size = max(target, s.small ? kSmallMin : kLargeMin);
-    return max(1, int(float(s.chunks) / float(size) + 0.5f));
+    const int size = max(target, s.small ? kSmallMin : kLargeMin * kLargeCost);
+    return max(1, int(float(s.chunks * s.cost()) / float(size) + 0.5f));
 }
 
 // The work of block `q`, the same in every wave; false: none.
@@ -259,7 +246,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     for (int base = 0; base < p.b.sequences; base += kWave) {
         if (base + lane < p.b.sequences) {
             mine = sequence_plan(p, base + lane, &fall);
-            units += int64_t(mine.tiles) * mine.chunks;
+            units += int64_t(mine.tiles) * mine.chunks * mine.cost();
         }
     }
     const bool ordered = !__any(fall);
@@ -269,7 +256,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     const int low = __builtin_amdgcn_readfirstlane(wave_isum64(int(units & 0xFFFFFF)));
     const int high = __builtin_amdgcn_readfirstlane(wave_isum64(int(min(units >> 24, int64_t(0xFFFFFF)))));
     units = ((int64_t(high) << 24) + low) * p.b.kv_heads;
-    const int target = int(min((units + p.target - 1) / p.target, int64_t(0x40000000)));
+    const int target = int(min((units + kTarget - 1) / kTarget, int64_t(0x40000000)));
     int pieces = 0, rows = 0;
     for (int base = 0; base < p.b.sequences; base += kWave) {
         const bool in = base + lane < p.b.sequences;
@@ -845,7 +832,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         // (a wave at its matrix instructions goes before one at its masks and
         // maxima: the SIMD's two waves then fall out of step, and overlap)
         __builtin_amdgcn_s_setprio(1);
-        constexpr int AHEAD = KAHEAD, VSET = VAHEAD + 1;
+        constexpr int AHEAD = 2, V_AHEAD = 3, VSET = V_AHEAD + 1;      // units whose operands are read ahead
         Weights now{};
         half8 ka[AHEAD + 1], va[VSET];
         uint32_t kb = 0, vb = 0;
@@ -861,7 +848,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             if constexpr (SC && i + AHEAD < UNITS) ka[(i + AHEAD) % (AHEAD + 1)] = k_unit(kb, i + AHEAD);
             if constexpr (WE && i == UNITS - 1) {
                 vb = opaque(v_lane + vbuf * kBufBytes + vt * 64 * D);
-                unrolled<(VAHEAD < VUNITS ? VAHEAD : VUNITS)>([&](auto q) { va[decltype(q)::value] = v_unit(vb, decltype(q)::value); });
+                unrolled<(V_AHEAD < VUNITS ? V_AHEAD : VUNITS)>([&](auto q) { va[decltype(q)::value] = v_unit(vb, decltype(q)::value); });
             }
             const half8 k = ka[i % (AHEAD + 1)];
             if constexpr (SC) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], next, 0, 0, 0);
@@ -879,7 +866,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             unrolled<VUNITS>([&](auto u) {
                 constexpr int i = decltype(u)::value;
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (i + VAHEAD < VUNITS) va[(i + VAHEAD) % VSET] = v_unit(vb, i + VAHEAD);
+                if constexpr (i + V_AHEAD < VUNITS) va[(i + V_AHEAD) % VSET] = v_unit(vb, i + V_AHEAD);
                 const half8 v = va[i % VSET];
                 acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8, now.lo[i / DT]), acc[i % DT], 0, 0, 0);
                 acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8, now.hi[i / DT]), acc[i % DT], 0, 0, 0);
@@ -1048,7 +1035,7 @@ struct AttnShared<D, true> {
 };
 
 template <int D, bool LARGE>
-__global__ __launch_bounds__(kBlock, LARGE ? 2 : OCC) void paged_attention_kernel(PagedAttnParams p)
+__global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnParams p)
 {
     __shared__ AttnShared<D, LARGE> S;
     Piece w;
@@ -1137,14 +1124,14 @@ struct AttnLayout {
     int part_rows;
 };
 
-// Rows of partial results: pieces are of T >= work / target chunks, and a
+// Rows of partial results: pieces are of T >= work / kTarget chunks, and a
 // sequence of S > 1 pieces a tile has at least 1.5 T chunks a tile, so S <=
-// chunks / T + 1/2 < 2 chunks / T, and over all of them fewer than 2 target.
+// chunks / T + 1/2 < 2 chunks / T, and over all of them fewer than 2 kTarget.
 static AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large)
 {
     AttnLayout L;
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
-    L.part_rows = large ? 2 * kTargetLarge * kTileRows : 2 * kTargetSmall * kSmallRows;
+    L.part_rows = 2 * kTarget * (large ? kTileRows : kSmallRows);
     L.desc = 256;
     L.ml = L.desc + up(size_t(tokens) * kv_heads * sizeof(int2));
     L.o = L.ml + up(size_t(L.part_rows) * sizeof(float2));
@@ -1196,13 +1183,12 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     p.desc = reinterpret_cast<int2*>(ws + L.desc);
     p.part_ml = reinterpret_cast<float2*>(ws + L.ml);
     p.part_o = reinterpret_cast<float*>(ws + L.o);
-    p.target = large ? kTargetLarge : kTargetSmall;
     // chunks / T + 1 pieces a tile and kv head at most, so `target` and one of each in all; nor more than the
     // table's width allows.  A block without a piece ends at once.
     const int64_t tiles = large ? int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences)
                                 : std::min(tokens, p.b.sequences);
     const int64_t widest = (int64_t(cache->max_pages) * cache->page_size + kChunkKeys - 1) / kChunkKeys;
-    const int64_t blocks = std::min(p.target + tiles * p.b.kv_heads,
+    const int64_t blocks = std::min(kTarget + tiles * p.b.kv_heads,
                                     tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
     if (blocks > 0x7fffffff) return HQ_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
