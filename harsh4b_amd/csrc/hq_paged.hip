@@ -24,16 +24,8 @@ struct AppendParams {
 // their loads together, then the spec's norm (64 fmaf partials, halving tree)
 // and rotation as the decode step's, so that K, V and q have its bits.  Bound
 // by HBM (a prompt) or latency (a token a sequence).
-#ifndef APP
-#define APP 4
-#endif
-#ifndef APT
-#define APT 1024
-#endif
-#ifndef APY
-#define APY 1
-#endif
-constexpr int kAppendPer = APP;
+constexpr int kAppendPer = 2;
+constexpr int kAppendWide = 1024;      // tokens from which on a block does a whole token
 
 template <int D>
 __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
@@ -146,10 +138,11 @@ extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const in
     p.eps = eps;
     p.rope_positions = rope_positions;
     p.query = query;
-    // few tokens: kAppendPer heads a wave; from 4 tokens a CU on a block does a token
+    // few tokens: kAppendPer heads a wave (32 tokens 3.9 us); many: a block a token, whose waves look its place up
+    // once for all their heads (2000 tokens 18.2 us, 5.0 TB/s; with kAppendPer heads a wave 23.2)
     const int slots = heads + 2 * cache->kv_heads;
     const int per_block = kAppendPer * (kBlock / kWave);
-    const dim3 grid(tokens, tokens < APT ? (slots + per_block - 1) / per_block : APY);
+    const dim3 grid(tokens, tokens < kAppendWide ? (slots + per_block - 1) / per_block : 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {
     case 16: hipLaunchKernelGGL(paged_append_kernel<16>, grid, dim3(kBlock), 0, s, p); break;

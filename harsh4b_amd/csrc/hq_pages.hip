@@ -34,7 +34,7 @@ struct PagesParams {
     int32_t* b;                        // resize: copy flags per row; compact: targets
     int32_t* free_list;                // resize
     int32_t* owner;                    // resize: per page, the first row growing in it
-    int32_t* count;                    // resize: per page, the rows growing in it; compact: new place
+    int32_t* count;                    // resize: per page, the rows growing in it
     int32_t* items;                    // resize: per copy the source, the target's rank, the positions filled
     int32_t* snapshot;                 // fork: the table, then the lengths
 };
@@ -92,24 +92,47 @@ __device__ __forceinline__ ResizeRow resize_row(const PagesParams& p, int r)
     return d;
 }
 
+// The pages free in round `base` of the search: bit `lane` of is_free[k] for
+// page base + 1024 wave + 64 k + lane.
+__device__ __forceinline__ void free_pages(const PagesParams& p, uint32_t at, uint64_t (&is_free)[kPlanStep])
+{
+    const uint32_t pages = p.c.pages;
+    int refs[kPlanStep];
+#pragma unroll
+    for (int k = 0; k < kPlanStep; ++k) refs[k] = p.c.refs[min(at + k * kWave, pages - 1)];
+#pragma unroll
+    for (int k = 0; k < kPlanStep; ++k) is_free[k] = __ballot(at + k * kWave < pages && refs[k] == 0);
+}
+
+// Bound by latency: three dependent reads (lengths, table, refs), the first
+// 16384 pages' refs beside them, and the block's barriers.
 __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PagesParams p)
 {
     __shared__ int wave_sum[kPlanWaves];
     __shared__ int refuse, copies;
+    __shared__ int sources[kPlanThreads];
     const int t = threadIdx.x;
+    const int lane = t & (kWave - 1), wave = t / kWave;
     const int rows = p.c.sequences;
+    // up to 1024 rows: a thread keeps its row, and the rows that grow in one page find each other in LDS
+    const bool few = rows <= kPlanThreads;
+    uint64_t is_free[kPlanStep];
+    free_pages(p, wave * kWave * kPlanStep + lane, is_free);
+    ResizeRow mine{};
+    mine.source = -1;
     if (t == 0) refuse = copies = 0;
     __syncthreads();
     for (int r = t; r < rows; r += kPlanThreads) {
-        const ResizeRow d = resize_row(p, r);
-        if (d.bad) atomicOr(&refuse, HQ_PAGES_BAD);
-        else if (d.new_entries > p.c.max_pages) atomicOr(&refuse, HQ_PAGES_FULL);
-        if (d.source >= 0) {
-            publish_i(p.count + d.source, 0);
-            publish_i(p.owner + d.source, 0x7fffffff);
+        mine = resize_row(p, r);
+        if (mine.bad) atomicOr(&refuse, HQ_PAGES_BAD);
+        else if (mine.new_entries > p.c.max_pages) atomicOr(&refuse, HQ_PAGES_FULL);
+        if (!few && mine.source >= 0) {
+            publish_i(p.count + mine.source, 0);
+            publish_i(p.owner + mine.source, 0x7fffffff);
         }
     }
-    wait_all_memory();
+    sources[t] = few ? mine.source : -1;
+    if (!few) wait_all_memory();
     __syncthreads();
     if (refuse) {
         if (t == 0) {
@@ -118,63 +141,73 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PagesParams p
         }
         return;
     }
-    for (int r = t; r < rows; r += kPlanThreads) {
-        const ResizeRow d = resize_row(p, r);
-        if (d.source >= 0) {
-            atomicAdd(p.count + d.source, 1);
-            atomicMin(p.owner + d.source, r);
+    if (!few) {
+        for (int r = t; r < rows; r += kPlanThreads) {
+            const ResizeRow d = resize_row(p, r);
+            if (d.source >= 0) {
+                atomicAdd(p.count + d.source, 1);
+                atomicMin(p.owner + d.source, r);
+            }
         }
+        wait_all_memory();
+        __syncthreads();
     }
-    wait_all_memory();
-    __syncthreads();
     // new pages of each row, in the order of the table's entries
     int need = 0;
     for (int base = 0; base < rows; base += kPlanThreads) {
         const int r = base + t;
-        int mine = 0;
+        int new_pages = 0;
         bool copied = false;
-        ResizeRow d{};
         if (r < rows) {
-            d = resize_row(p, r);
-            if (d.source >= 0) {
-                const int held = p.c.refs[d.source];
-                copied = held > 1 && !(read_i(p.owner + d.source) == r && read_i(p.count + d.source) == held);
+            if (!few) mine = resize_row(p, r);
+            if (mine.source >= 0) {
+                const int held = p.c.refs[mine.source];
+                if (held > 1) {
+                    int first = r, grow = 1;
+                    if (few) {
+                        grow = 0;
+                        for (int i = rows - 1; i >= 0; --i)
+                            if (sources[i] == mine.source) {
+                                first = i;
+                                ++grow;
+                            }
+                    } else {
+                        first = read_i(p.owner + mine.source);
+                        grow = read_i(p.count + mine.source);
+                    }
+                    copied = !(first == r && grow == held);
+                }
             }
-            mine = max(0, d.new_entries - d.old_entries) + (d.hole || copied ? 1 : 0);
+            new_pages = max(0, mine.new_entries - mine.old_entries) + (mine.hole || copied ? 1 : 0);
             p.b[r] = copied;
         }
         int total;
-        const int rank = plan_scan(mine, wave_sum, &total);
+        const int rank = plan_scan(new_pages, wave_sum, &total);
         if (r < rows) p.a[r] = need + rank;
         if (copied) {
             int32_t* item = p.items + 3 * atomicAdd(&copies, 1);
-            item[0] = d.source;
+            item[0] = mine.source;
             item[1] = need + rank;
-            item[2] = d.old_len & (p.c.page_size - 1);
+            item[2] = mine.old_len & (p.c.page_size - 1);
         }
         // (rows x entries fits the table; past the pool the call is refused)
         need = need > p.c.pages ? need : need + total;
     }
     // the first `need` free pages: a wave looks at 1024 pages a round
-    const int lane = t & (kWave - 1), wave = t / kWave;
     int found = 0;
-    for (int64_t base = 0; base < p.c.pages && found < need; base += int64_t(kPlanThreads) * kPlanStep) {
-        const int64_t at = base + int64_t(wave) * kWave * kPlanStep + lane;
-        uint64_t is_free[kPlanStep];
+    for (uint32_t base = 0; base < uint32_t(p.c.pages) && found < need; base += kPlanThreads * kPlanStep) {
+        const uint32_t at = base + wave * kWave * kPlanStep + lane;
+        if (base > 0) free_pages(p, at, is_free);
         int n = 0;
 #pragma unroll
-        for (int k = 0; k < kPlanStep; ++k) {
-            const int64_t page = at + k * kWave;
-            is_free[k] = __ballot(page < p.c.pages && p.c.refs[page < p.c.pages ? page : 0] == 0);
-            n += __popcll(is_free[k]);
-        }
+        for (int k = 0; k < kPlanStep; ++k) n += __popcll(is_free[k]);
         int total;
         int rank = found + plan_scan(lane == 0 ? n : 0, wave_sum, &total);
         rank = __builtin_amdgcn_readfirstlane(rank);
 #pragma unroll
         for (int k = 0; k < kPlanStep; ++k) {
-            const int mine = rank + __popcll(is_free[k] & ((uint64_t(1) << lane) - 1));
-            if (((is_free[k] >> lane) & 1) && mine < need) p.free_list[mine] = int(at + k * kWave);
+            const int at_rank = rank + __popcll(is_free[k] & ((uint64_t(1) << lane) - 1));
+            if (((is_free[k] >> lane) & 1) && at_rank < need) p.free_list[at_rank] = int(at + k * kWave);
             rank += __popcll(is_free[k]);
         }
         found += total;
@@ -196,11 +229,19 @@ __device__ __forceinline__ void copy_segment(const hq_pages& c, int src, int dst
     uint16_t* pool = (lw & 1) ? c.values : c.keys;
     const size_t layer = size_t(lw >> 1) * c.pages;
     const size_t head = size_t(c.page_size) * c.head_dim;
-    const uint4* from = reinterpret_cast<const uint4*>(pool + ((layer + src) * c.kv_heads + h) * head);
-    uint4* to = reinterpret_cast<uint4*>(pool + ((layer + dst) * c.kv_heads + h) * head);
+    typedef uint32_t piece __attribute__((ext_vector_type(4)));
+    const piece* from = reinterpret_cast<const piece*>(pool + ((layer + src) * c.kv_heads + h) * head);
+    piece* to = reinterpret_cast<piece*>(pool + ((layer + dst) * c.kv_heads + h) * head);
     const int n = fill * c.head_dim / 8;             // 16-byte pieces (head_dim is a multiple of 16)
-    const int lane = threadIdx.x & (kWave - 1);
-    for (int i = lane; i < n; i += kWave) to[i] = from[i];
+    int i = threadIdx.x & (kWave - 1);
+    for (; i + 3 * kWave < n; i += 4 * kWave) {      // four loads under way, then the stores
+        const piece x0 = from[i], x1 = from[i + kWave], x2 = from[i + 2 * kWave], x3 = from[i + 3 * kWave];
+        to[i] = x0;
+        to[i + kWave] = x1;
+        to[i + 2 * kWave] = x2;
+        to[i + 3 * kWave] = x3;
+    }
+    for (; i < n; i += kWave) to[i] = from[i];
 }
 
 __global__ __launch_bounds__(kBlock) void resize_apply_kernel(PagesParams p)
@@ -253,6 +294,54 @@ __device__ __forceinline__ bool parents_ok(const PagesParams& p)
     return !__syncthreads_or(bad);
 }
 
+// Tables of up to kForkEntries entries: one block, which holds all that the
+// rows take over before it writes any.
+constexpr int kForkPer = 16, kForkEntries = kForkPer * kPlanThreads;
+
+__global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(PagesParams p)
+{
+    const hq_pages& c = p.c;
+    const int t = threadIdx.x, entries = c.sequences * c.max_pages;
+    int now[kForkPer], was[kForkPer], bad = 0;
+#pragma unroll
+    for (int k = 0; k < kForkPer; ++k) {
+        const int i = t + k * kPlanThreads;
+        now[k] = was[k] = 0;
+        if (i < entries) {
+            const int r = i / c.max_pages;
+            const int parent = p.want[r];
+            bad |= parent >= c.sequences;
+            was[k] = c.table[i];
+            now[k] = parent < 0 || parent >= c.sequences ? was[k] : c.table[i + (parent - r) * c.max_pages];
+        }
+    }
+    // (at most as many rows as entries: a row's length to the thread of its number, several rows a thread)
+    int lengths[kForkPer];
+#pragma unroll
+    for (int k = 0; k < kForkPer; ++k) {
+        const int r = t + k * kPlanThreads;
+        lengths[k] = 0;
+        if (r < c.sequences) {
+            const int parent = p.want[r];
+            lengths[k] = c.lengths[parent < 0 || parent >= c.sequences ? r : parent];
+        }
+    }
+    if (__syncthreads_or(bad)) {
+        if (t == 0) atomicOr(c.status, HQ_PAGES_BAD);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < kForkPer; ++k) {
+        const int i = t + k * kPlanThreads;
+        if (i < entries && was[k] != now[k]) {
+            if (was[k] >= 0 && was[k] < c.pages) atomicSub(c.refs + was[k], 1);
+            if (now[k] >= 0 && now[k] < c.pages) atomicAdd(c.refs + now[k], 1);
+            c.table[i] = now[k];
+        }
+        if (i < c.sequences) c.lengths[i] = lengths[k];
+    }
+}
+
 __global__ __launch_bounds__(kBlock) void fork_snapshot_kernel(PagesParams p)
 {
     const int r = blockIdx.x;
@@ -283,53 +372,61 @@ __global__ __launch_bounds__(kBlock) void fork_rows_kernel(PagesParams p)
 }
 
 // ------------------------------------------------------------- compaction
+// The pages to move (in use, at `live` and above) to a[], the free places below
+// `live` to b[], both ascending: a[i] goes to b[i].
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagesParams p)
 {
     __shared__ int wave_sum[kPlanWaves];
     const int t = threadIdx.x;
     const int lane = t & (kWave - 1), wave = t / kWave;
-    const int64_t pages = p.c.pages;
+    const uint32_t pages = p.c.pages;
+    const uint32_t round = kPlanThreads * kPlanStep;
+    uint64_t used[kPlanStep];              // of the round looked at last
+    auto look = [&](uint32_t at) {
+        int refs[kPlanStep];
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) refs[k] = p.c.refs[min(at + k * kWave, pages - 1)];
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) used[k] = __ballot(at + k * kWave < pages && refs[k] > 0);
+    };
     int n = 0;
-    for (int64_t page = t; page < pages; page += kPlanThreads) n += p.c.refs[page] > 0;
+    for (uint32_t base = 0; base < pages; base += round) {
+        look(base + wave * kWave * kPlanStep + lane);
+#pragma unroll
+        for (int k = 0; k < kPlanStep; ++k) n += __popcll(used[k]);
+    }
     int live;
-    plan_scan(n, wave_sum, &live);
+    plan_scan(lane == 0 ? n : 0, wave_sum, &live);
     int sources = 0, targets = 0;
-    for (int64_t base = 0; base < pages; base += int64_t(kPlanThreads) * kPlanStep) {
-        const int64_t at = base + int64_t(wave) * kWave * kPlanStep + lane;
-        uint64_t moves[kPlanStep];         // at and above `live`: pages in use; below: free ones
+    for (uint32_t base = 0; base < pages; base += round) {
+        const uint32_t at = base + wave * kWave * kPlanStep + lane;
+        if (pages > round) look(at);
         int above = 0, below = 0;
 #pragma unroll
         for (int k = 0; k < kPlanStep; ++k) {
-            const int64_t page = at + k * kWave;
-            const bool used = page < pages && p.c.refs[page < pages ? page : 0] > 0;
-            moves[k] = __ballot(page < pages && used == (page >= live));
-            const uint64_t high = __ballot(page >= live);
-            above += __popcll(moves[k] & high);
-            below += __popcll(moves[k] & ~high);
-            if (page < pages && page >= live) p.count[page] = int(page);   // (overwritten below where it moves)
+            const uint32_t page = at + k * kWave;
+            above += __popcll(used[k] & __ballot(page >= uint32_t(live)));
+            below += __popcll(~used[k] & __ballot(page < uint32_t(live)));
         }
-        int total_above, total_below;
-        int rank_above = sources + plan_scan(lane == 0 ? above : 0, wave_sum, &total_above);
-        int rank_below = targets + plan_scan(lane == 0 ? below : 0, wave_sum, &total_below);
-        rank_above = __builtin_amdgcn_readfirstlane(rank_above);
-        rank_below = __builtin_amdgcn_readfirstlane(rank_below);
+        // (both fit 15 bits a round: one sum for the two)
+        int total;
+        const int ranks = plan_scan(lane == 0 ? above << 16 | below : 0, wave_sum, &total);
+        int rank_above = sources + (__builtin_amdgcn_readfirstlane(ranks) >> 16);
+        int rank_below = targets + (__builtin_amdgcn_readfirstlane(ranks) & 0xFFFF);
+        const uint64_t under = (uint64_t(1) << lane) - 1;
 #pragma unroll
         for (int k = 0; k < kPlanStep; ++k) {
-            const int64_t page = at + k * kWave;
-            const uint64_t high = __ballot(page >= live);
-            const uint64_t up = moves[k] & high, down = moves[k] & ~high;
-            const uint64_t under = (uint64_t(1) << lane) - 1;
+            const uint32_t page = at + k * kWave;
+            const uint64_t up = used[k] & __ballot(page >= uint32_t(live));
+            const uint64_t down = ~used[k] & __ballot(page < uint32_t(live));
             if ((up >> lane) & 1) p.a[rank_above + __popcll(up & under)] = int(page);
             if ((down >> lane) & 1) p.b[rank_below + __popcll(down & under)] = int(page);
             rank_above += __popcll(up);
             rank_below += __popcll(down);
         }
-        sources += total_above;
-        targets += total_below;
+        sources += total >> 16;
+        targets += total & 0xFFFF;
     }
-    wait_all_memory();
-    __syncthreads();
-    for (int i = t; i < sources; i += kPlanThreads) p.count[p.a[i]] = p.b[i];
     if (t == 0) {
         p.head[1] = sources;
         p.head[2] = live;
@@ -337,6 +434,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagesParams 
     }
 }
 
+// Bound by HBM: 154 pages of 36 layers of 64 KB in 86 us, 4.9 TB/s.
 __global__ __launch_bounds__(kBlock) void compact_apply_kernel(PagesParams p)
 {
     const hq_pages& c = p.c;
@@ -346,7 +444,14 @@ __global__ __launch_bounds__(kBlock) void compact_apply_kernel(PagesParams p)
     const int64_t first = int64_t(blockIdx.x) * kBlock + threadIdx.x;
     for (int64_t i = first; i < int64_t(c.sequences) * c.max_pages; i += threads) {
         const int page = c.table[i];
-        if (page >= live && page < c.pages) c.table[i] = p.count[page];
+        if (page < live || page >= c.pages) continue;
+        int lo = 0, hi = moves;            // its place among the pages that move
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (p.a[mid] < page) lo = mid + 1;
+            else hi = mid;
+        }
+        if (lo < moves && p.a[lo] == page) c.table[i] = p.b[lo];
     }
     for (int64_t i = first; i < moves; i += threads) {
         c.refs[p.b[i]] = c.refs[p.a[i]];
@@ -395,8 +500,8 @@ static PagesParams pages_params(const hq_pages* c, void* workspace)
     return p;
 }
 
-// blocks of 256 threads that keep the memory busy (8 a CU)
-constexpr int kCopyBlocks = 2048;
+// blocks of 256 threads for page copies: 16 a CU (1024 to 8192 blocks differ by 2 %)
+constexpr int kCopyBlocks = 4096;
 
 }  // namespace hq
 
@@ -437,8 +542,12 @@ extern "C" int hq_pages_fork(const hq_pages* cache, const int32_t* parents, void
     hipStream_t s = static_cast<hipStream_t>(stream);
     PagesParams p = pages_params(cache, workspace);
     p.want = parents;
-    hipLaunchKernelGGL(fork_snapshot_kernel, dim3(cache->sequences), dim3(kBlock), 0, s, p);
-    hipLaunchKernelGGL(fork_rows_kernel, dim3(cache->sequences), dim3(kBlock), 0, s, p);
+    if (int64_t(cache->sequences) * cache->max_pages <= kForkEntries) {
+        hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
+    } else {
+        hipLaunchKernelGGL(fork_snapshot_kernel, dim3(cache->sequences), dim3(kBlock), 0, s, p);
+        hipLaunchKernelGGL(fork_rows_kernel, dim3(cache->sequences), dim3(kBlock), 0, s, p);
+    }
     return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
 }
 

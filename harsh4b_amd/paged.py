@@ -44,8 +44,8 @@ _pack = struct.Struct("8i6P").pack
 
 
 def _is(t, dtype, index: int) -> bool:
-    """Whether t is a contiguous tensor of that type on that GPU."""
-    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous())
+    """Whether the tensor t is contiguous, of that type and on that GPU."""
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
 
 
 def _refuse(name: str, t, dtype, index: int, what: str):
@@ -131,7 +131,7 @@ def _launch(entry, args: tuple, nbytes: int, index: int, stream, tensors, what: 
     one of the tensors' GPU) with a workspace of this call alone: memory of any
     contents from torch's allocator, which hands it out in the stream's order
     and inside a capture from the graph's own pool."""
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _launch(entry, args, nbytes, index, stream, tensors, what)
     if stream is None:
