@@ -68,6 +68,11 @@ constexpr int kLargeMin = 4;
 // a prompt's 250 tokens takes 60.2 us so, 72.6 with 1, 74.1 with 3.
 constexpr int kLargeCost = 2;
 constexpr int kJoinThreads = 256;
+// Tables of up to 8 chunks (512 positions): no tile is cut, and there is no
+// join to launch.  One chat of 256: 9.3 us (10.7 with both), of 512 11.5
+// (10.8, and the caller's time for a second launch, 3), of 768 13.8 (10.8);
+// 64 chats of 512 23.1 (24.7).
+constexpr int kWholeChunks = 8;
 
 struct PagedAttnParams {
     PagedBatch b;
@@ -76,6 +81,7 @@ struct PagedAttnParams {
     int window, sinks;           // window 0: none
     int tile_tokens;             // tokens of a large tile
     int by_group;                // 65536 / groups + 1, for row_token
+    bool whole;                  // no tile is cut (short tables): no join
     int part_rows;               // rows of partial results there is room for
     int32_t* ordered;            // [1] starts never fall
     int2* desc;                  // [tokens, kv_heads] 2 * pieces + small, first partial row
@@ -230,8 +236,9 @@ __device__ __forceinline__ int wave_prefix(int v)
 }
 
 // Pieces a sequence's tiles are cut in for pieces of about `target` chunks.
-__device__ __forceinline__ int cuts_of(const SequencePlan& s, int target)
+__device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequencePlan& s, int target)
 {
+    if (p.whole) return 1;
     const int size = max(target, s.small ? kSmallMin : kLargeMin * kLargeCost);
     return max(1, int(float(s.chunks * s.cost()) / float(size) + 0.5f));
 }
@@ -262,7 +269,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         const bool in = base + lane < p.b.sequences;
         if (p.b.sequences > kWave && in) mine = sequence_plan(p, base + lane, &fall);
         if (!in) mine.tiles = 0;
-        const int cuts = cuts_of(mine, target);
+        const int cuts = cuts_of(p, mine, target);
         const int here = mine.tiles * cuts * p.b.kv_heads;
         const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
         const int incl = wave_prefix(here), part_incl = wave_prefix(part);
@@ -1157,7 +1164,8 @@ static void launch_attention(const PagedAttnParams& p, bool large, int64_t block
 {
     if (large) hipLaunchKernelGGL((paged_attention_kernel<D, true>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     else hipLaunchKernelGGL((paged_attention_kernel<D, false>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
-    hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.b.tokens, p.b.kv_heads), dim3(kJoinThreads), 0, s, p);
+    if (!p.whole)
+        hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.b.tokens, p.b.kv_heads), dim3(kJoinThreads), 0, s, p);
 }
 
 extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens,
@@ -1188,8 +1196,10 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     const int64_t tiles = large ? int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences)
                                 : std::min(tokens, p.b.sequences);
     const int64_t widest = (int64_t(cache->max_pages) * cache->page_size + kChunkKeys - 1) / kChunkKeys;
-    const int64_t blocks = std::min(kTarget + tiles * p.b.kv_heads,
-                                    tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
+    p.whole = widest <= kWholeChunks;
+    const int64_t blocks = p.whole ? tiles * p.b.kv_heads
+                                   : std::min(kTarget + tiles * p.b.kv_heads,
+                                              tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
     if (blocks > 0x7fffffff) return HQ_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {

@@ -247,6 +247,19 @@ class Scene:
         return out.cpu().numpy()
 
     def check(self, window=0, sinks=0, starts=True, **more):
+        """With the table as it is, and as a row of a longer cache's: tiles
+        are cut in pieces and joined only where a table is long."""
+        got = self._check(window, sinks, starts, **more)
+        table, page = self.table, self.keys.shape[2]
+        wide = -(-1100 // page)
+        if table.shape[1] < wide:
+            self.table = np.full((table.shape[0], wide), -1, dtype=np.int32)
+            self.table[:, :table.shape[1]] = table
+            self._check(window, sinks, starts, **more)
+            self.table = table
+        return got
+
+    def _check(self, window=0, sinks=0, starts=True, **more):
         got = self.attend(window, sinks, starts, **more)
         expect, bound = _reference(self.query, self.keys, self.values, self.table, self.counts, self.lengths, window,
                                    sinks)
