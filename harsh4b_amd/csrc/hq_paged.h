@@ -11,6 +11,9 @@
 
 namespace hq {
 
+// Positions a table's row may hold: the last chunk's end still fits an int.
+constexpr int64_t kMaxPositions = 0x7fffff00;
+
 struct PagedBatch {
     const uint16_t* keys;        // [pages, kv_heads, page_size, D]
     const uint16_t* values;
@@ -69,8 +72,9 @@ inline int paged_check(const hq_pages* c, const void* rows, const int32_t* start
 {
     if (!c || !rows || !out || !c->keys || !c->values || !c->table || !c->lengths) return HQ_ERR_ARG;
     if (c->pages < 1 || c->kv_heads < 1 || c->sequences < 1 || c->max_pages < 1 || tokens < 0) return HQ_ERR_ARG;
+    if (c->kv_heads > 65535) return HQ_ERR_ARG;          // (a grid's y)
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return HQ_ERR_ARG;
-    if (int64_t(c->max_pages) * c->page_size > 0x7fffffff || int64_t(c->sequences) * c->max_pages > 0x7fffffff)
+    if (int64_t(c->max_pages) * c->page_size > kMaxPositions || int64_t(c->sequences) * c->max_pages > 0x7fffffff)
         return HQ_ERR_ARG;
     if (heads < 1 || heads % c->kv_heads || heads / c->kv_heads > 8) return HQ_ERR_ARG;
     if (c->head_dim != 16 && c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return HQ_ERR_ARG;

@@ -247,6 +247,18 @@ __device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequenceP
 __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piece& out)
 {
     const int lane = threadIdx.x & (kWave - 1);
+    if (p.whole && !p.b.starts) {              // a tile a block: nothing to count
+        out.b = uniform(unsigned(q) / unsigned(p.b.kv_heads));
+        out.head = q - out.b * p.b.kv_heads;
+        out.first = out.b;
+        out.n = 1;
+        out.length = uniform(max(0, p.b.lengths[out.b]));
+        out.pos = out.length - 1;
+        out.pieces = 1;
+        out.split = out.part = 0;
+        out.small = true;
+        return true;
+    }
     bool fall = false;
     int64_t units = 0;
     SequencePlan mine{};
@@ -1048,7 +1060,7 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnPar
     Piece w;
     if (!plan_piece(p, blockIdx.x, w)) return;
     // the join's directory: which rows have parts, and where
-    if (w.split == 0)
+    if (w.split == 0 && !p.whole)
         for (int i = threadIdx.x; i < w.n; i += kBlock)
             p.desc[size_t(w.first + i) * p.b.kv_heads + w.head] =
                 make_int2(2 * w.pieces + (w.small ? 1 : 0), w.part + i * p.b.groups);

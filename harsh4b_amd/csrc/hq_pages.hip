@@ -16,6 +16,7 @@
 
 #include "hq_device.h"
 #include "hq_internal.h"
+#include "hq_paged.h"
 
 namespace hq {
 
@@ -474,7 +475,7 @@ static bool pages_shape_ok(const hq_pages* c)
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return false;
     if (c->head_dim != 16 && c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return false;
     // a length is an int, and so is a table's size
-    return int64_t(c->max_pages) * c->page_size <= 0x7fffffff && int64_t(c->sequences) * c->max_pages <= 0x7fffffff;
+    return int64_t(c->max_pages) * c->page_size <= kMaxPositions && int64_t(c->sequences) * c->max_pages <= 0x7fffffff;
 }
 
 static PagesParams pages_params(const hq_pages* c, void* workspace)

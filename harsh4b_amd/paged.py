@@ -92,8 +92,8 @@ def _cache(index: int, keys, values, table, lengths, refs, status, dims: int, po
     if not _is(table, _I32, index) or table.dim() != 2:
         _refuse("table", table, _I32, index, "[sequences, max_pages]")
     sequences, max_pages = table.shape
-    if sequences == 0 or max_pages == 0 or max_pages * page_size > 0x7FFFFFFF or sequences * max_pages > 0x7FFFFFFF:
-        raise ValueError("table must be [sequences, max_pages] with fewer than 2^31 entries and positions a row")
+    if sequences == 0 or max_pages == 0 or max_pages * page_size > 0x7FFFFF00 or sequences * max_pages > 0x7FFFFFFF:
+        raise ValueError("table must be [sequences, max_pages] with fewer than 2^31 entries and 2^31 - 256 positions a row")
     length_ptr = ref_ptr = status_ptr = 0
     if lengths is not None:
         if not _is(lengths, _I32, index) or lengths.dim() != 1 or lengths.shape[0] != sequences:
@@ -199,6 +199,8 @@ def paged_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
         out = torch.empty((tokens, heads, d), dtype=_F32, device=qkv.device)
     elif not _is(out, _F32, index) or out.shape != (tokens, heads, d):
         _refuse("out", out, _F32, index, "[tokens, heads, head_dim]")
+    elif -4 * out.numel() < out.data_ptr() - qkv.data_ptr() < 4 * qkv.numel():
+        raise ValueError("out must not overlap qkv")
     if tokens:
         _launch(_native.lib().hq_paged_append,
                 (cache, qkv.data_ptr(), first, tokens, heads, q_norm.data_ptr(), k_norm.data_ptr(), eps,
@@ -238,6 +240,8 @@ def paged_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tenso
         out = torch.empty_like(query)
     elif not _is(out, _F32, index) or out.shape != shape:
         _refuse("out", out, _F32, index, "like query")
+    elif abs(out.data_ptr() - query.data_ptr()) < 4 * tokens * heads * d:
+        raise ValueError("out must not overlap query")
     if tokens:
         _launch(_native.lib().hq_paged_attention,
                 (cache, query.data_ptr(), first, tokens, heads, window, sinks, out.data_ptr()),

@@ -187,7 +187,9 @@ int hq_quant_int4_gemm(const float* x, const uint8_t* weights, const float* scal
  * keys + ((layer*pages + p)*kv_heads + h)*page_size*head_dim for kv head h:
  * one head's positions of a page are contiguous.  Everything lives on the
  * device, so a captured graph of these calls is valid at every length.
- * page_size: a power of two from 16 to 256; head_dim in {16, 32, 64, 128}.
+ * page_size: a power of two from 16 to 256; head_dim in {16, 32, 64, 128};
+ * max_pages * page_size below 2^31 - 255.  Calls on one cache run one after
+ * another (one stream, or streams that wait for each other).
  * Entries, lengths, starts and parents outside their ranges are never
  * followed: an entry counts as -1, and the calls that take a status report
  * HQ_PAGES_BAD. */
@@ -245,7 +247,8 @@ int hq_pages_compact(const hq_pages* cache, int32_t* live, void* workspace, void
  * falling; NULL: token b of sequence b, tokens = sequences) at positions
  * lengths[b] - n_b .. lengths[b] - 1.  A row at a position outside the cache
  * or the rope tables, or without a page, sets HQ_PAGES_BAD, writes no K/V
- * and a query of zeros; rows of no sequence are not touched.  While status
+ * and a query of zeros; rows of no sequence are not touched.  qkv
+ * and query must not overlap.  While status
  * has HQ_PAGES_FULL set no K/V is written (the lengths did not grow, so the
  * rows would land on earlier ones). */
 int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* starts, int tokens, int heads,
@@ -258,7 +261,7 @@ int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* star
  * j > p - window or j < sinks.  query, output fp32 [tokens, heads,
  * head_dim], heads ordered [kv_head, group], groups = heads/kv_heads <= 8.
  * A row that sees nothing gets zeros; rows of no sequence are not touched.
- * Values at positions past a sequence's length are never used, whatever they
+ * query and output must not overlap.  Values at positions past a sequence's length are never used, whatever they
  * hold.  status may be NULL.  `workspace`:
  * hq_paged_attention_workspace_bytes(...) bytes (single: nonzero where starts
  * is NULL), 256-byte aligned, of any contents. */

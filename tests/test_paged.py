@@ -40,7 +40,7 @@ def _struct(**change):
 
 
 BAD_SHAPES = [dict(pages=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(head_dim=24),
-              dict(head_dim=256), dict(kv_heads=0), dict(sequences=0), dict(max_pages=0), dict(max_pages=1 << 28)]
+              dict(head_dim=256), dict(kv_heads=0), dict(sequences=0), dict(max_pages=0), dict(max_pages=1 << 28), dict(max_pages=(1 << 27) - 15)]
 
 
 @pytest.mark.parametrize("change", BAD_SHAPES + [dict(keys=None), dict(table=None), dict(lengths=None)])
@@ -423,16 +423,46 @@ def test_large_and_small_values():
 
 
 @gpu
-def test_other_stream_and_in_place():
+def test_other_streams():
+    # a stream of the caller's, and two calls side by side on two streams: each has its own workspace
     from harsh4b_amd.paged import paged_attention
-    s = Scene([1, 40], [100, 90], page=16, seed=12)
-    expect = s.check()
-    stream = torch.cuda.Stream()
-    got = s.attend(stream=stream)
-    np.testing.assert_array_equal(got, expect)
-    d = s.device()
-    paged_attention(**d, starts=torch.from_numpy(s.starts).cuda(), out=d["query"])
-    np.testing.assert_array_equal(d["query"].cpu().numpy(), expect)
+    scenes = [Scene([1, 40], [100, 1090], page=16, seed=12), Scene([33, 2], [2000, 700], page=16, seed=13)]
+    expect = [s.check() for s in scenes]
+    np.testing.assert_array_equal(scenes[0].attend(stream=torch.cuda.Stream()), expect[0])
+    streams = [torch.cuda.Stream() for _ in scenes]
+    inputs = [(s.device(), torch.from_numpy(s.starts).cuda()) for s in scenes]
+    for _ in range(20):
+        outs = [paged_attention(**d, starts=a, stream=x) for (d, a), x in zip(inputs, streams)]
+    torch.cuda.synchronize()
+    for out, e in zip(outs, expect):
+        np.testing.assert_array_equal(out.cpu().numpy(), e)
+
+
+@gpu
+def test_outputs_over_inputs_are_refused():
+    from harsh4b_amd import paged
+    c = paged.PagedCache(1, 6, 2, 32, sequences=2, max_pages=2, page_size=16)
+    q = torch.zeros((5, 4, 32), device="cuda")
+    for out in (q[:2], q[1:3]):
+        with pytest.raises(ValueError, match="overlap"):
+            paged.paged_attention(q[:2], c.keys[0], c.values[0], c.table, c.lengths, out=out)
+    flat = torch.zeros(2 * 8 * 32 + 64, device="cuda")
+    rope = torch.ones((8, 16), device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        paged.paged_append(flat[:512].view(2, 256), torch.ones(32, device="cuda"), torch.ones(32, device="cuda"), rope,
+                           rope, 1e-6, c.keys[0], c.values[0], c.table, c.lengths, c.status,
+                           out=flat[320:576].view(2, 4, 32))
+
+
+@gpu
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+def test_queries_that_are_not_finite(what):
+    # a row's value makes its own result NaN and no other
+    s = Scene([1, 3, 60], [90, 150, 100], page=16, seed=41)
+    for t, h, i in ((0, 1, 7), (2, 5, 127), (30, 0, 0), (63, 7, 64)):
+        s.query[t, h, i] = float(what)
+    got = s.check()
+    assert np.isnan(got).any(axis=-1).sum() == 4
 
 
 @gpu
