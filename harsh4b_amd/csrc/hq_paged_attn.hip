@@ -68,6 +68,7 @@ constexpr int kLargeMin = 4;
 // a prompt's 250 tokens takes 60.2 us so, 72.6 with 1, 74.1 with 3.
 constexpr int kLargeCost = 2;
 constexpr int kJoinThreads = 256;
+constexpr int kJoinBlocks = 4096;
 // Tables of up to 8 chunks (512 positions): no tile is cut, and there is no
 // join to launch.  One chat of 256: 9.3 us (10.7 with both), of 512 11.5
 // (10.8, and the caller's time for a second launch, 3), of 768 13.8 (10.8);
@@ -83,7 +84,7 @@ struct PagedAttnParams {
     int by_group;                // 65536 / groups + 1, for row_token
     bool whole;                  // no tile is cut (short tables): no join
     int part_rows;               // rows of partial results there is room for
-    int32_t* ordered;            // [1] starts never fall
+    int32_t* cut;                // [1] whether any tile is cut (0 too where starts fall)
     int2* desc;                  // [tokens, kv_heads] 2 * pieces + small, first partial row
     float* part_o;               // [part_rows, D]
     float2* part_ml;             // [part_rows] m (of the scores times log2 e), l
@@ -268,15 +269,17 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
             units += int64_t(mine.tiles) * mine.chunks * mine.cost();
         }
     }
-    const bool ordered = !__any(fall);
-    if (q == 0 && threadIdx.x == 0) *p.ordered = ordered;
-    if (!ordered) return false;
+    if (__any(fall)) {
+        if (q == 0 && threadIdx.x == 0) *p.cut = 0;
+        return false;
+    }
     // (the sum of 64 in two parts that fit an int each)
     const int low = __builtin_amdgcn_readfirstlane(wave_isum64(int(units & 0xFFFFFF)));
     const int high = __builtin_amdgcn_readfirstlane(wave_isum64(int(min(units >> 24, int64_t(0xFFFFFF)))));
     units = ((int64_t(high) << 24) + low) * p.b.kv_heads;
     const int target = int(min((units + kTarget - 1) / kTarget, int64_t(0x40000000)));
     int pieces = 0, rows = 0;
+    bool got = false;
     for (int base = 0; base < p.b.sequences; base += kWave) {
         const bool in = base + lane < p.b.sequences;
         if (p.b.sequences > kWave && in) mine = sequence_plan(p, base + lane, &fall);
@@ -286,6 +289,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
         const int incl = wave_prefix(here), part_incl = wave_prefix(part);
         const uint64_t found = __ballot(q >= pieces + incl - here && q < pieces + incl);
+        got |= found != 0;
         if (found) {
             const int src = __builtin_ctzll(found);
             auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
@@ -315,12 +319,13 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
             out.pos = out.length - n + tile * tokens;
             out.part = first_part + (((tile * p.b.kv_heads + out.head) * out.pieces) + out.split) *
                                         (out.small ? kSmallRows : kTileRows);
-            return true;
+            if (q != 0) return true;
         }
         pieces += __builtin_amdgcn_readlane(incl, kWave - 1);
         rows += __builtin_amdgcn_readlane(part_incl, kWave - 1);
     }
-    return false;
+    if (q == 0 && threadIdx.x == 0) *p.cut = rows > 0;     // (block 0 goes through all sequences)
+    return got;
 }
 
 // ------------------------------------------------------------- query operands
@@ -1081,60 +1086,66 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 {
     __shared__ float4v so[kJoinThreads];
     __shared__ float sl[kJoinThreads], sm[kJoinThreads];
-    const int t = blockIdx.x, h = blockIdx.y;
-    const int2 d = p.desc[size_t(t) * p.b.kv_heads + h];   // (of any contents where the row is nobody's)
-    const int ordered = *p.ordered;
-    int first = 0, count = 0;
-    if (paged_sequence(p.b, t, &first, &count) < 0 || ordered == 0) return;
-    const int pieces = d.x >> 1, stride = (d.x & 1) ? kSmallRows : kTileRows;
-    if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) return;
+    const int cut = *p.cut;                               // (waited for beside the first row's loads)
     const int quads = p.b.groups * D / 4;                 // at most 256
     const int sets = kJoinThreads / quads;
     const int set = threadIdx.x / quads, quad = threadIdx.x % quads;
     const int r = quad / (D / 4), at = quad % (D / 4);
-    float m = -__builtin_inff(), l = 0.0f;
-    float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-    float lost = 0.0f;                                    // NaN where a part saw only scores of -inf
-    auto add = [&](float pm, float pl, const float4v& po) {
-        if (pm == -__builtin_inff()) {
-            lost += pl;
-            return;
-        }
-        const float top = fmaxf(m, pm);
-        const float a = exp2_fast(m - top), b = exp2_fast(pm - top);
-        l = l * a + pl * b;
-        o = o * a + po * b;
-        m = top;
-    };
-    if (set < sets) {
-        for (int i0 = set; i0 < pieces; i0 += 4 * sets) {
-            float2 ml[4];
-            float4v x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = i0 + k * sets;
-                const size_t row = size_t(d.y) + size_t(i < pieces ? i : i0) * stride + r;
-                ml[k] = p.part_ml[row];
-                x[k] = reinterpret_cast<const float4v*>(p.part_o + row * D)[at];
+    const unsigned all = unsigned(p.b.tokens) * unsigned(p.b.kv_heads);
+    for (unsigned i = blockIdx.x; i < all; i += gridDim.x) {
+        const int t = int(i / unsigned(p.b.kv_heads)), h = int(i - unsigned(t) * unsigned(p.b.kv_heads));
+        const int2 d = p.desc[i];                         // (of any contents where the row is nobody's)
+        int first = 0, count = 0;
+        const int b = paged_sequence(p.b, t, &first, &count);
+        if (cut == 0) return;
+        if (b < 0) continue;
+        const int pieces = d.x >> 1, stride = (d.x & 1) ? kSmallRows : kTileRows;
+        if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) continue;
+        float m = -__builtin_inff(), l = 0.0f;
+        float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float lost = 0.0f;                                // NaN where a part saw only scores of -inf
+        auto add = [&](float pm, float pl, const float4v& po) {
+            if (pm == -__builtin_inff()) {
+                lost += pl;
+                return;
             }
+            const float top = fmaxf(m, pm);
+            const float a = exp2_fast(m - top), b = exp2_fast(pm - top);
+            l = l * a + pl * b;
+            o = o * a + po * b;
+            m = top;
+        };
+        if (set < sets) {
+            for (int i0 = set; i0 < pieces; i0 += 4 * sets) {
+                float2 ml[4];
+                float4v x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (i0 + k * sets < pieces) add(ml[k].x, ml[k].y, x[k]);
+                for (int k = 0; k < 4; ++k) {
+                    const int j = i0 + k * sets;
+                    const size_t row = size_t(d.y) + size_t(j < pieces ? j : i0) * stride + r;
+                    ml[k] = p.part_ml[row];
+                    x[k] = reinterpret_cast<const float4v*>(p.part_o + row * D)[at];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i0 + k * sets < pieces) add(ml[k].x, ml[k].y, x[k]);
+            }
         }
+        if (sets > 1) {
+            __syncthreads();                              // (the last row's readers)
+            sm[threadIdx.x] = m;
+            sl[threadIdx.x] = m == -__builtin_inff() ? lost : l;
+            so[threadIdx.x] = o;
+            __syncthreads();
+            if (set != 0) continue;
+            for (int k = 1; k < sets; ++k) add(sm[k * quads + quad], sl[k * quads + quad], so[k * quads + quad]);
+        }
+        const float f = 1.0f / l;
+        float4v y = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+        if (m == -__builtin_inff()) y = float4v{lost, lost, lost, lost};   // nothing seen: 0; only scores of -inf: NaN
+        const size_t row = size_t(t) * p.b.heads + h * p.b.groups + r;
+        reinterpret_cast<float4v*>(p.out + row * D)[at] = y;
     }
-    if (sets > 1) {
-        sm[threadIdx.x] = m;
-        sl[threadIdx.x] = m == -__builtin_inff() ? lost : l;
-        so[threadIdx.x] = o;
-        __syncthreads();
-        if (set != 0) return;
-        for (int k = 1; k < sets; ++k) add(sm[k * quads + quad], sl[k * quads + quad], so[k * quads + quad]);
-    }
-    const float f = 1.0f / l;
-    float4v y = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
-    if (m == -__builtin_inff()) y = float4v{lost, lost, lost, lost};   // nothing seen: 0; only scores of -inf: NaN
-    const size_t row = size_t(t) * p.b.heads + h * p.b.groups + r;
-    reinterpret_cast<float4v*>(p.out + row * D)[at] = y;
 }
 
 // -------------------------------------------------------------------- host
@@ -1177,7 +1188,7 @@ static void launch_attention(const PagedAttnParams& p, bool large, int64_t block
     if (large) hipLaunchKernelGGL((paged_attention_kernel<D, true>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     else hipLaunchKernelGGL((paged_attention_kernel<D, false>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     if (!p.whole)
-        hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.b.tokens, p.b.kv_heads), dim3(kJoinThreads), 0, s, p);
+        hipLaunchKernelGGL(paged_join_kernel<D>, dim3(unsigned(std::min<int64_t>(kJoinBlocks, int64_t(p.b.tokens) * p.b.kv_heads))), dim3(kJoinThreads), 0, s, p);
 }
 
 extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens,
@@ -1199,7 +1210,7 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     const AttnLayout L = attn_layout(tokens, p.b.kv_heads, cache->head_dim, large);
     char* ws = static_cast<char*>(workspace);
     p.part_rows = L.part_rows;
-    p.ordered = reinterpret_cast<int32_t*>(ws);
+    p.cut = reinterpret_cast<int32_t*>(ws);
     p.desc = reinterpret_cast<int2*>(ws + L.desc);
     p.part_ml = reinterpret_cast<float2*>(ws + L.ml);
     p.part_o = reinterpret_cast<float*>(ws + L.o);
@@ -1212,7 +1223,7 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     const int64_t blocks = p.whole ? tiles * p.b.kv_heads
                                    : std::min(kTarget + tiles * p.b.kv_heads,
                                               tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
-    if (blocks > 0x7fffffff) return HQ_ERR_ARG;
+    if (blocks > 0x7fffffff || int64_t(tokens) * p.b.kv_heads > 0x7fffffff) return HQ_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {
     case 16: launch_attention<16>(p, large, blocks, s); break;
