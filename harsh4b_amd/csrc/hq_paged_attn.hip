@@ -380,6 +380,26 @@ __device__ __forceinline__ void split_weights(const float (&w)[8], half8& hi, ha
     lo = __builtin_bit_cast(half8, b);
 }
 
+// Over the lanes 16, 32 and 48 away (the four that hold one row of a small tile), in every lane.
+__device__ __forceinline__ float max_over_g(float v)
+{
+    unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+    swap32(a, b);
+    v = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    a = b = __builtin_bit_cast(unsigned, v);
+    swap16(a, b);
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float sum_over_g(float v)
+{
+    unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+    swap32(a, b);
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    a = b = __builtin_bit_cast(unsigned, v);
+    swap16(a, b);
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
 __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
 
 // The result of one row, by one wave in fp32 (see paged_row), as this piece's output or part.
@@ -518,8 +538,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 y[s][i] = used ? x[s][i >> 2][i & 3] : 0.0f;
                 top = fmaxf(top, __builtin_fabsf(y[s][i]));
             }
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = max_over_g(top);
         const int e = row_exponent(top);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) split8(y[s], e, qhi[s], qlo[s]);
@@ -568,8 +587,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         }
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        top = max_over_g(top);
         top = fmaxf(m, top);
         const float safe = top == -__builtin_inff() ? 0.0f : top;
         if (__any(top > m)) {
@@ -606,8 +624,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         pg1 = next1;
         j0 = nj;
     }
-    l += __shfl_xor(l, 16, kWave);
-    l += __shfl_xor(l, 32, kWave);
+    l = sum_over_g(l);
     // join the four waves: lane (n, g) holds row n, dims VEC (4 g + i) + v
     const uint64_t any_seen = __ballot(seen);
     const bool row_seen = ((any_seen | (any_seen >> 16) | (any_seen >> 32) | (any_seen >> 48)) >> n) & 1;
@@ -1073,8 +1090,12 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnPar
     // (the same in every lane: kept where the compiler knows it)
     span.sink = uniform(span.sink);
     span.first = uniform(span.first);
-    const int c0 = uniform(int(int64_t(span.count) * w.split / w.pieces));
-    const int c1 = uniform(int(int64_t(span.count) * (w.split + 1) / w.pieces));
+    int c0 = 0, c1 = uniform(span.count);
+    if (w.pieces > 1) {                        // count / pieces chunks each, the first ones one more
+        const int each = uniform(int(unsigned(c1) / unsigned(w.pieces))), more = c1 - each * w.pieces;
+        c0 = each * w.split + min(w.split, more);
+        c1 = c0 + each + (w.split < more ? 1 : 0);
+    }
     if (w.small) small_tile<D>(p, w, span, c0, c1, S.small);
     else if constexpr (LARGE) large_tile<D>(p, w, span, c0, c1, S.large);
 }
