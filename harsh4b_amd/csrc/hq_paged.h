@@ -13,6 +13,8 @@ namespace hq {
 
 // Positions a table's row may hold: the last chunk's end still fits an int.
 constexpr int64_t kMaxPositions = 0x7fffff00;
+// Blocks of 256 threads a launch can have.
+constexpr int64_t kMaxBlocks = 0xffffff;
 
 struct PagedBatch {
     const uint16_t* keys;        // [pages, kv_heads, page_size, D]
@@ -26,6 +28,23 @@ struct PagedBatch {
     int heads, kv_heads, groups;
 };
 
+// How many of the rising values at[1 .. n] are at most t (wave-uniform; every
+// lane calls it; at[0] must exist).  Each round of loads leaves a 64th of
+// them.  Of values that do not rise: some number from 0 to n.
+__device__ __forceinline__ int wave_count_upto(const int32_t* at, int n, int t)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    int low = 0;
+    while (n > kWave) {
+        const int stride = (n - 1) / kWave + 1;
+        const int i = (lane + 1) * stride;
+        const int past = __popcll(__ballot(i <= n && at[i <= n ? low + i : low] <= t));
+        low += past * stride;
+        n = min(stride - 1, n - past * stride);
+    }
+    return low + __popcll(__ballot(lane < n && at[lane < n ? low + 1 + lane : low] <= t));
+}
+
 // The sequence of a batch row (wave-uniform; every lane calls it), or -1; its first row and its rows.
 __device__ __forceinline__ int paged_sequence(const PagedBatch& p, int t, int* first, int* count)
 {
@@ -34,15 +53,7 @@ __device__ __forceinline__ int paged_sequence(const PagedBatch& p, int t, int* f
         *count = 1;
         return t < p.sequences ? t : -1;
     }
-    // sequences whose rows all lie at or before t
-    const int lane = threadIdx.x & (kWave - 1);
-    int b = 0;
-    for (int base = 1; base <= p.sequences; base += kWave) {
-        const int i = base + lane;
-        const int past = __popcll(__ballot(i <= p.sequences && p.starts[i <= p.sequences ? i : 0] <= t));
-        b += past;
-        if (past < kWave) break;
-    }
+    const int b = wave_count_upto(p.starts, p.sequences, t);
     if (b >= p.sequences) return -1;
     const int a = p.starts[b], z = p.starts[b + 1];
     *first = a;
@@ -72,7 +83,8 @@ inline int paged_check(const hq_pages* c, const void* rows, const int32_t* start
 {
     if (!c || !rows || !out || !c->keys || !c->values || !c->table || !c->lengths) return HQ_ERR_ARG;
     if (c->pages < 1 || c->kv_heads < 1 || c->sequences < 1 || c->max_pages < 1 || tokens < 0) return HQ_ERR_ARG;
-    if (c->kv_heads > 65535) return HQ_ERR_ARG;          // (a grid's y)
+    // (a grid's sizes: append has a block a token, and eight heads a block in y)
+    if (tokens > kMaxBlocks || c->sequences > kMaxBlocks || c->kv_heads > 32768) return HQ_ERR_ARG;
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return HQ_ERR_ARG;
     if (int64_t(c->max_pages) * c->page_size > kMaxPositions || int64_t(c->sequences) * c->max_pages > 0x7fffffff)
         return HQ_ERR_ARG;

@@ -74,6 +74,11 @@ constexpr int kJoinBlocks = 4096;
 // (10.8, and the caller's time for a second launch, 3), of 768 13.8 (10.8);
 // 64 chats of 512 23.1 (24.7).
 constexpr int kWholeChunks = 8;
+// From here on a launch of one block works the plan out for all sequences, and
+// a piece looks itself up (1024 chats of 300: 278 us, 376 with a plan in every
+// wave; 256: 82 and 83; 128: 42 and 38).
+constexpr int kPlanSequences = 256;
+constexpr int kPlanThreads = 1024;
 
 struct PagedAttnParams {
     PagedBatch b;
@@ -83,8 +88,12 @@ struct PagedAttnParams {
     int tile_tokens;             // tokens of a large tile
     int by_group;                // 65536 / groups + 1, for row_token
     bool whole;                  // no tile is cut (short tables): no join
+    bool planned;                // the plan is in plan_first, plan_item, plan_count
     int part_rows;               // rows of partial results there is room for
     int32_t* cut;                // [1] whether any tile is cut (0 too where starts fall)
+    int32_t* plan_count;         // [1] sequences with rows
+    int32_t* plan_first;         // [count + 1] the first piece of each, and how many there are
+    int4* plan_item;             // [count] sequence, pieces a tile, first partial row
     int2* desc;                  // [tokens, kv_heads] 2 * pieces + small, first partial row
     float* part_o;               // [part_rows, D]
     float2* part_ml;             // [part_rows] m (of the scores times log2 e), l
@@ -244,6 +253,99 @@ __device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequenceP
     return max(1, int(float(s.chunks * s.cost()) / float(size) + 0.5f));
 }
 
+// Sequence b's piece number `local`, of `cuts` a tile; its partial rows start at first_part.
+__device__ __forceinline__ void place_piece(const PagedAttnParams& p, const SequencePlan& s, int b, int local, int cuts,
+                                            int first_part, Piece& out)
+{
+    out.b = b;
+    out.pieces = cuts;
+    out.small = s.small;
+    out.length = s.length;
+    int rest, tile;
+    if (out.small) {                                         // (one tile)
+        rest = unsigned(local) / unsigned(p.b.kv_heads);
+        out.split = rest;
+        tile = 0;
+    } else {
+        rest = unsigned(local) / unsigned(p.b.kv_heads);
+        const int done = unsigned(rest) / unsigned(out.pieces);
+        out.split = rest - done * out.pieces;
+        tile = s.tiles - 1 - done;                           // the longest first
+    }
+    tile = uniform(tile);
+    out.split = uniform(out.split);
+    out.head = uniform(local - rest * p.b.kv_heads);
+    out.first = s.first + tile * s.tile_tokens;
+    out.n = min(s.tile_tokens, s.n - tile * s.tile_tokens);
+    out.pos = out.length - s.n + tile * s.tile_tokens;
+    out.part = first_part + (((tile * p.b.kv_heads + out.head) * out.pieces) + out.split) *
+                                (out.small ? kSmallRows : kTileRows);
+}
+
+// Chunks a piece should have, for all the batch's chunks (of one kv head).
+__device__ __forceinline__ int piece_target(const PagedAttnParams& p, int64_t units)
+{
+    return int(min((units * p.b.kv_heads + kTarget - 1) / kTarget, int64_t(0x40000000)));
+}
+
+// The plan of many sequences, in one block: the sequences with rows in order,
+// their first pieces and partial rows.
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedAttnParams p)
+{
+    constexpr int WAVES = kPlanThreads / kWave;
+    __shared__ unsigned long long all_units;
+    __shared__ int falls;
+    __shared__ int3 wave_sum[WAVES];
+    const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
+    if (t == 0) all_units = 0, falls = 0;
+    __syncthreads();
+    bool fall = false;
+    int64_t units = 0;
+    SequencePlan mine{};
+    for (int b = t; b < p.b.sequences; b += kPlanThreads) {
+        mine = sequence_plan(p, b, &fall);
+        units += int64_t(mine.tiles) * mine.chunks * mine.cost();
+    }
+    if (units) atomicAdd(&all_units, static_cast<unsigned long long>(units));
+    if (fall) falls = 1;
+    __syncthreads();
+    int count = 0, pieces = 0, rows = 0;
+    if (!falls) {
+        const int target = piece_target(p, int64_t(all_units));
+        for (int base = 0; base < p.b.sequences; base += kPlanThreads) {
+            const int b = base + t;
+            if (p.b.sequences > kPlanThreads && b < p.b.sequences) mine = sequence_plan(p, b, &fall);
+            if (b >= p.b.sequences) mine.tiles = 0;
+            const int cuts = cuts_of(p, mine, target);
+            const int here = mine.tiles * cuts * p.b.kv_heads;
+            const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
+            const uint64_t has = __ballot(here > 0);
+            const int incl = wave_prefix(here), part_incl = wave_prefix(part);
+            __syncthreads();                   // (wave_sum's last readers)
+            if (lane == kWave - 1) wave_sum[wave] = make_int3(int(__popcll(has)), incl, part_incl);
+            __syncthreads();
+            int3 before = make_int3(count, pieces, rows);
+            for (int w = 0; w < WAVES; ++w) {
+                const int3 v = wave_sum[w];
+                if (w < wave) before.x += v.x, before.y += v.y, before.z += v.z;
+                count += v.x;
+                pieces += v.y;
+                rows += v.z;
+            }
+            if (here > 0) {                    // (a sequence with rows: no more than there are tokens)
+                const int at = before.x + int(__popcll(has & ((uint64_t(1) << lane) - 1)));
+                p.plan_first[at] = before.y + incl - here;
+                p.plan_item[at] = make_int4(b, cuts, before.z + part_incl - part, 0);
+            }
+        }
+    }
+    if (t == 0) {
+        p.plan_first[count] = pieces;
+        *p.plan_count = count;
+        *p.cut = rows > 0;
+    }
+}
+
 // The work of block `q`, the same in every wave; false: none.
 __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piece& out)
 {
@@ -261,6 +363,15 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         return true;
     }
     bool fall = false;
+    if (p.planned) {
+        const int count = *p.plan_count;
+        const int i = wave_count_upto(p.plan_first, count, q);
+        if (i >= count) return false;
+        const int4 item = p.plan_item[i];
+        const int b = uniform(item.x);
+        place_piece(p, sequence_plan(p, b, &fall), b, q - uniform(p.plan_first[i]), uniform(item.y), uniform(item.z), out);
+        return true;
+    }
     int64_t units = 0;
     SequencePlan mine{};
     for (int base = 0; base < p.b.sequences; base += kWave) {
@@ -276,8 +387,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     // (the sum of 64 in two parts that fit an int each)
     const int low = __builtin_amdgcn_readfirstlane(wave_isum64(int(units & 0xFFFFFF)));
     const int high = __builtin_amdgcn_readfirstlane(wave_isum64(int(min(units >> 24, int64_t(0xFFFFFF)))));
-    units = ((int64_t(high) << 24) + low) * p.b.kv_heads;
-    const int target = int(min((units + kTarget - 1) / kTarget, int64_t(0x40000000)));
+    const int target = piece_target(p, (int64_t(high) << 24) + low);
     int pieces = 0, rows = 0;
     bool got = false;
     for (int base = 0; base < p.b.sequences; base += kWave) {
@@ -293,32 +403,14 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         if (found) {
             const int src = __builtin_ctzll(found);
             auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
-            const int local = q - from(pieces + incl - here);
-            const int first_part = from(rows + part_incl - part);
-            out.pieces = from(cuts);
-            out.small = from(mine.small);
-            out.length = from(mine.length);
-            const int n = from(mine.n), tokens = from(mine.tile_tokens), tiles = from(mine.tiles);
-            out.b = base + src;
-            int rest, tile;
-            if (out.small) {                                         // (one tile)
-                rest = unsigned(local) / unsigned(p.b.kv_heads);
-                out.split = rest;
-                tile = 0;
-            } else {
-                rest = unsigned(local) / unsigned(p.b.kv_heads);
-                const int done = unsigned(rest) / unsigned(out.pieces);
-                out.split = rest - done * out.pieces;
-                tile = tiles - 1 - done;                             // the longest first
-            }
-            tile = uniform(tile);
-            out.split = uniform(out.split);
-            out.head = uniform(local - rest * p.b.kv_heads);
-            out.first = from(mine.first) + tile * tokens;
-            out.n = min(tokens, n - tile * tokens);
-            out.pos = out.length - n + tile * tokens;
-            out.part = first_part + (((tile * p.b.kv_heads + out.head) * out.pieces) + out.split) *
-                                        (out.small ? kSmallRows : kTileRows);
+            SequencePlan s;
+            s.first = from(mine.first);
+            s.n = from(mine.n);
+            s.length = from(mine.length);
+            s.tile_tokens = from(mine.tile_tokens);
+            s.tiles = from(mine.tiles);
+            s.small = from(mine.small);
+            place_piece(p, s, base + src, q - from(pieces + incl - here), from(cuts), from(rows + part_incl - part), out);
             if (q != 0) return true;
         }
         pieces += __builtin_amdgcn_readlane(incl, kWave - 1);
@@ -1171,7 +1263,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 
 // -------------------------------------------------------------------- host
 struct AttnLayout {
-    size_t desc, ml, o, total;
+    size_t first, item, desc, ml, o, total;
     int part_rows;
 };
 
@@ -1183,7 +1275,9 @@ static AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large
     AttnLayout L;
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
     L.part_rows = 2 * kTarget * (large ? kTileRows : kSmallRows);
-    L.desc = 256;
+    L.first = 256;                             // (the plan's, of sequences with rows)
+    L.item = L.first + up((size_t(tokens) + 1) * sizeof(int32_t));
+    L.desc = L.item + up(size_t(tokens) * sizeof(int4));
     L.ml = L.desc + up(size_t(tokens) * kv_heads * sizeof(int2));
     L.o = L.ml + up(size_t(L.part_rows) * sizeof(float2));
     L.total = L.o + up(size_t(L.part_rows) * head_dim * sizeof(float));
@@ -1206,6 +1300,7 @@ extern "C" size_t hq_paged_attention_workspace_bytes(int tokens, int heads, int 
 template <int D>
 static void launch_attention(const PagedAttnParams& p, bool large, int64_t blocks, hipStream_t s)
 {
+    if (p.planned) hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
     if (large) hipLaunchKernelGGL((paged_attention_kernel<D, true>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     else hipLaunchKernelGGL((paged_attention_kernel<D, false>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     if (!p.whole)
@@ -1232,6 +1327,9 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     char* ws = static_cast<char*>(workspace);
     p.part_rows = L.part_rows;
     p.cut = reinterpret_cast<int32_t*>(ws);
+    p.plan_count = p.cut + 1;
+    p.plan_first = reinterpret_cast<int32_t*>(ws + L.first);
+    p.plan_item = reinterpret_cast<int4*>(ws + L.item);
     p.desc = reinterpret_cast<int2*>(ws + L.desc);
     p.part_ml = reinterpret_cast<float2*>(ws + L.ml);
     p.part_o = reinterpret_cast<float*>(ws + L.o);
@@ -1244,7 +1342,8 @@ extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, con
     const int64_t blocks = p.whole ? tiles * p.b.kv_heads
                                    : std::min(kTarget + tiles * p.b.kv_heads,
                                               tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
-    if (blocks > 0x7fffffff || int64_t(tokens) * p.b.kv_heads > 0x7fffffff) return HQ_ERR_ARG;
+    p.planned = cache->sequences >= kPlanSequences && !(p.whole && !starts);
+    if (blocks > kMaxBlocks || int64_t(tokens) * p.b.kv_heads > 0x7fffffff) return HQ_ERR_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (cache->head_dim) {
     case 16: launch_attention<16>(p, large, blocks, s); break;
