@@ -59,6 +59,7 @@ class HqPages(ctypes.Structure):
 
 HQ_PAGES_FULL = 1
 HQ_PAGES_BAD = 2
+HQ_PAGES_REFUSED = 4
 HQ_STEP_BAD_TOKEN = 1
 HQ_STEP_FULL = 2
 HQ_STEP_SYNC = 4

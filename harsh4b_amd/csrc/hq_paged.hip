@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
     const int pos = paged_position(p.b, b, count, t - first);
     const int page = paged_page(p.b, b, pos);
     const bool placed = pos >= 0 && pos < p.rope_positions && page >= 0;
-    const bool full = (*p.b.status & HQ_PAGES_FULL) != 0;
+    const bool held = (*p.b.status & (HQ_PAGES_FULL | HQ_PAGES_REFUSED)) != 0;
     if (!placed && lane == 0) atomicOr(p.b.status, HQ_PAGES_BAD);
     // pairs (i, i + D/2): of D = 128 in one lane, else in lanes D/2 apart
     const int pair = VALUES == 2 ? lane : lane & (D / 2 - 1);
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
                 float* to = p.query + (size_t(t) * heads + slot) * D;
                 if (in) to[lane] = placed ? y0[i] : 0.0f;
                 if (VALUES == 2) to[lane + 64] = placed ? y1[i] : 0.0f;
-            } else if (slot < total && placed && !full) {
+            } else if (slot < total && placed && !held) {
                 uint16_t* to = slot < heads + kv_heads ? krow + (slot - heads) * head
                                                        : vrow + (slot - heads - kv_heads) * head;
                 if (in) to[lane] = f32_to_f16(y0[i]);

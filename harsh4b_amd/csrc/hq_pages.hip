@@ -68,7 +68,6 @@ struct ResizeRow {
     int old_len, new_len;
     int old_entries, new_entries;      // table entries the two lengths need
     int source;                        // page the growth goes on writing to, or -1
-    bool hole;                         // that page is missing
     bool bad;
 };
 
@@ -83,12 +82,11 @@ __device__ __forceinline__ ResizeRow resize_row(const PagesParams& p, int r)
     d.old_entries = int((int64_t(d.old_len) + ps - 1) >> p.shift);
     d.new_entries = int((int64_t(d.new_len) + ps - 1) >> p.shift);
     d.source = -1;
-    d.hole = false;
     if (!d.bad && d.new_len > d.old_len && (d.old_len & (ps - 1))) {
         const int e = d.old_len >> p.shift;
         const int page = p.c.table[size_t(r) * p.c.max_pages + e];
         if (page >= 0 && page < p.c.pages) d.source = page;
-        else d.hole = true;
+        else d.bad = true;             // (another in its place would hold some other sequence's rows)
     }
     return d;
 }
@@ -137,7 +135,7 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PagesParams p
     __syncthreads();
     if (refuse) {
         if (t == 0) {
-            atomicOr(p.c.status, refuse);
+            atomicOr(p.c.status, refuse | (refuse & HQ_PAGES_BAD ? HQ_PAGES_REFUSED : 0));
             p.head[0] = 0;
         }
         return;
@@ -179,7 +177,7 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PagesParams p
                     copied = !(first == r && grow == held);
                 }
             }
-            new_pages = max(0, mine.new_entries - mine.old_entries) + (mine.hole || copied ? 1 : 0);
+            new_pages = max(0, mine.new_entries - mine.old_entries) + (copied ? 1 : 0);
             p.b[r] = copied;
         }
         int total;
@@ -252,7 +250,7 @@ __global__ __launch_bounds__(kBlock) void resize_apply_kernel(PagesParams p)
     for (int r = blockIdx.x; r < c.sequences; r += gridDim.x) {
         const ResizeRow d = resize_row(p, r);
         const int rank = p.a[r];
-        const bool fresh_source = d.hole || p.b[r] != 0;
+        const bool fresh_source = p.b[r] != 0;
         const int e0 = d.old_len >> p.shift;             // the partly filled page's entry
         // positions no query from here on sees: [sinks, low)
         const int64_t low = p.window > 0 ? int64_t(min(d.old_len, d.new_len)) - p.window + 1 : 0;
@@ -328,7 +326,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(PagesParams p)
         }
     }
     if (__syncthreads_or(bad)) {
-        if (t == 0) atomicOr(c.status, HQ_PAGES_BAD);
+        if (t == 0) atomicOr(c.status, HQ_PAGES_BAD | HQ_PAGES_REFUSED);
         return;
     }
 #pragma unroll
@@ -356,7 +354,7 @@ __global__ __launch_bounds__(kBlock) void fork_rows_kernel(PagesParams p)
     const hq_pages& c = p.c;
     const int r = blockIdx.x;
     if (!parents_ok(p)) {
-        if (r == 0 && threadIdx.x == 0) atomicOr(c.status, HQ_PAGES_BAD);
+        if (r == 0 && threadIdx.x == 0) atomicOr(c.status, HQ_PAGES_BAD | HQ_PAGES_REFUSED);
         return;
     }
     const int parent = p.want[r];
@@ -474,6 +472,8 @@ static bool pages_shape_ok(const hq_pages* c)
     if (!c || c->layers < 1 || c->pages < 1 || c->kv_heads < 1 || c->sequences < 1 || c->max_pages < 1) return false;
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return false;
     if (c->head_dim != 16 && c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return false;
+    // (a fork of a large table has a block a sequence)
+    if (c->sequences > kMaxBlocks) return false;
     // a length is an int, and so is a table's size
     return int64_t(c->max_pages) * c->page_size <= kMaxPositions && int64_t(c->sequences) * c->max_pages <= 0x7fffffff;
 }

@@ -265,7 +265,9 @@ def pages_resize(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
     lowest free pages, and copies the partly filled page it goes on in where
     others hold it too; shrinking releases pages, and `window` > 0 those that
     no later query sees.  Too few free pages, or a length past the table, set
-    HQ_PAGES_FULL in `status` and change nothing."""
+    HQ_PAGES_FULL in `status` and change nothing; so does, with HQ_PAGES_BAD
+    and HQ_PAGES_REFUSED, growth from the middle of a page that was
+    released."""
     if lengths is None or refs is None or status is None:
         raise ValueError("pages_resize needs lengths, refs and status")
     index = _index(table)

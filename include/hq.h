@@ -188,8 +188,9 @@ int hq_quant_int4_gemm(const float* x, const uint8_t* weights, const float* scal
  * one head's positions of a page are contiguous.  Everything lives on the
  * device, so a captured graph of these calls is valid at every length.
  * page_size: a power of two from 16 to 256; head_dim in {16, 32, 64, 128};
- * max_pages * page_size below 2^31 - 255.  Calls on one cache run one after
- * another (one stream, or streams that wait for each other).
+ * max_pages * page_size below 2^31 - 255; fewer than 2^24 sequences and
+ * tokens.  Calls on one cache run one after another (one stream, or streams
+ * that wait for each other).
  * Entries, lengths, starts and parents outside their ranges are never
  * followed: an entry counts as -1, and the calls that take a status report
  * HQ_PAGES_BAD. */
@@ -208,6 +209,7 @@ typedef struct hq_pages {
 
 #define HQ_PAGES_FULL 1   /* too few free pages, or a sequence past max_pages: that call changed nothing */
 #define HQ_PAGES_BAD 2    /* an entry, length, start or parent outside its range */
+#define HQ_PAGES_REFUSED 4 /* with HQ_PAGES_BAD: a resize or a fork was refused for it and changed nothing */
 
 /* Set the lengths: sequence b goes to new_lengths[b] positions (device int32
  * [sequences]; negative: unchanged).  A growing sequence gets the pages it
@@ -219,8 +221,9 @@ typedef struct hq_pages {
  * call are free for the next call, not for this one.  With window > 0 every
  * sequence also releases the pages that no query from position min(old, new)
  * on sees under that window and `sinks` (hq_paged_attention); their entries
- * become -1.  All or nothing: HQ_PAGES_FULL or HQ_PAGES_BAD leave everything
- * as it was.  `workspace`: hq_pages_workspace_bytes(cache) bytes, 256-byte
+ * become -1 (a sequence cut back to where it goes on in such an entry cannot
+ * grow again: HQ_PAGES_BAD).  All or nothing: a refused call leaves
+ * everything as it was.  `workspace`: hq_pages_workspace_bytes(cache) bytes, 256-byte
  * aligned, of any contents. */
 size_t hq_pages_workspace_bytes(const hq_pages* cache);
 int hq_pages_resize(const hq_pages* cache, const int32_t* new_lengths, int window, int sinks, void* workspace,
@@ -249,8 +252,10 @@ int hq_pages_compact(const hq_pages* cache, int32_t* live, void* workspace, void
  * or the rope tables, or without a page, sets HQ_PAGES_BAD, writes no K/V
  * and a query of zeros; rows of no sequence are not touched.  qkv
  * and query must not overlap.  While status
- * has HQ_PAGES_FULL set no K/V is written (the lengths did not grow, so the
- * rows would land on earlier ones). */
+ * has HQ_PAGES_FULL or HQ_PAGES_REFUSED set no K/V is written (the lengths
+ * did not grow, so the rows would land on earlier ones).  A page that several
+ * entries hold is written for all of them: hq_pages_resize gives a growing
+ * sequence its own. */
 int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* starts, int tokens, int heads,
                     const float* q_norm, const float* k_norm, float eps, const float* rope_cos,
                     const float* rope_sin, int rope_positions, float* query, void* stream);
@@ -261,9 +266,9 @@ int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* star
  * j > p - window or j < sinks.  query, output fp32 [tokens, heads,
  * head_dim], heads ordered [kv_head, group], groups = heads/kv_heads <= 8.
  * A row that sees nothing gets zeros; rows of no sequence are not touched.
- * query and output must not overlap.  Values at positions past a sequence's length are never used, whatever they
- * hold.  status may be NULL.  `workspace`:
- * hq_paged_attention_workspace_bytes(...) bytes (single: nonzero where starts
+ * query and output must not overlap.  Values at positions past a sequence's
+ * length are never used, whatever they hold.  status may be NULL.
+ * `workspace`: hq_paged_attention_workspace_bytes(...) bytes (single: nonzero where starts
  * is NULL), 256-byte aligned, of any contents. */
 size_t hq_paged_attention_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim, int single);
 int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens, int heads,

@@ -74,6 +74,7 @@ def test_c_entries_refuse_bad_arguments():
     assert at(c, p + 4, None, 3, 4, 0, 0, p, p, None) == 2 and at(c, p, None, 3, 4, 0, 0, p + 8, p, None) == 2
     assert at(c, p, None, 3, 4, 0, 0, p, p + 16, None) == 2          # workspace: 256 bytes
     assert at(c, p, p, 0, 4, 0, 0, p, p, None) == 0                  # no rows: nothing to do
+    assert at(c, p, p, 2**24, 4, 0, 0, p, p, None) == 1              # more blocks than a launch has
     ap = lib.hq_paged_append
     assert ap(c, p, None, 3, 4, None, p, 1e-6, p, p, 10, p, None) == 1
     assert ap(c, p, None, 3, 4, p, p, 1e-6, p, p, 0, p, None) == 1   # rope positions
@@ -82,6 +83,10 @@ def test_c_entries_refuse_bad_arguments():
     assert ap(ctypes.byref(n), p, None, 3, 4, p, p, 1e-6, p, p, 10, p, None) == 1
     assert lib.hq_pages_resize(ctypes.byref(n), p, 0, 0, p, None) == 1
     assert lib.hq_pages_fork(ctypes.byref(n), p, p, None) == 1
+    many, _, _ = _struct(sequences=2**24, max_pages=1)
+    assert at(ctypes.byref(many), p, p, 5, 4, 0, 0, p, p, None) == 1
+    assert lib.hq_pages_workspace_bytes(ctypes.byref(many)) == 0
+    assert lib.hq_pages_fork(ctypes.byref(many), p, p, None) == 1
     for bad in (dict(keys=p + 8), dict(values=p + 2)):
         u, _, _ = _struct(**bad)
         assert at(ctypes.byref(u), p, None, 3, 4, 0, 0, p, p, None) == 2
@@ -381,6 +386,54 @@ def test_starts_out_of_order(starts):
 
 
 @gpu
+@pytest.mark.parametrize("sequences", [255, 256, 300, 1300])
+def test_many_sequences(sequences):
+    # the plan in every wave, and in a launch of its own (more than one round of its block)
+    from harsh4b_amd.paged import paged_attention
+    rng = np.random.default_rng(sequences)
+    counts = rng.integers(0, 4, sequences)
+    counts[[0, 7, sequences - 1]] = 30, 0, 9
+    lengths = counts + rng.integers(0, 60, sequences)
+    lengths[[0, 9, 200, 254]] = 700, 900, 30, 301
+    s = Scene(counts.tolist(), lengths.tolist(), 1, 2, 16, seed=sequences)
+    s.check()
+    s.check(window=40, sinks=5)
+    one = Scene([1] * sequences, np.maximum(lengths, 1).tolist(), 2, 2, 16, seed=sequences)
+    one.check(starts=False)
+    s.starts[100] = s.starts[101] + 1              # starts that fall: no row is touched
+    out = torch.full((s.tokens, 2, 16), 7.0, device="cuda")
+    paged_attention(**s.device(), starts=torch.from_numpy(s.starts).cuda(), out=out)
+    assert (out == 7.0).all()
+
+
+@gpu
+@pytest.mark.parametrize("sequences", [64, 65, 128, 129, 4096, 4097])
+def test_rows_find_their_sequence(sequences):
+    # one row each, at the borders of the search; every third sequence without a row
+    from harsh4b_amd.paged import paged_attention
+    counts = np.array([0 if b % 3 == 1 else 1 for b in range(sequences)])
+    s = Scene(counts.tolist(), [3] * sequences, 1, 1, 16, seed=sequences)
+    s.values[:] = 0.0
+    for b in range(sequences):
+        for j in range(3):
+            s.values[s.place(b, j)] = b % 2048
+    starts = torch.from_numpy(s.starts).cuda()
+    out = paged_attention(**s.device(), starts=starts).cpu().numpy()
+    np.testing.assert_allclose(out[:, 0, 0], np.flatnonzero(counts) % 2048, rtol=1e-5)
+    dev = s.dev
+    qkv = torch.zeros((s.tokens, 3 * 16), device="cuda")
+    qkv[:, 32:] = torch.arange(s.tokens, device="cuda")[:, None] % 2048
+    norm, rope = torch.ones(16, device="cuda"), torch.ones((3, 8), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    from harsh4b_amd.paged import paged_append
+    paged_append(qkv, norm, norm, rope, rope, 1e-6, dev["keys"], dev["values"], dev["table"], dev["lengths"], status,
+                 starts=starts)
+    assert int(status.item()) == 0
+    rows = dev["values"].cpu().numpy()[s.table[np.flatnonzero(counts), 0], 0, 2, 0]
+    np.testing.assert_array_equal(rows, np.arange(s.tokens) % 2048)
+
+
+@gpu
 @pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
 @pytest.mark.parametrize("count,window", [(1, 0), (1, 30), (3, 30), (60, 0), (60, 30)])
 def test_masked_places_of_any_value(what, count, window):
@@ -566,12 +619,13 @@ def test_append_of_rows_without_a_place():
     changed = {(int(p), int(j)) for p, _, j, _ in np.argwhere(before != after)}
     assert changed == {(int(s.table[b, j // 16]), j % 16) for b, j in [(0, 0), (0, 1), (2, 46), (2, 47), (3, 19)]}
     # a cache that could not grow takes no rows
-    status.fill_(native().HQ_PAGES_FULL)
-    dev = s.device()
-    paged_append(torch.from_numpy(inputs[0]).cuda(), *[torch.from_numpy(a).cuda() for a in inputs[1:]], 1e-6,
-                 dev["keys"], dev["values"], dev["table"], dev["lengths"], status,
-                 starts=torch.from_numpy(s.starts).cuda())
-    np.testing.assert_array_equal(dev["values"].cpu().numpy().view(np.uint16), before)
+    for code in native().HQ_PAGES_FULL, native().HQ_PAGES_REFUSED:
+        status.fill_(code)
+        dev = s.device()
+        paged_append(torch.from_numpy(inputs[0]).cuda(), *[torch.from_numpy(a).cuda() for a in inputs[1:]], 1e-6,
+                     dev["keys"], dev["values"], dev["table"], dev["lengths"], status,
+                     starts=torch.from_numpy(s.starts).cuda())
+        np.testing.assert_array_equal(dev["values"].cpu().numpy().view(np.uint16), before)
 
 
 # ------------------------------------------------------------------ page management
@@ -586,11 +640,17 @@ class Book:
     def resize(self, want, window=0, sinks=0):
         ps, self.copies = self.page, []
         new = [old if w < 0 else w for old, w in zip(self.lengths, want)]
-        if any(-(-n // ps) > len(self.table[0]) for n in new):
-            self.status |= 1
-            return False
         growing = [r for r, n in enumerate(new) if n > self.lengths[r]]
         writes = {r: self.table[r][self.lengths[r] // ps] for r in growing if self.lengths[r] % ps}
+        refused = 0
+        for r, n in enumerate(new):
+            if writes.get(r, 0) < 0:              # growth from the middle of a page that is not there
+                refused |= 6
+            elif -(-n // ps) > len(self.table[0]):
+                refused |= 1
+        if refused:
+            self.status |= refused
+            return False
         copied = []
         for r, p in writes.items():
             same = [x for x in writes if writes[x] == p]
@@ -601,8 +661,7 @@ class Book:
         for r, n in enumerate(new):
             old = self.lengths[r]
             for e in range(len(self.table[0])):
-                if (r in copied or (r in writes and writes[r] < 0)) and e == old // ps or \
-                        -(-old // ps) <= e < -(-n // ps):
+                if r in copied and e == old // ps or -(-old // ps) <= e < -(-n // ps):
                     taken.append((r, e))
         if len(taken) > len(free):
             self.status |= 1
@@ -734,7 +793,8 @@ def test_bad_books_are_refused():
     cache, book, pools, _ = _cache_and_book(3, 4, 9, 16)
     book.resize([20, 40, 5])
     cache.resize([20, 40, 5])
-    book.status = native().HQ_PAGES_BAD
+    refused = native().HQ_PAGES_BAD | native().HQ_PAGES_REFUSED
+    book.status = refused
     cache.fork([0, 3, 1])                          # no sequence 3: nothing changes
     _agree(cache, book, pools)
     with pytest.raises(ValueError, match="outside its range"):
@@ -744,18 +804,41 @@ def test_bad_books_are_refused():
         cache.lengths[1] = bad
         cache.status.zero_()
         cache.resize([21, -1, 6])
-        assert int(cache.status.item()) == native().HQ_PAGES_BAD
+        assert int(cache.status.item()) == refused
         cache.lengths.copy_(good)
         _agree(cache, book, pools)
-    # a partly filled page whose entry is bad is replaced, without a copy
-    cache.table[0, 1] = 100
-    book.table[0][1] = -1
+    # nothing grows from the middle of a page that is not there
+    for bad in (100, 9, -1, -7):
+        cache.table[0, 1] = bad
+        cache.status.zero_()
+        cache.resize([21, 41, -1])
+        assert int(cache.status.item()) == refused
+        cache.table[0, 1] = book.table[0][1]
+        _agree(cache, book, pools)
+
+
+@gpu
+def test_a_window_s_sequence_cut_back_too_far_does_not_grow():
+    cache, book, pools, _ = _cache_and_book(2, 20, 24, 16)
+    calls = [([200, 30], 0), ([210, 31], 50), ([206, 31], 50), ([208, 31], 0), ([70, 31], 0)]
+    for want, window in calls:                     # (position 70 is in a page that went with the window)
+        book.resize(want, window)
+        cache.resize(want, window)
+        _agree(cache, book, pools)
+    assert book.table[0][4] == -1 and book.status == 0
+    book.resize([71, 32])
+    cache.resize([71, 32])
+    assert book.status == native().HQ_PAGES_BAD | native().HQ_PAGES_REFUSED
+    _agree(cache, book, pools)
+    with pytest.raises(ValueError, match="outside its range"):
+        cache.check_status()
     cache.status.zero_()
     book.status = 0
-    book.resize([21, -1, -1])
-    cache.resize([21, -1, -1])
-    book.refs[1] = 1                               # the entry overwritten by hand still counts
-    _agree(cache, book, pools)
+    for want in [64, -1], [71, 32]:                # from a page's start it does
+        book.resize(want)
+        cache.resize(want)
+        _agree(cache, book, pools)
+    assert book.status == 0
 
 
 @gpu
