@@ -387,7 +387,7 @@ def test_starts_out_of_order(starts):
 
 @gpu
 @pytest.mark.parametrize("sequences", [255, 256, 300, 1300])
-def test_many_sequences(sequences):
+def test_plans_of_many_sequences(sequences):
     # the plan in every wave, and in a launch of its own (more than one round of its block)
     from harsh4b_amd.paged import paged_attention
     rng = np.random.default_rng(sequences)
