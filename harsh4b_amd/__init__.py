@@ -3,4 +3,4 @@
 libhq.so (HIP kernels + C ABI, include/hq.h) does all arithmetic; the Python
 side mirrors the reference's cpu_lightspark.py call surface.
 """
-__all__ = ["lightspark", "synthetic", "config", "build"]
+__all__ = ["lightspark", "synthetic", "config", "build", "paged"]

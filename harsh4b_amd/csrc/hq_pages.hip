@@ -6,7 +6,7 @@
 // border without the host.  A page is free while no table entry holds it
 // (refs = 0) and allocation takes the lowest free pages, so every call's
 // outcome is a function of the tables alone, whatever order its atomics run
-// in.  Each call is two launches:
+// in.  Each call is two launches (a fork of a small table one):
 //   plan    one block (resize, compact): counts, prefix sums, the list of free
 //           pages; decides whether the call can be done at all
 //   apply   many blocks: table rows, reference counts and the page copies
@@ -104,7 +104,8 @@ __device__ __forceinline__ void free_pages(const PagesParams& p, uint32_t at, ui
 }
 
 // Bound by latency: three dependent reads (lengths, table, refs), the first
-// 16384 pages' refs beside them, and the block's barriers.
+// 16384 pages' refs beside them, and the block's barriers.  32 rows: 4.0 us
+// where nothing is copied, 7.0 with 21 copies.
 __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PagesParams p)
 {
     __shared__ int wave_sum[kPlanWaves];
@@ -243,6 +244,8 @@ __device__ __forceinline__ void copy_segment(const hq_pages& c, int src, int dst
     for (; i < n; i += kWave) to[i] = from[i];
 }
 
+// 32 rows without a copy 3.8 us; with 21 copies in 36 layers (24 MB each way, of
+// pages that the last-level cache holds) 7.1.
 __global__ __launch_bounds__(kBlock) void resize_apply_kernel(PagesParams p)
 {
     if (p.head[0] == 0) return;
@@ -294,7 +297,7 @@ __device__ __forceinline__ bool parents_ok(const PagesParams& p)
 }
 
 // Tables of up to kForkEntries entries: one block, which holds all that the
-// rows take over before it writes any.
+// rows take over before it writes any (32 rows: 3.7 us).
 constexpr int kForkPer = 16, kForkEntries = kForkPer * kPlanThreads;
 
 __global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(PagesParams p)
@@ -433,7 +436,8 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagesParams 
     }
 }
 
-// Bound by HBM: 154 pages of 36 layers of 64 KB in 86 us, 4.9 TB/s.
+// Bound by HBM: 89 pages of 16 positions in 36 layers, 420 MB read and written
+// in 84 us, 5.0 TB/s.
 __global__ __launch_bounds__(kBlock) void compact_apply_kernel(PagesParams p)
 {
     const hq_pages& c = p.c;
