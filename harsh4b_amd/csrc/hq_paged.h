@@ -28,21 +28,27 @@ struct PagedBatch {
     int heads, kv_heads, groups;
 };
 
-// How many of the rising values at[1 .. n] are at most t (wave-uniform; every
-// lane calls it; at[0] must exist).  Each round of loads leaves a 64th of
-// them.  Of values that do not rise: some number from 0 to n.
-__device__ __forceinline__ int wave_count_upto(const int32_t* at, int n, int t)
+// How many of the rising values at[1 .. n] are at most t: i (wave-uniform;
+// every lane calls it; at[0] must exist), and at[i] and (for i < n) at[i + 1].
+// Each round of loads leaves a 64th of them.  Of values that do not rise: some
+// i from 0 to n.
+__device__ __forceinline__ int wave_count_upto(const int32_t* at, int n, int t, int* here, int* next)
 {
     const int lane = threadIdx.x & (kWave - 1);
+    const int end = n;
     int low = 0;
-    while (n > kWave) {
+    while (n > kWave - 2) {
         const int stride = (n - 1) / kWave + 1;
         const int i = (lane + 1) * stride;
         const int past = __popcll(__ballot(i <= n && at[i <= n ? low + i : low] <= t));
         low += past * stride;
         n = min(stride - 1, n - past * stride);
     }
-    return low + __popcll(__ballot(lane < n && at[lane < n ? low + 1 + lane : low] <= t));
+    const int v = at[min(low + lane, end)];
+    const int past = __popcll(__ballot(lane >= 1 && lane <= n && v <= t));
+    *here = __builtin_amdgcn_readlane(v, past);
+    *next = __builtin_amdgcn_readlane(v, past + 1);
+    return low + past;
 }
 
 // The sequence of a batch row (wave-uniform; every lane calls it), or -1; its first row and its rows.
@@ -53,12 +59,11 @@ __device__ __forceinline__ int paged_sequence(const PagedBatch& p, int t, int* f
         *count = 1;
         return t < p.sequences ? t : -1;
     }
-    const int b = wave_count_upto(p.starts, p.sequences, t);
-    if (b >= p.sequences) return -1;
-    const int a = p.starts[b], z = p.starts[b + 1];
+    int a, z;
+    const int b = wave_count_upto(p.starts, p.sequences, t, &a, &z);
     *first = a;
     *count = z - a;
-    return a < 0 || a > t || z <= t || z > p.tokens ? -1 : b;
+    return b >= p.sequences || a < 0 || a > t || z <= t || z > p.tokens ? -1 : b;
 }
 
 // The position of sequence b's i-th new row of `count`; negative: before the sequence.

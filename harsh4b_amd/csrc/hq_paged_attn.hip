@@ -72,6 +72,11 @@ constexpr int kLargeMin = 4;           // of a large one (100 tokens at 1024: 26
 // A chunk of a large tile counts as two of a small one: a step of 24 chats and
 // a prompt's 250 tokens takes 60.2 us so, 72.6 with 1, 74.1 with 3.
 constexpr int kLargeCost = 2;
+// Where there is a tile for every CU, large ones of so few chunks stay whole:
+// a second block on the CU gains less than the join of the parts costs (4 x
+// 256 tokens at 512: 36 us, 44 in two pieces each; at 1024 53, 60; at 2048,
+// 32 chunks, 88, 92; 1000 tokens at 1000 50, 51; at 2000 85, 79).
+constexpr int kLargeWhole = 16;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBlocks = 4096;
 // Tables of up to 8 chunks (512 positions): no tile is cut, and there is no
@@ -250,10 +255,12 @@ __device__ __forceinline__ int wave_prefix(int v)
     return v;
 }
 
-// Pieces a sequence's tiles are cut in for pieces of about `target` chunks.
-__device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequencePlan& s, int target)
+// Pieces a sequence's tiles are cut in for pieces of about `target` chunks;
+// tiles: of the whole batch (of one kv head).
+__device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequencePlan& s, int target, int tiles)
 {
     if (p.whole) return 1;
+    if (!s.small && s.chunks <= kLargeWhole && int64_t(tiles) * p.b.kv_heads >= kTarget / 2) return 1;
     const int size = max(target, s.small ? kSmallMin : kLargeMin * kLargeCost);
     return max(1, int(float(s.chunks * s.cost()) / float(size) + 0.5f));
 }
@@ -299,29 +306,32 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedAttnParam
 {
     constexpr int WAVES = kPlanThreads / kWave;
     __shared__ unsigned long long all_units;
-    __shared__ int falls;
+    __shared__ int falls, all_tiles;
     __shared__ int3 wave_sum[WAVES];
     const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
-    if (t == 0) all_units = 0, falls = 0;
+    if (t == 0) all_units = 0, falls = all_tiles = 0;
     __syncthreads();
     bool fall = false;
     int64_t units = 0;
+    int sum = 0;
     SequencePlan mine{};
     for (int b = t; b < p.b.sequences; b += kPlanThreads) {
         mine = sequence_plan(p, b, &fall);
         units += int64_t(mine.tiles) * mine.chunks * mine.cost();
+        sum += mine.tiles;
     }
+    if (sum) atomicAdd(&all_tiles, sum);
     if (units) atomicAdd(&all_units, static_cast<unsigned long long>(units));
     if (fall) falls = 1;
     __syncthreads();
     int count = 0, pieces = 0, rows = 0;
     if (!falls) {
-        const int target = piece_target(p, int64_t(all_units));
+        const int target = piece_target(p, int64_t(all_units)), tiles = all_tiles;
         for (int base = 0; base < p.b.sequences; base += kPlanThreads) {
             const int b = base + t;
             if (p.b.sequences > kPlanThreads && b < p.b.sequences) mine = sequence_plan(p, b, &fall);
             if (b >= p.b.sequences) mine.tiles = 0;
-            const int cuts = cuts_of(p, mine, target);
+            const int cuts = cuts_of(p, mine, target, tiles);
             const int here = mine.tiles * cuts * p.b.kv_heads;
             const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
             const uint64_t has = __ballot(here > 0);
@@ -370,19 +380,22 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     bool fall = false;
     if (p.planned) {
         const int count = *p.plan_count;
-        const int i = wave_count_upto(p.plan_first, count, q);
+        int first, next;
+        const int i = wave_count_upto(p.plan_first, count, q, &first, &next);
         if (i >= count) return false;
         const int4 item = p.plan_item[i];
         const int b = uniform(item.x);
-        place_piece(p, sequence_plan(p, b, &fall), b, q - uniform(p.plan_first[i]), uniform(item.y), uniform(item.z), out);
+        place_piece(p, sequence_plan(p, b, &fall), b, q - first, uniform(item.y), uniform(item.z), out);
         return true;
     }
     int64_t units = 0;
+    int tiles = 0;
     SequencePlan mine{};
     for (int base = 0; base < p.b.sequences; base += kWave) {
         if (base + lane < p.b.sequences) {
             mine = sequence_plan(p, base + lane, &fall);
             units += int64_t(mine.tiles) * mine.chunks * mine.cost();
+            tiles += mine.tiles;
         }
     }
     if (__any(fall)) {
@@ -393,6 +406,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     const int low = __builtin_amdgcn_readfirstlane(wave_isum64(int(units & 0xFFFFFF)));
     const int high = __builtin_amdgcn_readfirstlane(wave_isum64(int(min(units >> 24, int64_t(0xFFFFFF)))));
     int target = piece_target(p, (int64_t(high) << 24) + low);
+    tiles = uniform(wave_isum64(tiles));
     // Rounded, they may be a few more pieces than places, and those run alone
     // at the end: larger ones that all have a place, if up to twice the size
     // gives such (800 tokens after 8200: 228 us, 264 without; 400 after 4600
@@ -400,7 +414,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     if (p.b.sequences <= kWave && !p.whole) {
         int larger = target;
         for (int k = 0; k < 7; ++k) {
-            if (uniform(wave_isum64(mine.tiles * cuts_of(p, mine, larger))) * p.b.kv_heads <= kTarget) {
+            if (uniform(wave_isum64(mine.tiles * cuts_of(p, mine, larger, tiles))) * p.b.kv_heads <= kTarget) {
                 target = larger;
                 break;
             }
@@ -413,7 +427,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         const bool in = base + lane < p.b.sequences;
         if (p.b.sequences > kWave && in) mine = sequence_plan(p, base + lane, &fall);
         if (!in) mine.tiles = 0;
-        const int cuts = cuts_of(p, mine, target);
+        const int cuts = cuts_of(p, mine, target, tiles);
         const int here = mine.tiles * cuts * p.b.kv_heads;
         const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
         const int incl = wave_prefix(here), part_incl = wave_prefix(part);
