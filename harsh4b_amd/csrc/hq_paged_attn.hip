@@ -454,17 +454,6 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
 }
 
 // ------------------------------------------------------------- query operands
-// Eight values of a row as fp16 parts hi + lo of 2^-e times them.
-__device__ __forceinline__ void split8(const float (&x)[8], int e, half8& hi, half8& lo)
-{
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = __builtin_ldexpf(x[i], -e);
-        hi[i] = _Float16(y);
-        lo[i] = _Float16(y - float(hi[i]));
-    }
-}
-
 // The exponent that takes values of at most `top` to below 2^10 (0 for a row of zeros or without a finite maximum).
 __device__ __forceinline__ int row_exponent(float top)
 {
@@ -489,8 +478,8 @@ __device__ __forceinline__ float2v residual(float a, float b, half2v h)
     return r;
 }
 
-// Weights p (of up to 2^14) as hi + lo.
-__device__ __forceinline__ void split_weights(const float (&w)[8], half8& hi, half8& lo)
+// Eight values within fp16's range as hi + lo.
+__device__ __forceinline__ void split8(const float (&w)[8], half8& hi, half8& lo)
 {
     uint4v a, b;
 #pragma unroll
@@ -653,7 +642,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     half8 qhi[STEPS], qlo[STEPS];
     float c;
     {
-        const bool used = mine && (D >= 32 || g < 2);
+        const bool used = D >= 32 || g < 2;   // (a lane of no row: the tile's first row, not stored)
         float top = 0.0f;
         float y[STEPS][8];
 #pragma unroll
@@ -665,8 +654,13 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
             }
         top = max_over_g(top);
         const int e = row_exponent(top);
+        const float down = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) split8(y[s], e, qhi[s], qlo[s]);
+        for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[s][i] *= down;
+            split8(y[s], qhi[s], qlo[s]);
+        }
         c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
     }
     for (int k = 0; k < own; ++k) {
@@ -732,7 +726,7 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 l += e[4 * t + i];
             }
         half8 hi, lo;
-        split_weights(e, hi, lo);
+        split8(e, hi, lo);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             // dims VEC n + i: half (i & 1) of word i / 2 of each key
@@ -870,16 +864,21 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             const float4v a = *reinterpret_cast<const float4v*>(q + 16 * s + 8 * g);
             const float4v b = *reinterpret_cast<const float4v*>(q + 16 * s + 8 * g + 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[s][i] = mine ? a[i] : 0.0f;
-                x[s][4 + i] = mine ? b[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) {      // (a lane of no row: the tile's first row, not stored)
+                x[s][i] = a[i];
+                x[s][4 + i] = b[i];
                 top = fmaxf(top, fmaxf(__builtin_fabsf(x[s][i]), __builtin_fabsf(x[s][4 + i])));
             }
         }
         top = fmaxf(top, __shfl_xor(top, 32, kWave));
         const int e = row_exponent(top);
+        const float down = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) split8(x[s], e, qhi[s], qlo[s]);
+        for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[s][i] *= down;
+            split8(x[s], qhi[s], qlo[s]);
+        }
         c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
     }
     const bool active = 32 * wave < rows;      // (wave-uniform)
@@ -1154,15 +1153,17 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const bool mine_end = r_end < rows;
     const int token_end = mine_end ? row_token(p, r_end) : 0;
     const size_t row_end = size_t(w.first + token_end) * p.b.heads + w.head * G + (mine_end ? r_end - token_end * G : 0);
-    bool ok = finite(l) && l != 0.0f;
+    float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN where an output is not finite
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            if (32 * dt + 8 * (i >> 2) < D) ok &= finite(acc[dt][i]);
+            if (32 * dt + 8 * (i >> 2) < D) zero[i & 3] = __builtin_fmaf(acc[dt][i], 0.0f, zero[i & 3]);
     const uint64_t was_seen = __ballot(seen);
     const bool none = (((was_seen | (was_seen >> 32)) >> n_end) & 1) == 0;
-    const uint64_t wrong = __ballot(mine_end && !none && !ok);
+    // (a row that sees nothing has zeros, unless its tile holds something not finite)
+    const bool ok = (zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f && (none || (finite(l) && l != 0.0f));
+    const uint64_t wrong = __ballot(mine_end && !ok);
     const uint32_t again = uint32_t(wrong | (wrong >> 32));
     if (mine_end && ((again >> n_end) & 1) == 0) {
         const bool direct = w.pieces == 1;
@@ -1176,7 +1177,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 if (dim < D) {
                     float4v x;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] = none ? 0.0f : acc[dt][4 * i + k] * f;
+                    for (int k = 0; k < 4; ++k) x[k] = acc[dt][4 * i + k] * f;
                     *reinterpret_cast<float4v*>(to + dim) = x;
                 }
             }
