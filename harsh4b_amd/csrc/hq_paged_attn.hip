@@ -112,6 +112,16 @@ struct PagedAttnParams {
 // The token of a tile's row: r / groups (exact: r < 128, groups <= 8).
 __device__ __forceinline__ int row_token(const PagedAttnParams& p, int r) { return (r * p.by_group) >> 16; }
 
+// a / b for 0 <= a < 2^24 and 0 < b < 2^24 (exact: the quotient by the
+// reciprocal is off by one at most; a third of a division's instructions, and
+// the plan makes five one after another).
+__device__ __forceinline__ int quotient(int a, int b)
+{
+    const int q = int(float(a) * __builtin_amdgcn_rcpf(float(b)));
+    const int rest = a - q * b;
+    return q + (rest >= b ? 1 : 0) - (rest < 0 ? 1 : 0);
+}
+
 // Whether the query at position `pos` sees position j (pages aside).
 __device__ __forceinline__ bool paged_visible(int pos, int j, int window, int sinks)
 {
@@ -222,7 +232,7 @@ __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, 
         s.n = a < 0 || a >= z || z > p.b.tokens ? 0 : z - a;
         s.small = s.n <= kSmallRows / p.b.groups;
         s.tile_tokens = s.small ? max(1, s.n) : p.tile_tokens;
-        s.tiles = int(unsigned(s.n + s.tile_tokens - 1) / unsigned(s.tile_tokens));
+        s.tiles = s.small ? min(s.n, 1) : quotient(s.n + s.tile_tokens - 1, s.tile_tokens);
     }
     const int origin = s.length - s.n;
     s.chunks = s.n ? span_of(p, origin + (s.tiles - 1) * s.tile_tokens, s.length - 1).count : 0;
@@ -275,14 +285,19 @@ __device__ __forceinline__ void place_piece(const PagedAttnParams& p, const Sequ
     out.length = s.length;
     int rest, tile;
     if (out.small) {                                         // (one tile)
-        rest = unsigned(local) / unsigned(p.b.kv_heads);
+        rest = quotient(local, p.b.kv_heads);
         out.split = rest;
         tile = 0;
     } else {
-        rest = unsigned(local) / unsigned(p.b.kv_heads);
-        const int done = unsigned(rest) / unsigned(out.pieces);
+        // The longest first; and since blocks i and i + 256 share a CU, where
+        // all have a place the second 256 the other way round (a prompt of
+        // 1800 tokens: 87 us, 90 without; of 2048: 101, 105).
+        const int all = s.tiles * cuts * p.b.kv_heads;
+        if (all <= kTarget && local >= kTarget / 2) local = kTarget / 2 + all - 1 - local;
+        rest = quotient(local, p.b.kv_heads);
+        const int done = quotient(rest, out.pieces);
         out.split = rest - done * out.pieces;
-        tile = s.tiles - 1 - done;                           // the longest first
+        tile = s.tiles - 1 - done;
     }
     tile = uniform(tile);
     out.split = uniform(out.split);
@@ -366,7 +381,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
 {
     const int lane = threadIdx.x & (kWave - 1);
     if (p.whole && !p.b.starts) {              // a tile a block: nothing to count
-        out.b = uniform(unsigned(q) / unsigned(p.b.kv_heads));
+        out.b = uniform(quotient(q, p.b.kv_heads));
         out.head = q - out.b * p.b.kv_heads;
         out.first = out.b;
         out.n = 1;
@@ -411,7 +426,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     // at the end: larger ones that all have a place, if up to twice the size
     // gives such (800 tokens after 8200: 228 us, 264 without; 400 after 4600
     // 86, 105; 700 after 800 58, 64).
-    if (p.b.sequences <= kWave && !p.whole) {
+    if (p.b.sequences <= kWave && !p.whole && int64_t(tiles) * p.b.kv_heads <= kTarget) {
         int larger = target;
         for (int k = 0; k < 7; ++k) {
             if (uniform(wave_isum64(mine.tiles * cuts_of(p, mine, larger, tiles))) * p.b.kv_heads <= kTarget) {
