@@ -314,6 +314,14 @@ def test_longer(count, length):
 
 
 @gpu
+@pytest.mark.parametrize("counts,lengths", [([600], [600]), ([300], [1500]), ([352], [1500]), ([1, 900, 1], [700, 1300, 90]),
+                                            ([1100], [1100]), ([64, 256, 1, 256], [400, 1000, 800, 256])])
+def test_many_tiles(counts, lengths):
+    # 16 tokens a tile and 8 kv heads: 152 to 552 tiles, whole and cut, more and fewer than there are places
+    Scene(counts, lengths, 8, 8, 16, 64, seed=len(counts) + counts[-1])._check()
+
+
+@gpu
 @pytest.mark.parametrize("count", [1, 2, 40])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
 def test_border_positions_count(count, window, sinks):
