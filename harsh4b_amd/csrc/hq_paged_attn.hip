@@ -1241,6 +1241,28 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnPar
     else if constexpr (LARGE) large_tile<D>(p, w, span, c0, c1, S.large);
 }
 
+// The join's threads are sets of groups * D / 4, one thread for four values of
+// the output; what 256 leaves over is no whole set.  Set 0 stores.
+__host__ __device__ constexpr int join_set(int thread, int quads) { return thread / quads; }
+__host__ __device__ constexpr int join_quad(int thread, int quads) { return thread % quads; }
+__host__ __device__ constexpr bool join_stores(int thread, int quads) { return join_set(thread, quads) == 0; }
+
+// Whether every four values have one thread that stores them, for each head size and group.
+constexpr bool join_has_one_writer()
+{
+    for (int D = 16; D <= 128; D *= 2)
+        for (int groups = 1; groups <= 8; ++groups) {
+            int writers[kJoinThreads] = {};
+            const int quads = groups * D / 4;
+            for (int t = 0; t < kJoinThreads; ++t)
+                if (join_stores(t, quads)) ++writers[join_quad(t, quads)];
+            for (int q = 0; q < quads; ++q)
+                if (writers[q] != 1) return false;
+        }
+    return true;
+}
+static_assert(join_has_one_writer());
+
 // Join the parts of one token's heads of one kv head: thread (set of parts,
 // four values), the parts' loads four at a time ahead of their use.  Bound by
 // latency where the parts are few (32 chats: 4.9 us) and by the L2 and HBM
@@ -1254,7 +1276,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
     const int cut = *p.cut;                               // (waited for beside the first row's loads)
     const int quads = p.b.groups * D / 4;                 // at most 256
     const int sets = kJoinThreads / quads;
-    const int set = threadIdx.x / quads, quad = threadIdx.x % quads;
+    const int set = join_set(threadIdx.x, quads), quad = join_quad(threadIdx.x, quads);
     const int r = quad / (D / 4), at = quad % (D / 4);
     const unsigned all = unsigned(p.b.tokens) * unsigned(p.b.kv_heads);
     for (unsigned i = blockIdx.x; i < all; i += gridDim.x) {
@@ -1302,7 +1324,10 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
             sl[threadIdx.x] = m == -__builtin_inff() ? lost : l;
             so[threadIdx.x] = o;
             __syncthreads();
-            if (set != 0) continue;
+        }
+        // (of one set and threads left over too: groups of 5 to 7 heads of 128)
+        if (!join_stores(threadIdx.x, quads)) continue;
+        if (sets > 1) {
             for (int k = 1; k < sets; ++k) add(sm[k * quads + quad], sl[k * quads + quad], so[k * quads + quad]);
         }
         const float f = 1.0f / l;

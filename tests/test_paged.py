@@ -321,6 +321,53 @@ def test_many_tiles(counts, lengths):
     Scene(counts, lengths, 8, 8, 16, 64, seed=len(counts) + counts[-1])._check()
 
 
+def _reference_of_heads(s, window=0, sinks=0):
+    """_reference, a sequence's head at a time, where everything visible is finite."""
+    kv, d, heads = s.keys.shape[1], s.keys.shape[3], s.query.shape[1]
+    out, bound = np.zeros(s.query.shape), np.zeros(s.tokens)
+    for b, (n, length) in enumerate(zip(s.counts, s.lengths)):
+        if n == 0:
+            continue
+        j, p = np.arange(length), np.arange(length - n, length)[:, None]
+        seen = j <= p
+        if window:
+            seen &= (j > p - window) | (j < sinks)
+        keys, values = (pool[s.place(b, j)[0], :, j % pool.shape[2]].astype(np.float64) for pool in (s.keys, s.values))
+        rows = slice(s.starts[b], s.starts[b + 1])
+        for h in range(heads):
+            k, v, q = keys[:, h // (heads // kv)], values[:, h // (heads // kv)], s.query[rows, h].astype(np.float64)
+            score = np.where(seen, q @ k.T / math.sqrt(d), -np.inf)
+            e = np.exp(score - score.max(axis=1, keepdims=True))
+            out[rows, h] = e @ v / e.sum(axis=1, keepdims=True)
+            size = np.where(seen, np.abs(q) @ np.abs(k).T, 0.0).max(axis=1) / math.sqrt(d)
+            bound[rows] = np.maximum(bound[rows], np.abs(v).max() * (2 * (d + 8) * 2.0 ** -24 * size +
+                                                                     (seen.sum(axis=1) + 64) * 2.0 ** -24))
+    return out, bound
+
+
+def _check_heads(s, window=0, sinks=0):
+    got = s.attend(window, sinks)
+    expect, bound = _reference_of_heads(s, window, sinks)
+    off = np.abs(got - expect).reshape(s.tokens, -1).max(axis=1)
+    assert (off <= bound).all(), (np.argmax(off - bound), off.max(), bound[np.argmax(off - bound)])
+
+
+@gpu
+@pytest.mark.parametrize("kv,groups", [(2, 5), (1, 6), (2, 7)])
+def test_joins_with_threads_left_over(kv, groups):
+    # 5 to 7 heads of 128: one set of the join's threads and some of a second, which have nothing to store
+    for starts in False, True:
+        Scene([1] * 6, [1, 15, 16, 17, 64, 301], kv, groups, 128, 16, seed=groups).check(starts=starts)
+    Scene([5, 0, 1, 37, 130, 0, 2, 64], [5, 40, 77, 100, 130, 0, 300, 65], kv, groups, 128, 32, seed=groups).check()
+    Scene([129, 1], [1111, 900], kv, groups, 128, 64, seed=groups).check()
+
+
+@gpu
+def test_more_rows_than_the_join_has_blocks():
+    # every tile in two pieces, 4200 tokens of a kv head to join
+    _check_heads(Scene([2100], [2100], 2, 7, 128, 64, seed=71))
+
+
 @gpu
 @pytest.mark.parametrize("count", [1, 2, 40])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
