@@ -31,6 +31,7 @@ import torch
 from . import _native
 from ._native import check
 
+MAX_SEQUENCES = 0xFFFFFF
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (16, 32, 64, 128)
 MAX_GROUPS = 8
@@ -93,8 +94,10 @@ def _cache(index: int, keys, values, table, lengths, refs, status, dims: int, po
     if len(shape) != 2 or table.dtype is not _I32 or table.get_device() != index or not table.is_contiguous():
         _refuse("table", table, _I32, index, "[sequences, max_pages]")
     sequences, max_pages = shape
-    if sequences == 0 or max_pages == 0 or max_pages * page_size > 0x7FFFFF00 or sequences * max_pages > 0x7FFFFFFF:
-        raise ValueError("table must be [sequences, max_pages] with fewer than 2^31 entries and 2^31 - 256 positions a row")
+    if (sequences == 0 or max_pages == 0 or max_pages * page_size > 0x7FFFFF00 or sequences * max_pages > 0x7FFFFFFF or
+            sequences > MAX_SEQUENCES):
+        raise ValueError("table must be [sequences, max_pages] with fewer than 2^24 sequences, fewer than 2^31 entries "
+                         "and 2^31 - 256 positions a row")
     length_ptr = ref_ptr = status_ptr = 0
     if lengths is not None:
         if (lengths.shape != (sequences,) or lengths.dtype is not _I32 or lengths.get_device() != index or
@@ -130,12 +133,14 @@ def _starts(starts, sequences: int, tokens: int, index: int) -> int | None:
     return starts.data_ptr()
 
 
-def _launch(entry, args: tuple, nbytes: int, index: int, stream, tensors, what: str) -> None:
+def _launch(entry, args: tuple, nbytes: int | None, index: int, stream, tensors, what: str) -> None:
     """entry(*args[, workspace], stream handle) on `stream` (None: the current
-    one of the tensors' GPU) with a workspace of this call alone: memory of any
-    contents from torch's allocator, which hands it out in the stream's order
-    and inside a capture from the graph's own pool (straight from it: a
-    tensor's making takes 0.9 us more)."""
+    one of the tensors' GPU) with a workspace of this call alone (nbytes None:
+    an entry without one): memory of any contents from torch's allocator, which
+    hands it out in the stream's order and inside a capture from the graph's
+    own pool (straight from it: a tensor's making takes 0.9 us more)."""
+    if nbytes == 0:                            # (what the size functions return for sizes that the entries refuse)
+        raise ValueError(f"{what}: sizes outside the entry's range")
     if index != _current_device():
         with torch.cuda.device(index):
             return _launch(entry, args, nbytes, index, stream, tensors, what)
@@ -151,14 +156,14 @@ def _launch(entry, args: tuple, nbytes: int, index: int, stream, tensors, what: 
             if t is not None:
                 t.record_stream(stream)
         handle = stream.cuda_stream
-    if nbytes:
+    if nbytes is None:
+        status = entry(*args, handle)
+    else:
         workspace = _alloc(nbytes, handle)
         try:
             status = entry(*args, workspace, handle)
         finally:
             _free(workspace)                   # (to the stream's pool: what follows on it may have it)
-    else:
-        status = entry(*args, handle)
     if status:
         check(status, what)
 
@@ -209,7 +214,7 @@ def paged_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     if tokens:
         _launch(_native.lib().hq_paged_append,
                 (cache, qkv.data_ptr(), first, tokens, heads, q_norm.data_ptr(), k_norm.data_ptr(), eps,
-                 rope_cos.data_ptr(), rope_sin.data_ptr(), positions, out.data_ptr()), 0, index, stream,
+                 rope_cos.data_ptr(), rope_sin.data_ptr(), positions, out.data_ptr()), None, index, stream,
                 (qkv, q_norm, k_norm, rope_cos, rope_sin, keys, values, table, lengths, status, starts, out),
                 "hq_paged_append")
     return out

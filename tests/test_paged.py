@@ -116,6 +116,31 @@ def test_python_refuses_host_tensors_and_bad_caches():
         paged.PagedCache(1, 0, 2, 32, 2, 3, device="cpu")
 
 
+def test_sizes_that_the_entries_refuse():
+    # the size functions return 0 for them: an error, and no call without the workspace
+    from harsh4b_amd import paged
+    with pytest.raises(ValueError, match="2\\^24 sequences"):
+        paged._cache(-1, None, None, torch.empty((2**24, 1), dtype=torch.int32), None, None, None, 5, pools=False)
+    paged._cache(-1, None, None, torch.empty((2**24 - 1, 1), dtype=torch.int32), None, None, None, 5, pools=False)
+    calls = []
+    with pytest.raises(ValueError, match="hq_some_entry: sizes"):
+        paged._launch(lambda *args: calls.append(args) or 0, (1, 2), 0, 0, None, (), "hq_some_entry")
+    assert calls == []
+
+
+@gpu
+def test_tables_of_too_many_sequences():
+    from harsh4b_amd import paged
+    ints = dict(dtype=torch.int32, device="cuda")
+    table, each, refs = torch.full((2**24, 1), -1, **ints), torch.zeros(2**24, **ints), torch.zeros(4, **ints)
+    status, pool = torch.zeros(1, **ints), torch.zeros((1, 4, 1, 16, 16), dtype=torch.float16, device="cuda")
+    for call in (lambda: paged.pages_fork(table, each, refs, status, each),
+                 lambda: paged.pages_resize(pool, pool.clone(), table, each, refs, status, each),
+                 lambda: paged.pages_compact(pool, pool.clone(), table, refs)):
+        with pytest.raises(ValueError, match="fewer than 2\\^24 sequences"):
+            call()
+
+
 @gpu
 def test_python_refuses_bad_device_arguments():
     from harsh4b_amd import paged
