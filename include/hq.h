@@ -192,8 +192,9 @@ int hq_quant_int4_gemm(const float* x, const uint8_t* weights, const float* scal
  * tokens.  Calls on one cache run one after another (one stream, or streams
  * that wait for each other).
  * Entries, lengths, starts and parents outside their ranges are never
- * followed: an entry counts as -1, and the calls that take a status report
- * HQ_PAGES_BAD. */
+ * followed: an entry counts as -1.  HQ_PAGES_BAD is set by hq_pages_resize for
+ * a length and for the entry that a growth goes on in, by hq_pages_fork for a
+ * parent, by hq_paged_append for the starts and for a row's place. */
 typedef struct hq_pages {
     int32_t layers;       /* layers of keys and values (see each call) */
     int32_t pages, page_size, kv_heads, head_dim;
@@ -208,7 +209,7 @@ typedef struct hq_pages {
 } hq_pages;
 
 #define HQ_PAGES_FULL 1   /* too few free pages, or a sequence past max_pages: that call changed nothing */
-#define HQ_PAGES_BAD 2    /* an entry, length, start or parent outside its range */
+#define HQ_PAGES_BAD 2    /* an entry, length, start or parent outside its range (above) */
 #define HQ_PAGES_REFUSED 4 /* with HQ_PAGES_BAD: a resize or a fork was refused for it and changed nothing */
 
 /* Set the lengths: sequence b goes to new_lengths[b] positions (device int32
@@ -250,8 +251,10 @@ int hq_pages_compact(const hq_pages* cache, int32_t* live, void* workspace, void
  * falling; NULL: token b of sequence b, tokens = sequences) at positions
  * lengths[b] - n_b .. lengths[b] - 1.  A row at a position outside the cache
  * or the rope tables, or without a page, sets HQ_PAGES_BAD, writes no K/V
- * and a query of zeros; rows of no sequence are not touched.  qkv
- * and query must not overlap.  While status
+ * and a query of zeros; rows of no sequence are not touched.  Starts
+ * below 0, above `tokens` or falling set HQ_PAGES_BAD too: the rows of such a
+ * sequence are not touched (where starts fall, others may be left out as
+ * well).  qkv and query must not overlap.  While status
  * has HQ_PAGES_FULL or HQ_PAGES_REFUSED set no K/V is written (the lengths
  * did not grow, so the rows would land on earlier ones).  A page that several
  * entries hold is written for all of them: hq_pages_resize gives a growing
@@ -265,8 +268,9 @@ int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* star
  * positions j <= p that have a page, with window > 0 only those with
  * j > p - window or j < sinks.  query, output fp32 [tokens, heads,
  * head_dim], heads ordered [kv_head, group], groups = heads/kv_heads <= 8.
- * A row that sees nothing gets zeros; rows of no sequence are not touched.
- * query and output must not overlap.  Values at positions past a sequence's
+ * A row that sees nothing gets zeros; rows of no sequence are not touched, nor
+ * those of one whose starts lie below 0 or above `tokens`, and where starts
+ * fall none is.  query and output must not overlap.  Values at positions past a sequence's
  * length are never used, whatever they hold.  status may be NULL.
  * `workspace`: hq_paged_attention_workspace_bytes(...) bytes (single: nonzero where starts
  * is NULL), 256-byte aligned, of any contents. */

@@ -708,6 +708,76 @@ def test_append_of_rows_without_a_place():
         np.testing.assert_array_equal(dev["values"].cpu().numpy().view(np.uint16), before)
 
 
+@gpu
+@pytest.mark.parametrize("starts", [[0, 2, 5], [1, 3, 4], [0, 0, 0], [5, 5, 5], [0, 2, 1], [0, 9, 10], [-3, 2, 5], [4, 2, 5],
+                                    [0, 5, 6], [0, 0, 6], [2, 2, 1], [0, 2**31 - 1, 2**31 - 1], [-(2**31), 0, 5]])
+def test_append_reports_starts_outside_the_batch(starts):
+    # a range that is none loses its sequence's rows: reported, and nothing else is written in their place
+    from harsh4b_amd.paged import paged_append
+    s = Scene([2, 3], [40, 20], page=16, seed=6)
+    inputs, dev = _append_inputs(s, 2, 4, 128), s.device()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full((5, 8, 128), 7.0, device="cuda")
+    paged_append(*[torch.from_numpy(a).cuda() for a in inputs], 1e-6, dev["keys"], dev["values"], dev["table"],
+                 dev["lengths"], status, starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), out=out)
+    good = [0 <= a <= z <= 5 for a, z in zip(starts, starts[1:])]
+    assert int(status.item()) == (0 if all(good) else native().HQ_PAGES_BAD)
+    rows, host = set(), out.cpu().numpy()
+    values, written = s.values.copy(), dev["values"].cpu().numpy()
+    for b, (a, z) in enumerate(zip(starts, starts[1:])):
+        if good[b] and sorted(starts) == starts:
+            rows |= set(range(a, z))
+            for t in range(a, z):
+                values[s.place(b, s.lengths[b] - (z - a) + t - a)] = inputs[0][t, 10 * 128:].reshape(2, 128)
+    if sorted(starts) == starts:
+        np.testing.assert_array_equal(written.view(np.uint16), values.view(np.uint16))
+        assert all((host[t] != 7.0).any() == (t in rows) for t in range(5))
+
+
+@gpu
+def test_append_looks_at_all_starts():
+    # more sequences than the launch has threads, the bad one among the last
+    from harsh4b_amd.paged import paged_append
+    n, d = 2000, 16
+    ints = dict(dtype=torch.int32, device="cuda")
+    starts = torch.ones(n + 1, **ints)
+    starts[0] = 0
+    pool, rope, norm = (torch.zeros((4, 1, 16, d), dtype=torch.float16, device="cuda"), torch.ones((16, d // 2), device="cuda"),
+                        torch.ones(d, device="cuda"))
+    table, lengths = torch.zeros((n, 1), **ints), torch.ones(n, **ints)
+    for bad in None, n - 1, n, 1500, 1:
+        status, at = torch.zeros(1, **ints), starts.clone()
+        if bad is not None:
+            at[bad:] = 2 if bad != 1500 else -1
+        paged_append(torch.ones((1, 3 * d), device="cuda"), norm, norm, rope, rope, 1e-6, pool, pool.clone(), table, lengths,
+                     status, starts=at)
+        assert int(status.item()) == (0 if bad is None else native().HQ_PAGES_BAD), bad
+
+
+@gpu
+def test_append_of_the_most_tokens():
+    # as many as a launch has blocks: those that look at the starts have a launch of their own
+    from harsh4b_amd.paged import paged_append
+    tokens, d = 2**24 - 1, 16
+    pages = 2**24 // 256
+    ints = dict(dtype=torch.int32, device="cuda")
+    keys = torch.zeros((pages, 1, 256, d), dtype=torch.float16, device="cuda")
+    values, rope, norm = torch.zeros_like(keys), torch.ones((tokens, d // 2), device="cuda"), torch.ones(d, device="cuda")
+    qkv = torch.zeros((tokens, 3 * d), device="cuda")
+    qkv[:, 2 * d:] = (torch.arange(tokens, device="cuda") % 2039)[:, None]
+    table, lengths = torch.arange(pages, **ints)[None], torch.full((1,), tokens, **ints)
+    for end in tokens, 2**24:
+        status = torch.zeros(1, **ints)
+        values.zero_()
+        paged_append(qkv, norm, norm, rope, rope, 1e-6, keys, values, table, lengths, status,
+                     starts=torch.tensor([0, end], **ints))
+        good = end == tokens
+        assert int(status.item()) == (0 if good else native().HQ_PAGES_BAD)
+        expect = torch.arange(2**24, device="cuda").remainder_(2039).mul_(good).half()
+        expect[-1] = 0.0
+        assert torch.equal(values[:, 0].reshape(-1, d), expect[:, None].expand(-1, d))
+
+
 # ------------------------------------------------------------------ page management
 class Book:
     """The tables as lists, and what the calls do to them."""
