@@ -382,7 +382,8 @@ class PagedCache:
                                sinks, out, stream)
 
     def check_status(self) -> None:
-        """Wait for the calls so far and raise where one was refused."""
+        """Wait for the calls so far, on whatever stream, and raise where one was refused."""
+        torch.cuda.synchronize(self.status.device)
         code = int(self.status.item())
         if code & _native.HQ_PAGES_FULL:
             raise ValueError("the cache's free pages, or a sequence's table entries, did not suffice")

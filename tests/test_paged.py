@@ -992,6 +992,21 @@ def test_a_window_s_sequence_cut_back_too_far_does_not_grow():
 
 
 @gpu
+def test_status_of_calls_on_another_stream():
+    from harsh4b_amd.paged import PagedCache
+    cache = PagedCache(1, 4, 1, 16, sequences=2, max_pages=8, page_size=16)
+    want = torch.tensor([200, 0], dtype=torch.int32, device="cuda")
+    busy, stream = torch.zeros((8192, 8192), dtype=torch.float16, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):                # the refused call waits behind some 100 ms of other work
+        for _ in range(100):
+            busy = busy @ busy
+    cache.resize(want, stream=stream)
+    with pytest.raises(ValueError, match="free pages"):
+        cache.check_status()
+
+
+@gpu
 def test_large_pools():
     # more pages than one round of the free-page search looks at, the free ones at its end
     cache, book, pools, _ = _cache_and_book(4, 9000, 36000, 16, layers=1, kv=1, d=16)
