@@ -466,6 +466,41 @@ def test_starts_out_of_order(starts):
 
 
 @gpu
+@pytest.mark.parametrize("starts", [[0, 2, 5], [1, 3, 4], [0, 0, 0], [5, 5, 5], [0, 2, 1], [0, 9, 10], [-3, 2, 5], [4, 2, 5],
+                                    [0, 5, 6], [0, 2**31 - 1, 2**31 - 1], [-(2**31), 0, 5]])
+@pytest.mark.parametrize("spare", [0, 300])
+def test_rows_of_starts_outside_the_batch(starts, spare):
+    # the rows of ranges in the batch have their values, the others stay; where starts fall all do (spare: sequences
+    # without rows behind, for the plan's own launch)
+    from harsh4b_amd.paged import paged_attention
+    s = Scene([2, 3] + [0] * spare, [40, 20] + [0] * spare, page=16, seed=6)
+    d = s.device()
+    out = torch.full((5, 8, 128), 7.0, device="cuda")
+    at = torch.tensor(starts + [starts[-1]] * spare, dtype=torch.int32, device="cuda")
+    paged_attention(**d, starts=at, out=out)
+    host = out.cpu().numpy()
+    for b, (a, z) in enumerate(zip(starts, starts[1:])):
+        if sorted(starts) == starts and 0 <= a < z <= 5:
+            expect, bound = _reference(s.query[a:z], s.keys, s.values, s.table[b:b + 1], [z - a], s.lengths[b:b + 1], 0, 0)
+            assert (np.abs(host[a:z] - expect).reshape(z - a, -1).max(axis=1) <= bound).all()
+            host[a:z] = 7.0
+    assert (host == 7.0).all()
+
+
+@gpu
+@pytest.mark.parametrize("kv,groups,counts,lengths,window,sinks", [
+    (8, 8, [600], [600], 0, 0),                    # 304 tiles whole, the second half of the places the other way round
+    (8, 4, [300], [1500], 0, 0),                   # 80 tiles, cut
+    (8, 4, [1, 900, 1], [700, 1300, 90], 0, 0),    # 232 tiles and single tokens, cut
+    (4, 4, [1100], [1300], 333, 5),                # a window: tiles of different chunks
+    (8, 5, [500, 3], [1800, 40], 0, 0),            # tiles that are not full: 25 tokens of 5 heads
+    (8, 8, [1100], [1100], 0, 0),                  # 552 tiles: more than places
+])
+def test_many_tiles_of_128_dims(kv, groups, counts, lengths, window, sinks):
+    _check_heads(Scene(counts, lengths, kv, groups, 128, 64, seed=groups + counts[-1]), window, sinks)
+
+
+@gpu
 @pytest.mark.parametrize("sequences", [255, 256, 300, 1300])
 def test_plans_of_many_sequences(sequences):
     # the plan in every wave, and in a launch of its own (more than one round of its block)
