@@ -26,13 +26,13 @@ struct AppendParams {
 // A token's heads (q, k, v) over the waves of gridDim.y blocks, PER at a time:
 // their loads together, then the spec's norm (64 fmaf partials, halving tree)
 // and rotation as the decode step's, so that K, V and q have its bits.  Bound
-// by HBM (2000 tokens of 48 heads, 91 MB: 17.5 us, 5.2 TB/s) or latency (32
-// single tokens: 3.4 us).
+// by HBM (2000 tokens of 48 heads, 91 MB: 17.0 us, 5.3 TB/s) or latency (32
+// single tokens: 3.2 us).
 constexpr int kAppendPer = 2;
 constexpr int kAppendWide = 1024;      // tokens from which on a block does a whole token
 
 // Starts that are no ranges of the batch's rows are reported, by the launch's
-// first blocks, `looks` of them: they cost nothing there (2000 tokens 17.8 us,
+// first blocks, `looks` of them: they cost nothing there (2000 tokens 17.9 us,
 // 18.0 without them; behind the rows' blocks 18.3, by the rows' own 18.5).
 constexpr int kLookBlocks = 64;
 
@@ -169,7 +169,7 @@ extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const in
     p.rope_positions = rope_positions;
     p.query = query;
     // few tokens: kAppendPer heads a wave; many: a block a token, whose waves look its place up once for all their
-    // heads (2000 tokens 18.2 us; with kAppendPer heads a wave 23.2)
+    // heads (2000 tokens 17.9 us; with kAppendPer heads a wave 23.1)
     const int slots = heads + 2 * cache->kv_heads;
     const int per_block = kAppendPer * (kBlock / kWave);
     p.looks = starts ? std::min((cache->sequences + kBlock - 1) / kBlock, kLookBlocks) : 0;

@@ -64,25 +64,27 @@ constexpr int kChunkKeys = 64;
 constexpr int kSmallRows = 16;
 constexpr int kTileRows = 128;
 // Pieces aimed at: one for each place on the chip (two blocks a CU), all
-// started at once.  With twice as many, 16 windows of 1024 take 26.4 us
-// (22.2), 3 chats of 40960 101 (91), a question of 501 tokens 155 (143).
+// started at once.  With twice as many, 16 windows of 1024 take 28 us (23), 3
+// chats of 40960 92 (86), a question of 501 tokens after 7000 142 (129).
 constexpr int kTarget = 512;
 constexpr int kSmallMin = 2;           // fewest chunks of a small piece: a step of 32 keys a wave
-constexpr int kLargeMin = 4;           // of a large one (100 tokens at 1024: 26.2 us, 28.6 with 2, 27.6 with 3)
+constexpr int kLargeMin = 4;           // of a large one (100 tokens after 1024: 22.7 us, 23.6 with 2, 22.6 with 3)
 // A chunk of a large tile counts as two of a small one: a step of 24 chats and
-// a prompt's 250 tokens takes 60.2 us so, 72.6 with 1, 74.1 with 3.
+// a prompt's 250 tokens takes 75 us so, 82 with 1, 79 with 3 (over data that
+// the last-level cache does not hold; where it does 67, 75, 72).
 constexpr int kLargeCost = 2;
 // Where there is a tile for every CU, large ones of so few chunks stay whole:
 // a second block on the CU gains less than the join of the parts costs (4 x
-// 256 tokens at 512: 36 us, 44 in two pieces each; at 1024 53, 60; at 2048,
-// 32 chunks, 88, 92; 1000 tokens at 1000 50, 51; at 2000 85, 79).
+// 256 tokens at 512: 34 us, 43 in two pieces each; at 1024 51, 59; 1000 tokens
+// at 1000 48, 50).  At 32 chunks it goes both ways: 4 x 256 at 2048 83 whole,
+// 87 cut; 1000 at 2000 80, 75.
 constexpr int kLargeWhole = 16;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBlocks = 4096;
 // Tables of up to 8 chunks (512 positions): no tile is cut, and there is no
-// join to launch.  One chat of 256: 9.3 us (10.7 with both), of 512 11.5
-// (10.8, and the caller's time for a second launch, 3), of 768 13.8 (10.8);
-// 64 chats of 512 23.1 (24.7).
+// join to launch.  One chat of 256: 7.9 us (11.4 with both), of 480 10.5
+// (11.7), of 736 12.8 (11.6), and the caller's time for a second launch, 3; 64
+// chats of 480 25.9 (29.6).
 constexpr int kWholeChunks = 8;
 // From here on a launch of one block works the plan out for all sequences, and
 // a piece looks itself up (1024 chats of 300: 278 us, 376 with a plan in every
@@ -212,7 +214,10 @@ __device__ __forceinline__ Span span_of(const PagedAttnParams& p, int pa, int pb
 struct SequencePlan {
     int first, n;                // rows
     int length;                  // (a negative one counts as 0)
-    int tile_tokens, tiles, chunks;   // chunks of the last tile (no other has more)
+    // chunks: the last tile's.  Under a window a tile before it may have a few
+    // more (it may be fuller, and lie across one more border of chunks): its
+    // pieces are that much longer, and no bound relies on it.
+    int tile_tokens, tiles, chunks;
     bool small;
     __device__ __forceinline__ int cost() const { return small ? 1 : kLargeCost; }   // of a chunk
 };
@@ -291,7 +296,7 @@ __device__ __forceinline__ void place_piece(const PagedAttnParams& p, const Sequ
     } else {
         // The longest first; and since blocks i and i + 256 share a CU, where
         // all have a place the second 256 the other way round (a prompt of
-        // 1800 tokens: 87 us, 90 without; of 2048: 101, 105).
+        // 1800 tokens: 82 us, 85.5 without; of 2048: 94, 97.5).
         const int all = s.tiles * cuts * p.b.kv_heads;
         if (all <= kTarget && local >= kTarget / 2) local = kTarget / 2 + all - 1 - local;
         rest = quotient(local, p.b.kv_heads);
@@ -424,8 +429,9 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     tiles = uniform(wave_isum64(tiles));
     // Rounded, they may be a few more pieces than places, and those run alone
     // at the end: larger ones that all have a place, if up to twice the size
-    // gives such (800 tokens after 8200: 228 us, 264 without; 400 after 4600
-    // 86, 105; 700 after 800 58, 64).
+    // gives such (800 tokens after 8200: 233 us, 273 without; 400 after 4600
+    // 84, 108; 700 after 800 56, 63).  Of up to 64 sequences, whose plans the
+    // lanes hold; more would be worked out anew for every size tried.
     if (p.b.sequences <= kWave && !p.whole && int64_t(tiles) * p.b.kv_heads <= kTarget) {
         int larger = target;
         for (int k = 0; k < 7; ++k) {
