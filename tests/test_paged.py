@@ -1195,6 +1195,69 @@ def test_captured_steps():
 
 
 @gpu
+@pytest.mark.parametrize("sequences", [2, 300])
+def test_captured_batches_that_are_cut(sequences):
+    """Tiles in pieces and their join, with the plan in every wave and in a
+    launch of its own: two graphs, replayed in turn with eager work between."""
+    from harsh4b_amd.paged import paged_attention
+    scenes = []
+    for seed, counts, lengths in ((61, [1, 129], [900, 1111]), (62, [200, 3], [1300, 700])):
+        spare = sequences - 2
+        s = Scene(counts + [1] * spare, lengths + [30] * spare, 2, 5, 128, 64, seed=seed)
+        d, starts = s.device(), torch.from_numpy(s.starts).cuda()
+        scenes.append((d, starts, paged_attention(**d, starts=starts).clone()))
+    torch.cuda.synchronize()
+    graphs = []
+    for d, starts, _ in scenes:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = paged_attention(**d, starts=starts)
+        graphs.append((g, out))
+    for i in range(6):
+        (g, out), (d, starts, expect) = graphs[i % 2], scenes[i % 2]
+        out.fill_(7.0)
+        g.replay()
+        other = scenes[1 - i % 2]
+        assert torch.equal(paged_attention(**other[0], starts=other[1]), other[2]), i
+        torch.cuda.synchronize()
+        assert torch.equal(out, expect), i
+
+
+@gpu
+def test_captured_bookkeeping_of_many_rows():
+    # more rows than the planning block has threads, a table past one block's fork: replays against an eager twin
+    from harsh4b_amd.paged import PagedCache
+    rows, rng = 1100, np.random.default_rng(63)
+    eager, replayed = (PagedCache(1, 9000, 1, 16, sequences=rows, max_pages=16, page_size=16) for _ in range(2))
+    first = rng.integers(0, 30, rows).tolist()
+    parents = torch.from_numpy(rng.integers(-1, rows, rows).astype(np.int32)).cuda()
+    for c in eager, replayed:
+        c.keys.zero_()
+        c.values.copy_(torch.arange(9000, device="cuda")[None, :, None, None, None] % 2039)
+        c.resize(first)
+    want = torch.empty(rows, dtype=torch.int32, device="cuda")
+
+    def step(c):
+        c.fork(parents)
+        torch.add(c.lengths, 3, out=want)
+        c.resize(want)
+        c.compact()
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(replayed)
+    for i in range(5):
+        step(eager)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for name in ("table", "lengths", "refs", "status", "values"):
+            assert torch.equal(getattr(eager, name), getattr(replayed, name)), (i, name)
+    assert int(eager.status.item()) == 0
+
+
+@gpu
 def test_appended_rows_are_the_decode_step_s():
     """The rows that paged_append writes, and its queries, have the bits of the
     decode step's norm and rotation (the oracle's)."""
