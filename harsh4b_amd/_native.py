@@ -57,6 +57,12 @@ class HqPages(ctypes.Structure):
     ]
 
 
+class HqTree(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("starts", vp), ("parents", vp), ("depths", vp), ("ancestors", vp)]
+
+
+HQ_TREE_NODES = 256
 HQ_PAGES_FULL = 1
 HQ_PAGES_BAD = 2
 HQ_PAGES_REFUSED = 4
@@ -72,6 +78,7 @@ _SIGNATURES = {
     "hq_quant_int4_gemv": ([vp, vp, vp, vp, c_int, c_int, vp, vp, vp, vp], c_int),
     "hq_quantize_activation": ([vp, c_int, vp, vp, vp], c_int),
     "hq_rmsnorm": ([vp, vp, vp, c_int, c_float, vp], c_int),
+    "hq_add_rmsnorm_quant": ([vp, vp, vp, vp, vp, vp, c_int, c_int, c_float, vp], c_int),
     "hq_gqa_workspace_bytes": ([c_int, c_int, c_int, c_int], c_size),
     "hq_gqa_decode": ([vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int, vp], c_int),
     "hq_gqa_decode_noalloc": ([vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int, vp], c_int),
@@ -90,6 +97,12 @@ _SIGNATURES = {
                         c_int),
     "hq_paged_attention_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int], c_size),
     "hq_paged_attention": ([vp, vp, vp, c_int, c_int, c_int, c_int, vp, vp, vp], c_int),
+    "hq_tree_plan": ([vp, c_int, vp, vp], c_int),
+    "hq_paged_append_tree": ([vp, vp, vp, c_int, vp, vp, c_float, vp, vp, c_int, vp, vp], c_int),
+    "hq_paged_attention_tree_workspace_bytes": ([c_int, c_int, c_int, c_int], c_size),
+    "hq_paged_attention_tree": ([vp, vp, vp, c_int, c_int, c_int, vp, vp, vp], c_int),
+    "hq_pages_accept_workspace_bytes": ([c_int, c_int, c_int, c_int], c_size),
+    "hq_pages_accept": ([vp, vp, vp, vp, vp, c_int, c_int, vp, vp, vp, vp, vp], c_int),
     "hq_step_layer_blocks": ([ctypes.POINTER(HqModel)], c_int),
     "hq_step_workspace_bytes": ([ctypes.POINTER(HqModel), c_int], c_size),
     "hq_decode_step": ([ctypes.POINTER(HqModel), ctypes.POINTER(HqState), vp], c_int),

@@ -28,6 +28,14 @@ struct PagedBatch {
     int heads, kv_heads, groups;
 };
 
+// The trees of a batch (struct hq_tree), by batch row.
+constexpr int kTreeNodes = HQ_TREE_NODES;
+constexpr int kTreeWords = kTreeNodes / 32;
+struct TreeBatch {
+    const int32_t* depths;
+    const uint32_t* ancestors;   // [tokens, kTreeWords]
+};
+
 // How many of the rising values at[1 .. n] are at most t: i (wave-uniform;
 // every lane calls it; at[0] must exist), and at[i] and (for i < n) at[i + 1].
 // Each round of loads leaves a 64th of them.  Of values that do not rise: some
@@ -101,6 +109,17 @@ inline int paged_check(const hq_pages* c, const void* rows, const int32_t* start
     *b = PagedBatch{c->keys, c->values, c->table, c->lengths, starts, c->status, c->pages, c->page_size,
                     __builtin_ctz(unsigned(c->page_size)), c->sequences, c->max_pages, tokens, heads, c->kv_heads,
                     heads / c->kv_heads};
+    return HQ_OK;
+}
+
+// A tree's pointers, checked on the host: the plan's outputs too.
+inline int tree_check(const hq_tree* t)
+{
+    if (!t || t->tokens < 0 || !t->starts) return HQ_ERR_ARG;
+    if (t->tokens && (!t->parents || !t->depths || !t->ancestors)) return HQ_ERR_ARG;
+    for (const void* q : {static_cast<const void*>(t->starts), static_cast<const void*>(t->parents),
+                          static_cast<const void*>(t->depths), static_cast<const void*>(t->ancestors)})
+        if (reinterpret_cast<uintptr_t>(q) & (q == t->ancestors ? 15u : 3u)) return HQ_ERR_ALIGN;
     return HQ_OK;
 }
 

@@ -1,4 +1,5 @@
-// hq_paged.hip - append to the paged K/V cache on gfx950 (hq_paged_append).
+// hq_paged.hip - append to the paged K/V cache on gfx950 (hq_paged_append, and
+// of drafted trees' nodes hq_paged_append_tree).
 // No reference counterpart: the reference writes one contiguous cache per
 // session (cpu_lightspark.py:435-440), token by token.
 #include <algorithm>
@@ -21,6 +22,7 @@ struct AppendParams {
     int rope_positions;
     int looks;                   // the first blocks, which look at the starts
     float* query;                // [tokens, heads, D]
+    const int32_t* depths;       // (TREE) [tokens]
 };
 
 // A token's heads (q, k, v) over the waves of gridDim.y blocks, PER at a time:
@@ -44,7 +46,8 @@ __device__ __forceinline__ void look_at_starts(const PagedBatch& p, int i, int n
     }
 }
 
-template <int D>
+// TREE: the K and V of a node go to its slot, the rotation is by its depth.
+template <int D, bool TREE>
 __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
 {
     constexpr int VALUES = D == 128 ? 2 : 1;       // a lane holds of a row
@@ -74,12 +77,14 @@ __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
     if (b < 0) return;
     const int pos = paged_position(p.b, b, count, t - first);
     const int page = paged_page(p.b, b, pos);
-    const bool placed = pos >= 0 && pos < p.rope_positions && page >= 0;
+    const int depth = TREE ? p.depths[t] : 0;
+    const int angle = TREE ? pos - (t - first) + depth : pos;      // (pos - (t - first): the tree's base)
+    const bool placed = (TREE ? pos >= t - first && depth >= 0 && depth <= t - first : pos >= 0) && angle < p.rope_positions && page >= 0;
     const bool held = (*p.b.status & (HQ_PAGES_FULL | HQ_PAGES_REFUSED)) != 0;
     if (!placed && lane == 0) atomicOr(p.b.status, HQ_PAGES_BAD);
     // pairs (i, i + D/2): of D = 128 in one lane, else in lanes D/2 apart
     const int pair = VALUES == 2 ? lane : lane & (D / 2 - 1);
-    const size_t rope = size_t(placed ? pos : 0) * (D / 2) + pair;
+    const size_t rope = size_t(placed ? angle : 0) * (D / 2) + pair;
     const float cos = p.rope_cos[rope], sin = p.rope_sin[rope];
     const float qw0 = in ? p.q_norm[lane] : 0.0f, kw0 = in ? p.k_norm[lane] : 0.0f;
     const float qw1 = VALUES == 2 ? p.q_norm[lane + 64] : 0.0f, kw1 = VALUES == 2 ? p.k_norm[lane + 64] : 0.0f;
@@ -141,19 +146,21 @@ __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
 
 using namespace hq;
 
+template <bool TREE>
 static void launch_append(int head_dim, dim3 grid, hipStream_t s, const AppendParams& p)
 {
     switch (head_dim) {
-    case 16: hipLaunchKernelGGL(paged_append_kernel<16>, grid, dim3(kBlock), 0, s, p); break;
-    case 32: hipLaunchKernelGGL(paged_append_kernel<32>, grid, dim3(kBlock), 0, s, p); break;
-    case 64: hipLaunchKernelGGL(paged_append_kernel<64>, grid, dim3(kBlock), 0, s, p); break;
-    default: hipLaunchKernelGGL(paged_append_kernel<128>, grid, dim3(kBlock), 0, s, p); break;
+    case 16: hipLaunchKernelGGL((paged_append_kernel<16, TREE>), grid, dim3(kBlock), 0, s, p); break;
+    case 32: hipLaunchKernelGGL((paged_append_kernel<32, TREE>), grid, dim3(kBlock), 0, s, p); break;
+    case 64: hipLaunchKernelGGL((paged_append_kernel<64, TREE>), grid, dim3(kBlock), 0, s, p); break;
+    default: hipLaunchKernelGGL((paged_append_kernel<128, TREE>), grid, dim3(kBlock), 0, s, p); break;
     }
 }
 
-extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* starts, int tokens, int heads,
-                               const float* q_norm, const float* k_norm, float eps, const float* rope_cos,
-                               const float* rope_sin, int rope_positions, float* query, void* stream)
+template <bool TREE>
+static int run_append(const hq_pages* cache, const float* qkv, const int32_t* starts, const int32_t* depths, int tokens,
+                      int heads, const float* q_norm, const float* k_norm, float eps, const float* rope_cos,
+                      const float* rope_sin, int rope_positions, float* query, void* stream)
 {
     AppendParams p;
     const int err = paged_check(cache, qkv, starts, tokens, heads, query, &p.b);
@@ -168,6 +175,7 @@ extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const in
     p.eps = eps;
     p.rope_positions = rope_positions;
     p.query = query;
+    p.depths = depths;
     // few tokens: kAppendPer heads a wave; many: a block a token, whose waves look its place up once for all their
     // heads (2000 tokens 17.9 us; with kAppendPer heads a wave 23.1)
     const int slots = heads + 2 * cache->kv_heads;
@@ -176,9 +184,27 @@ extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const in
     const int y = tokens < kAppendWide ? (slots + per_block - 1) / per_block : 1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (int64_t(tokens) + p.looks > kMaxBlocks) {  // (a launch of their own)
-        launch_append(cache->head_dim, dim3(p.looks), s, p);
+        launch_append<TREE>(cache->head_dim, dim3(p.looks), s, p);
         p.looks = 0;
     }
-    launch_append(cache->head_dim, dim3(tokens + p.looks, y), s, p);
+    launch_append<TREE>(cache->head_dim, dim3(tokens + p.looks, y), s, p);
     return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
+}
+
+extern "C" int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* starts, int tokens, int heads,
+                               const float* q_norm, const float* k_norm, float eps, const float* rope_cos,
+                               const float* rope_sin, int rope_positions, float* query, void* stream)
+{
+    return run_append<false>(cache, qkv, starts, nullptr, tokens, heads, q_norm, k_norm, eps, rope_cos, rope_sin,
+                             rope_positions, query, stream);
+}
+
+extern "C" int hq_paged_append_tree(const hq_pages* cache, const float* qkv, const hq_tree* tree, int heads,
+                                    const float* q_norm, const float* k_norm, float eps, const float* rope_cos,
+                                    const float* rope_sin, int rope_positions, float* query, void* stream)
+{
+    const int bad = tree_check(tree);
+    if (bad) return bad;
+    return run_append<true>(cache, qkv, tree->starts, tree->depths, tree->tokens, heads, q_norm, k_norm, eps, rope_cos,
+                            rope_sin, rope_positions, query, stream);
 }

@@ -30,6 +30,7 @@ import torch
 
 from . import _native
 from ._native import HqLayer, HqModel, HqState, check
+from .paged import _apart, _launch
 
 DEFAULT_GEMV_KERNEL = "hip-gfx950"
 
@@ -674,6 +675,43 @@ def rmsnorm(x: torch.Tensor, gamma: torch.Tensor, eps: float, out: torch.Tensor 
     check(_native.lib().hq_rmsnorm(x.data_ptr(), gamma.data_ptr(), out.data_ptr(), x.numel(), float(eps),
                                    _stream_handle(stream)), "hq_rmsnorm")
     return out
+
+
+def add_rmsnorm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float, delta: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                      act_scales: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """What stands between the int4 products of a batch (hq_add_rmsnorm_quant):
+    the RMSNorm of x + delta, quantised to int8 a row, as (q int8 [rows, n],
+    act_scales float32 [rows]), which int4_i8_gemm takes; the bits of rmsnorm
+    and quantize_activation row by row.  x, delta: float32 [rows, n].  The sum
+    goes to `out`; without one, and with a delta, to x itself."""
+    index = x.get_device() if isinstance(x, torch.Tensor) else -1
+    if index < 0 or x.dim() != 2 or x.dtype is not torch.float32 or not x.is_contiguous():
+        raise ValueError("x must be a contiguous float32 device tensor [rows, n]")
+    shape = x.shape
+    rows, n = shape
+    if n == 0 or n > 1 << 30 or rows >= 1 << 24:
+        raise ValueError("x must be [rows, n] with n from 1 to 2^30 and fewer than 2^24 rows")
+    for t, name, dims, dtype in ((gamma, "gamma", (n,), torch.float32), (delta, "delta", shape, torch.float32),
+                                 (out, "out", shape, torch.float32), (q, "q", shape, torch.int8),
+                                 (act_scales, "act_scales", (rows,), torch.float32)):
+        if t is None:
+            if name == "gamma":
+                raise ValueError("gamma is needed")
+        elif t.shape != dims or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor {list(dims)} on x's device")
+    if out is None and delta is not None:
+        out = x
+    if q is None:
+        q = torch.empty(shape, dtype=torch.int8, device=x.device)
+    if act_scales is None:
+        act_scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _apart((out, q, act_scales), (x, gamma, delta), (out, x))
+    if rows:
+        _launch(_native.lib().hq_add_rmsnorm_quant,
+                (x.data_ptr(), _ptr(delta), gamma.data_ptr(), _ptr(out), q.data_ptr(), act_scales.data_ptr(), rows, n,
+                 float(eps)), None, index, stream, (x, gamma, delta, out, q, act_scales), "hq_add_rmsnorm_quant")
+    return q, act_scales
 
 
 @functools.lru_cache(maxsize=1024)

@@ -168,6 +168,21 @@ def _launch(entry, args: tuple, nbytes: int | None, index: int, stream, tensors,
         check(status, what)
 
 
+def _apart(outputs: tuple, inputs: tuple, same: tuple = ()) -> None:
+    """Refuse outputs that overlap each other or an input (None: not given).
+    same: an output and the input that it may be, whole and in place."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), t) for t in (*outputs, *inputs)
+             if t is not None]
+    made = sum(t is not None for t in outputs)
+    for i in range(made):
+        low, high, t = spans[i]
+        for other_low, other_high, other in spans[i + 1:]:
+            if other_low < high and low < other_high:
+                if same and t is same[0] and other is same[1] and (low, high) == (other_low, other_high):
+                    continue
+                raise ValueError("outputs must not overlap each other or an input")
+
+
 # --------------------------------------------------------------------------- append, attention
 def paged_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, rope_cos: torch.Tensor,
                  rope_sin: torch.Tensor, eps: float, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor,
@@ -380,6 +395,31 @@ class PagedCache:
         """paged_attention over one layer."""
         return paged_attention(query, self.keys[layer], self.values[layer], self.table, self.lengths, starts, window,
                                sinks, out, stream)
+
+    def plan_tree(self, parents, starts, stream=None):
+        """tree_plan; lists or device tensors."""
+        from .tree import tree_plan
+        return tree_plan(self._ints(parents), self._ints(starts), self.status, stream=stream)
+
+    def append_tree(self, layer: int, qkv, q_norm, k_norm, rope_cos, rope_sin, eps: float, tree, out=None,
+                    stream=None) -> torch.Tensor:
+        """paged_append_tree of one layer."""
+        from .tree import paged_append_tree
+        return paged_append_tree(qkv, q_norm, k_norm, rope_cos, rope_sin, eps, self.keys[layer], self.values[layer],
+                                 self.table, self.lengths, self.status, tree, out, stream)
+
+    def attend_tree(self, layer: int, query, tree, window: int = 0, sinks: int = 0, out=None,
+                    stream=None) -> torch.Tensor:
+        """paged_attention_tree over one layer."""
+        from .tree import paged_attention_tree
+        return paged_attention_tree(query, self.keys[layer], self.values[layer], self.table, self.lengths, tree, window,
+                                    sinks, out, stream)
+
+    def accept(self, tree, drafted, choices=None, logits=None, levels: int = 256, stream=None):
+        """pages_accept over all layers; drafted and choices: lists or device tensors."""
+        from .tree import pages_accept
+        return pages_accept(self.keys, self.values, self.table, self.lengths, self.status, tree, self._ints(drafted),
+                            None if choices is None else self._ints(choices), logits, levels, stream=stream)
 
     def check_status(self) -> None:
         """Wait for the calls so far, on whatever stream, and raise where one was refused."""

@@ -68,6 +68,20 @@ int hq_quantize_activation(const float* x, int n, int8_t* q, float* act_scale, v
  * (kernel.rmsnorm_into, cpu_lightspark.py:431,447,461). */
 int hq_rmsnorm(const float* x, const float* gamma, float* y, int n, float eps, void* stream);
 
+/* ------------------------------------ residual + RMSNorm + int8 rows --
+ * What stands between the int4 products of a batch: per row of `rows`
+ *   sum = x + delta (delta NULL: sum = x)
+ *   y = (sum / sqrt(mean(sum^2) + eps)) * gamma        (hq_rmsnorm)
+ *   q, act_scale = the int8 quantization of y          (hq_quantize_activation)
+ * with those calls' bits.  x, delta fp32 [rows, n]; gamma fp32 [n]; sum fp32
+ * [rows, n], x itself (the residual stream in place), or NULL where delta is
+ * NULL; q int8 [rows, n] and act_scales fp32 [rows] as hq_int4_i8_gemm takes
+ * them.  Otherwise the outputs overlap no input.  No reference counterpart as
+ * one call (cpu_lightspark.py:431-433, 446-449 row by row).  Pointers have
+ * their elements' alignment; 1 <= n <= 2^30, fewer than 2^24 rows. */
+int hq_add_rmsnorm_quant(const float* x, const float* delta, const float* gamma, float* sum, int8_t* q,
+                         float* act_scales, int rows, int n, float eps, void* stream);
+
 /* ------------------------------------------- GQA decode attention --
  * Fused single-token GQA attention: score, softmax and V accumulation per
  * 64-position chunk, with the chunks' combine in the same launch or, for long
@@ -277,6 +291,76 @@ int hq_paged_append(const hq_pages* cache, const float* qkv, const int32_t* star
 size_t hq_paged_attention_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim, int single);
 int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens, int heads,
                        int window, int sinks, float* output, void* workspace, void* stream);
+
+/* ----------------------------------------------------- drafted trees --
+ * A step over trees of drafted tokens: every sequence brings the nodes of a
+ * tree, the model runs all of them at once, and the longest path that its own
+ * choices follow is kept.  No reference counterpart.
+ * Sequence b's nodes are rows starts[b] .. starts[b+1] - 1 (device int32
+ * [sequences + 1], not falling; none: the sequence takes no part).  parents
+ * (int32 [tokens]): the place of a node's parent among its sequence's nodes,
+ * before the node's own; -1: none.  Its first node is the root, the last token
+ * that is sure; any others without a parent are seen by their own descendants
+ * alone.  A tree has at most HQ_TREE_NODES nodes.
+ * In the cache the n nodes take the sequence's last n slots in their order
+ * (lengths count them, as in hq_paged_append): slot base + i for node i, base =
+ * lengths[b] - n.  A node's position is base + its depth. */
+#define HQ_TREE_NODES 256
+typedef struct hq_tree {
+    int32_t tokens;            /* rows of the batch's tensors */
+    int32_t reserved;
+    const int32_t* starts;     /* [sequences + 1] */
+    const int32_t* parents;    /* [tokens] */
+    int32_t* depths;           /* [tokens] nodes above it, or -1 (hq_tree_plan) */
+    uint32_t* ancestors;       /* [tokens, HQ_TREE_NODES / 32] (16-byte aligned) bit i of a node's 256: node i of its
+                                  sequence is the node itself or above it */
+} hq_tree;
+
+/* depths and ancestors from starts and parents, once for all layers of a step.
+ * A sequence with a parent outside its range or with too many nodes gets depths
+ * of -1 and no ancestors, and sets HQ_PAGES_BAD in status (int32 [1]), as do
+ * starts below 0, above `tokens` or falling: such a sequence's rows are not
+ * touched (where starts fall, rows of two sequences get one's or the other's).
+ * Rows of no sequence are not touched. */
+int hq_tree_plan(const hq_tree* tree, int sequences, int32_t* status, void* stream);
+
+/* hq_paged_append of the nodes: node i's K and V go to slot base + i, and
+ * the rotation is by its position, which the rope tables must hold.  A node of
+ * depth -1 sets HQ_PAGES_BAD, writes no K/V and a query of zeros. */
+int hq_paged_append_tree(const hq_pages* cache, const float* qkv, const hq_tree* tree, int heads, const float* q_norm,
+                         const float* k_norm, float eps, const float* rope_cos, const float* rope_sin,
+                         int rope_positions, float* query, void* stream);
+
+/* hq_paged_attention of the nodes: a node sees the slots before base that have
+ * a page, and of its tree its ancestors and itself; with window > 0 only what
+ * stands at positions above its own - window, or below `sinks`.  A node of depth
+ * -1 gets zeros.  `workspace`: hq_paged_attention_tree_workspace_bytes(...)
+ * bytes, 256-byte aligned, of any contents. */
+size_t hq_paged_attention_tree_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim);
+int hq_paged_attention_tree(const hq_pages* cache, const float* query, const hq_tree* tree, int heads, int window,
+                            int sinks, float* output, void* workspace, void* stream);
+
+/* Keep the path that the model's choices follow: from the root, the child whose
+ * drafted token (int32 [tokens]) is the choice at its parent (the first of equal
+ * ones), and so on, at most `levels` nodes with the root (1 .. HQ_TREE_NODES).  The
+ * choices are given (int32 [tokens], logits NULL) or the argmax of logits (fp32
+ * [tokens, vocab], choices NULL) in hq_argmax's order.  The path's K and V move
+ * to slots base, base + 1, .. in every layer of the cache.  Tables and lengths
+ * stay: kept (int32 [sequences]) receives base + the path's nodes, for a
+ * hq_pages_resize to it (or beyond, to the next tree).  path (int32 [tokens]):
+ * the i-th node of the path at row starts[b] + i, then -1.  next (int32
+ * [sequences]): the choice at the path's last node.  A sequence without nodes,
+ * with a root of depth -1 or with a negative base (these two set HQ_PAGES_BAD),
+ * and all of them while status has HQ_PAGES_FULL or HQ_PAGES_REFUSED set, get
+ * kept -1, next -1 and a path of -1; nothing moves.  A row that would move from
+ * or to a slot without a page stays and sets HQ_PAGES_BAD.  Rows of no sequence
+ * are not touched; the logits of rows off the path may be read or not.  The
+ * outputs overlap no input.  `workspace`: hq_pages_accept_workspace_bytes(...) bytes (vocab 0: the
+ * choices are given), 256-byte aligned, of any contents. */
+size_t hq_pages_accept_workspace_bytes(int tokens, int sequences, int vocab, int levels);
+int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const int32_t* drafted, const int32_t* choices,
+                    const float* logits, int vocab, int levels, int32_t* kept, int32_t* path, int32_t* next,
+                    void* workspace, void* stream);
 
 /* ----------------------------------------------------- decode step --
  * One decode step of a Qwen3-shaped model, as LiteSparkQwen.forward_token
