@@ -9,6 +9,9 @@
 
 namespace hq {
 
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
 constexpr int kTreeLanes = kTreeNodes / kWave;   // nodes a lane holds: lane, lane + 64, ..
 constexpr int kTreeWaves = kBlock / kWave;
 
@@ -62,6 +65,11 @@ __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequen
 }
 
 // ------------------------------------------------------------------ accept
+// Greedy choices: a node's choice can be the token of one of its children
+// alone, of the one with the largest logit there (in argmax's order).  So the
+// path is the beginning of a chain that a look at the children's logits gives,
+// from the root to a leaf: one launch finds the argmax of the chain's rows, and
+// no others are read.  The next walks the path and moves K and V.
 struct Best {
     float v;
     int i;
@@ -74,10 +82,10 @@ struct AcceptParams {
     const int32_t* choices;      // or
     const float* logits;         // [tokens, vocab]
     int vocab, levels, shift;
+    int slots;                   // levels of a chain looked at side by side
     int splits;                  // parts of a row of logits
-    Best* best;                  // [tokens, splits], by levels [2, sequences, splits]
-    int32_t* nodes;              // by levels: [levels, sequences] the path's node, or -1
-    int32_t* last;               // by levels: [sequences] the choice where the path ended
+    Best* best;                  // [tokens, splits] (the chains' rows)
+    int32_t* chain;              // [tokens] a sequence's chain in its first rows, then -1
     int32_t* kept;
     int32_t* path;
     int32_t* next;
@@ -85,196 +93,242 @@ struct AcceptParams {
 
 __device__ __forceinline__ Best better(Best a, Best b) { return argmax_better(b.v, b.i, a.v, a.i) ? b : a; }
 
+// The least of the wave's values, in every lane (levels as in wave_max64_all).
+__device__ __forceinline__ int wave_imin64_all(int v)
+{
+    unsigned x = unsigned(v), y = x;
+    swap32(x, y);
+    v = min(int(x), int(y));
+    x = y = unsigned(v);
+    swap16(x, y);
+    v = min(int(x), int(y));
+    v = min(v, dpp_i<kRowShl8>(v));
+    v = min(v, dpp_i<kRowShl4>(v));
+    v = min(v, dpp_i<kRowShl2>(v));
+    v = min(v, dpp_i<kRowShl1>(v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// The best of the wave's, in every lane (no shuffles through LDS: a chain's
+// levels follow one another).
 __device__ __forceinline__ Best wave_best(Best x)
 {
-#pragma unroll
-    for (int o = kWave / 2; o >= 1; o >>= 1)
-        x = better(x, Best{__shfl_xor(x.v, o, kWave), __shfl_xor(x.i, o, kWave)});
-    return x;
+    const uint64_t nans = __ballot(x.v != x.v);
+    const float top = wave_max64_all(x.v);             // (of the numbers)
+    const bool leads = nans ? x.v != x.v : x.v == top;
+    const int i = wave_imin64_all(leads ? x.i : 0x7fffffff);
+    return Best{nans ? __builtin_nanf("") : top, i};
 }
 
-// The best of part `part` of a row of logits, by a block; valid in thread 0.
-__device__ Best row_part_best(const float* row, int vocab, int part, int splits, Best* red)
-{
-    const int each = (vocab + splits - 1) / splits;
-    const int from = min(part * each, vocab), to = min(from + each, vocab);
-    Best x{-__builtin_inff(), 0x7fffffff};
-    for (int i = from + int(threadIdx.x); i < to; i += kBlock) {
-        const float v = row[i];
-        if (argmax_better(v, i, x.v, x.i)) x = Best{v, i};
-    }
-    x = wave_best(x);
-    const int wave = threadIdx.x / kWave;
-    if ((threadIdx.x & (kWave - 1)) == 0) red[wave] = x;
-    __syncthreads();
-    for (int w = 0; w < kTreeWaves; ++w) x = better(x, red[w]);
-    return x;
-}
+// A sequence, its nodes in the lanes of a wave; n = 0: it takes no part
+// (wave-uniform).
+struct Sequence {
+    int first, n, base;
+    int rows;                    // its rows of the batch (whether it takes part or not)
+    bool bad;
+    int parent[kTreeLanes], token[kTreeLanes], choice[kTreeLanes];
 
-// The choice that a row's parts give (wave-uniform; every lane calls it).
-__device__ __forceinline__ int choice_of(const Best* parts, int splits)
-{
-    const int lane = threadIdx.x & (kWave - 1);
-    Best x{-__builtin_inff(), 0x7fffffff};
-    if (lane < splits) x = parts[lane];
-    return __builtin_amdgcn_readfirstlane(wave_best(x).i);
-}
+    int depth, status;
 
-// Whether a sequence takes part (wave-uniform): its rows, and slot of the root.
-__device__ __forceinline__ bool accept_rows(const AcceptParams& p, int b, int* first, int* n, int* base, bool* bad)
-{
-    *bad = !tree_rows(p.t.starts, b, p.t.tokens, first, n);
-    *base = 0;
-    if (*n == 0) return false;
-    *base = p.c.lengths[b] - *n;
-    *bad = p.t.depths[*first] < 0 || *n > kTreeNodes || *base < 0;
-    return !*bad && (*p.c.status & (HQ_PAGES_FULL | HQ_PAGES_REFUSED)) == 0;
-}
-
-// A sequence's nodes in the lanes of a wave.
-struct Nodes {
-    int parent[kTreeLanes], token[kTreeLanes];
-    __device__ __forceinline__ void load(const AcceptParams& p, int first, int n)
+    // Two round trips, the second under way when this returns: the sequence's
+    // numbers, then its nodes' together.
+    __device__ __forceinline__ void load(const AcceptParams& p, int b)
     {
         const int lane = threadIdx.x & (kWave - 1);
+        const int length = p.c.lengths[b];
+        status = *p.c.status;
+        bad = !tree_rows(p.t.starts, b, p.t.tokens, &first, &rows);
+        first = __builtin_amdgcn_readfirstlane(first);
+        rows = __builtin_amdgcn_readfirstlane(rows);
+        base = __builtin_amdgcn_readfirstlane(length) - rows;
+        n = 0;
+        if (rows == 0) return;
+        depth = p.t.depths[first];
 #pragma unroll
         for (int k = 0; k < kTreeLanes; ++k) {
             const int i = lane + k * kWave;
-            parent[k] = i < n ? p.t.parents[first + i] : -2;
-            token[k] = i < n ? p.drafted[first + i] : 0;
+            parent[k] = i < rows ? p.t.parents[first + i] : -2;
+            token[k] = i < rows ? p.drafted[first + i] : 0;
+            choice[k] = i < rows && p.choices ? p.choices[first + i] : 0;
         }
+    }
+    // Whether it takes part.
+    __device__ __forceinline__ bool settle()
+    {
+        if (rows == 0) return false;
+        bad = __builtin_amdgcn_readfirstlane(depth) < 0 || rows > kTreeNodes || base < 0;
+        if (!bad && (__builtin_amdgcn_readfirstlane(status) & (HQ_PAGES_FULL | HQ_PAGES_REFUSED)) == 0) n = rows;
+        return n != 0;
+    }
+    __device__ __forceinline__ bool below(int k, int u) const      // whether the lane's k-th node is a child of u
+    {
+        return parent[k] == u && int(threadIdx.x & (kWave - 1)) + k * kWave > u;
     }
     // The first child of node u that holds `choice`, or -1.
     __device__ __forceinline__ int child(int u, int choice) const
     {
-        const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
         for (int k = 0; k < kTreeLanes; ++k) {
-            const uint64_t m = __ballot(parent[k] == u && token[k] == choice && lane + k * kWave > u);
+            if (k * kWave >= n) break;
+            const uint64_t m = __ballot(below(k, u) && token[k] == choice);
             if (m) return k * kWave + __builtin_ctzll(m);
         }
         return -1;
     }
 };
 
-// Every row's choice, a block a part.
-__global__ __launch_bounds__(kBlock) void accept_rows_kernel(AcceptParams p)
-{
-    __shared__ Best red[kTreeWaves];
-    const int row = blockIdx.x;
-    const Best x = row_part_best(p.logits + size_t(row) * p.vocab, p.vocab, blockIdx.y, p.splits, red);
-    if (threadIdx.x == 0) p.best[size_t(row) * p.splits + blockIdx.y] = x;
-}
+constexpr int kRowAhead = 8;           // fours of logits a thread has on their way
 
-// The path's node of level `level` (from the choice at the one above), or -1: for every block of a sequence.
-__device__ __forceinline__ int step_down(const AcceptParams& p, int b, int level, bool writes)
+// The best of part `part` of a row of logits, by a block; valid in thread 0.
+// The row in fours from its first 16-byte border on; what lies before it goes
+// to part 0, the rest behind the fours to the last part.
+__device__ Best row_part_best(const float* row, int vocab, int part, int splits, Best* red)
 {
-    const int lane = threadIdx.x & (kWave - 1);
-    int first, n, base, v = -1;
-    bool bad;
-    if (level == 0) {
-        if (accept_rows(p, b, &first, &n, &base, &bad)) v = 0;
-    } else {
-        const int u = p.nodes[size_t(level - 1) * p.c.sequences + b];
-        if (u >= 0) {
-            const Best* parts = p.best + (size_t((level - 1) & 1) * p.c.sequences + b) * p.splits;
-            const int choice = choice_of(parts, p.splits);
-            if (level < p.levels) {
-                accept_rows(p, b, &first, &n, &base, &bad);
-                Nodes nodes;
-                nodes.load(p, first, n);
-                v = nodes.child(u, choice);
-            }
-            if (v < 0 && writes && lane == 0) p.last[b] = choice;
+    const int t = threadIdx.x;
+    const int head = min(int(-(reinterpret_cast<uintptr_t>(row) >> 2) & 3), vocab);
+    const int quads = (vocab - head) / 4, each = (quads + splits - 1) / splits;
+    const int from = min(part * each, quads), to = min(from + each, quads);
+    const float4v* body = reinterpret_cast<const float4v*>(row + head);
+    Best x{-__builtin_inff(), 0x7fffffff};
+    // (a thread's indices rise: a later value has to be larger, or the first NaN)
+    auto take = [&](float v, int i) {
+        if (x.i == 0x7fffffff || (!(v <= x.v) && x.v == x.v)) x = Best{v, i};
+    };
+    if (part == 0 && t < head) take(row[t], t);
+    // (the last ones' places taken again rather than one at a time: a round trip each)
+    constexpr int AHEAD = kRowAhead;
+    for (int q = from + t; q < to; q += AHEAD * kBlock) {
+        float4v v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) v[k] = body[min(q + k * kBlock, to - 1)];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (q + k * kBlock >= to) continue;
+            const int i = head + 4 * (q + k * kBlock);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) take(v[k][e], i + e);
         }
     }
-    if (writes && lane == 0 && level < p.levels) p.nodes[size_t(level) * p.c.sequences + b] = v;
-    return v;
+    const int tail = head + 4 * quads + t;
+    if (part == splits - 1 && tail < vocab) take(row[tail], tail);
+    x = wave_best(x);
+    const int wave = t / kWave;
+    __syncthreads();                   // (red's last readers)
+    if ((t & (kWave - 1)) == 0) red[wave] = x;
+    __syncthreads();
+    for (int w = 0; w < kTreeWaves; ++w) x = better(x, red[w]);
+    return x;
 }
 
-// One level of the paths: the node, and the parts of its row of logits.
-__global__ __launch_bounds__(kBlock) void accept_level_kernel(AcceptParams p, int level)
+// The argmax of the chains' rows: blocks (sequence, part of its rows, first of
+// the chain's levels that the block takes, every slots-th).  Every wave works
+// the chain out, while the root's row is read.
+__global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
 {
     __shared__ Best red[kTreeWaves];
-    const int b = blockIdx.x;
-    const int v = step_down(p, b, level, blockIdx.y == 0 && threadIdx.x < kWave);
-    if (v < 0) return;
-    const size_t row = size_t(p.t.starts[b]) + v;
-    const Best x = row_part_best(p.logits + row * p.vocab, p.vocab, blockIdx.y, p.splits, red);
-    if (threadIdx.x == 0) p.best[(size_t(level & 1) * p.c.sequences + b) * p.splits + blockIdx.y] = x;
+    Sequence s;
+    s.load(p, blockIdx.x);
+    if (s.rows == 0) return;
+    auto take_row = [&](int u) {
+        const size_t row = size_t(s.first) + u;
+        const Best x = row_part_best(p.logits + row * p.vocab, p.vocab, blockIdx.y, p.splits, red);
+        if (threadIdx.x == 0) p.best[row * p.splits + blockIdx.y] = x;
+    };
+    const bool writes = blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0;
+    if (blockIdx.z == 0) take_row(0);
+    if (!s.settle()) return;
+    Best own[kTreeLanes];              // a node's logit at its parent
+#pragma unroll
+    for (int k = 0; k < kTreeLanes; ++k) {
+        const int u = s.parent[k], i = s.token[k];
+        own[k] = Best{-__builtin_inff(), 0x7fffffff};
+        if (u >= 0 && i >= 0 && i < p.vocab && s.below(k, u)) own[k] = Best{p.logits[size_t(s.first + u) * p.vocab + i], i};
+    }
+    int u = 0;
+    for (int level = 0; u >= 0 && level < p.levels; ++level) {
+        if (writes) p.chain[s.first + level] = u;
+        if (level > 0 && level % p.slots == int(blockIdx.z)) take_row(u);
+        Best x{-__builtin_inff(), 0x7fffffff};
+#pragma unroll
+        for (int k = 0; k < kTreeLanes; ++k)
+            if (s.below(k, u)) x = better(x, own[k]);
+        const int choice = __builtin_amdgcn_readfirstlane(wave_best(x).i);
+        u = choice == 0x7fffffff ? -1 : s.child(u, choice);
+        if (u < 0 && level + 1 < s.n && writes) p.chain[s.first + level + 1] = -1;
+    }
 }
 
-// The end of a path walked by levels.
-__global__ __launch_bounds__(kBlock) void accept_last_kernel(AcceptParams p)
+// The choices along a sequence's chain, into LDS, by a wave: splits lanes (a
+// power of two) a level, 64 / splits levels at a time.
+__device__ __forceinline__ void chain_choices(const AcceptParams& p, const Sequence& s, int* level_choice)
 {
-    const int b = blockIdx.x * kTreeWaves + threadIdx.x / kWave;
-    if (b < p.c.sequences) step_down(p, b, p.levels, true);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int part = lane & (p.splits - 1), each = kWave / p.splits;
+    const int levels = min(p.levels, s.n);
+    for (int from = 0; from < levels; from += each) {
+        const int level = from + lane / p.splits;
+        // (what follows the chain's end is of any contents)
+        int ended = 0;
+        int u = level < levels ? p.chain[s.first + level] : -1;
+        if (u < 0 || u >= s.n) u = -1;
+        Best x{-__builtin_inff(), 0x7fffffff};
+        if (u >= 0) x = p.best[size_t(s.first + u) * p.splits + part];
+        for (int o = p.splits / 2; o >= 1; o >>= 1)
+            x = better(x, Best{__shfl_xor(x.v, o, kWave), __shfl_xor(x.i, o, kWave)});
+        if (level < levels && part == 0) level_choice[level] = x.i;
+        ended = __any(level < levels && u < 0);
+        if (ended) break;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // The path, and its K and V to their slots: blocks (sequence, slice of the
-// layers' heads); each wave walks the path by itself.
+// layers' heads).  A block's first wave walks the path.
 constexpr int kMoveItems = 4;          // a wave's rows of (layer, K or V, kv head)
 
-template <int D, bool LEVELS>
+template <int D>
 __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
 {
     constexpr int PIECES = D / 8, ROWS = kWave / PIECES;   // 16-byte pieces of a K row, rows a wave moves at a time
+    __shared__ int level_choice[kTreeNodes], path[kTreeNodes];
+    __shared__ int shared_count, shared_base;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int b = blockIdx.x;
-    int first, n, base;
-    bool bad;
-    const bool takes_part = accept_rows(p, b, &first, &n, &base, &bad);
-    const bool writes = blockIdx.y == 0 && wave == 0;
-    int path[kTreeLanes];
-#pragma unroll
-    for (int k = 0; k < kTreeLanes; ++k) path[k] = -1;
-    int count = 0, choice = -1;
-    if (takes_part) {
-        if constexpr (LEVELS) {
-#pragma unroll
-            for (int k = 0; k < kTreeLanes; ++k) {
-                const int level = lane + k * kWave;
-                if (level < p.levels) path[k] = p.nodes[size_t(level) * p.c.sequences + b];
-                count += __popcll(__ballot(path[k] >= 0));
-            }
-            choice = p.last[b];
-        } else {
-            Nodes nodes;
-            nodes.load(p, first, n);
-            int mine[kTreeLanes];
-            if (!p.logits) {
-#pragma unroll
-                for (int k = 0; k < kTreeLanes; ++k) mine[k] = lane + k * kWave < n ? p.choices[first + lane + k * kWave] : 0;
-            }
-            for (int u = 0; u >= 0; u = count < p.levels ? nodes.child(u, choice) : -1) {
-#pragma unroll
-                for (int k = 0; k < kTreeLanes; ++k)
-                    if (lane + k * kWave == count) path[k] = u;
-                ++count;
+    const bool writes = blockIdx.y == 0;
+    if (wave == 0) {
+        Sequence s;
+        s.load(p, b);
+        int count = 0, choice = -1;
+        if (s.settle()) {
+            if (p.logits) chain_choices(p, s, level_choice);
+            for (int u = 0; u >= 0; u = count < p.levels ? s.child(u, choice) : -1) {
+                if (lane == 0) path[count] = u;
                 if (p.logits) {
-                    choice = choice_of(p.best + size_t(first + u) * p.splits, p.splits);
+                    choice = __builtin_amdgcn_readfirstlane(level_choice[count]);
                 } else {
 #pragma unroll
                     for (int k = 0; k < kTreeLanes; ++k)
-                        if (u >> 6 == k) choice = __builtin_amdgcn_readlane(mine[k], u & (kWave - 1));
+                        if (u >> 6 == k) choice = __builtin_amdgcn_readlane(s.choice[k], u & (kWave - 1));
                 }
+                ++count;
             }
         }
-    }
-    if (writes) {
         if (lane == 0) {
-            p.kept[b] = takes_part ? base + count : -1;
-            p.next[b] = choice;
-            if (bad) atomicOr(p.c.status, HQ_PAGES_BAD);
+            shared_count = count;
+            shared_base = s.base;
+            if (writes) {
+                p.kept[b] = s.n ? s.base + count : -1;
+                p.next[b] = choice;
+                if (s.bad) atomicOr(p.c.status, HQ_PAGES_BAD);
+            }
         }
-        for (int i = lane; i < n; i += kWave) {
-            int v = -1;
-#pragma unroll
-            for (int k = 0; k < kTreeLanes; ++k)
-                if (i >> 6 == k) v = path[k];
-            p.path[first + i] = v;
+        if (writes) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int i = lane; i < s.rows; i += kWave) p.path[s.first + i] = i < count ? path[i] : -1;
         }
     }
+    lds_sync();
+    const int count = __builtin_amdgcn_readfirstlane(shared_count), base = __builtin_amdgcn_readfirstlane(shared_base);
     // Rows in the path's order, ROWS at a time, all read before the first is
     // written: node i of the path stands at or behind place i, so what is
     // written is no later one's source.
@@ -282,10 +336,7 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
     const size_t head = size_t(p.c.page_size) * D;
     for (int from = 0; from < count; from += ROWS) {
         const int i = from + lane / PIECES;
-        int v = -1;
-#pragma unroll
-        for (int k = 0; k < kTreeLanes; ++k)
-            if (from >> 6 == k) v = __shfl(path[k], i & (kWave - 1), kWave);
+        const int v = i < count ? path[i] : -1;
         bool moves = i < count && v != i;
         if (!__any(moves)) continue;
         auto page_of = [&](int slot) {
@@ -303,53 +354,57 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
         const size_t src = size_t(max(of, 0)) * heads * head + size_t((base + max(v, 0)) & (p.c.page_size - 1)) * D + place;
         for (int item = (blockIdx.y * kTreeWaves + wave) * kMoveItems; item < items;
              item += gridDim.y * kTreeWaves * kMoveItems) {
-            uint4 x[kMoveItems];
+            uint4v x[kMoveItems];
             uint16_t* at[kMoveItems];
+            int rest = item / heads, h = item - rest * heads;
 #pragma unroll
             for (int k = 0; k < kMoveItems; ++k) {
-                const int it = min(item + k, items - 1);
-                const int h = it % heads, rest = it / heads;
                 at[k] = ((rest & 1) ? p.c.values : p.c.keys) + (size_t(rest >> 1) * p.c.pages * heads + h) * head;
-                if (moves) x[k] = *reinterpret_cast<const uint4*>(at[k] + src);
+                x[k] = uint4v{0, 0, 0, 0};
+                if (moves && item + k < items) x[k] = *reinterpret_cast<const uint4v*>(at[k] + src);
+                if (++h == heads) {
+                    h = 0;
+                    ++rest;
+                }
             }
 #pragma unroll
             for (int k = 0; k < kMoveItems; ++k)
-                if (moves && item + k < items) *reinterpret_cast<uint4*>(at[k] + dst) = x[k];
+                if (moves && item + k < items) *reinterpret_cast<uint4v*>(at[k] + dst) = x[k];
         }
     }
 }
 
 // -------------------------------------------------------------------- host
-// How the choices are found: each row's of the batch in one launch, or a launch
-// for each level of the paths that reads its nodes' rows alone.
 struct AcceptPlan {
-    bool by_levels;
-    int splits;
-    size_t nodes, last, total;   // (best is at 0)
+    int slots, splits;
+    size_t chain, total;         // (best is at 0)
 };
+
+// Blocks aimed at for the rows of the chains' levels, many of which no chain reaches.
+constexpr int kChainBlocks = 512;
 
 static AcceptPlan accept_plan(int tokens, int sequences, int vocab, int levels)
 {
     AcceptPlan a{};
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
-    const double row_us = vocab * 4.0 / 5e6;
-    a.by_levels = vocab > 0 && tokens * row_us > levels * (3.0 + sequences * row_us);
-    const int64_t rows = std::max(1, a.by_levels ? sequences : tokens);
-    a.splits = vocab ? int(std::max<int64_t>(1, std::min<int64_t>({64, (1024 + rows - 1) / rows, (vocab + 2047) / 2048}))) : 0;
-    a.nodes = up((a.by_levels ? 2 * rows : rows) * a.splits * sizeof(Best));
-    a.last = a.nodes + (a.by_levels ? up(size_t(levels) * sequences * 4) : 0);
-    a.total = a.last + (a.by_levels ? up(size_t(sequences) * 4) : 0);
+    if (vocab) {                                       // (a power of two: see chain_choices)
+        a.slots = int(std::max<int64_t>(1, std::min<int64_t>({levels, tokens, 16, kMaxBlocks / sequences})));
+        a.splits = 1;
+        const int64_t rows = int64_t(sequences) * a.slots;
+        while (a.splits < kWave && a.splits * rows < kChainBlocks && a.splits * 2048 < vocab) a.splits *= 2;
+    }
+    a.chain = up(size_t(tokens) * a.splits * sizeof(Best));
+    a.total = a.chain + up(vocab ? size_t(tokens) * 4 : 0);
     return a;
 }
 
-template <bool LEVELS>
 static void launch_move(const AcceptParams& p, dim3 grid, hipStream_t s)
 {
     switch (p.c.head_dim) {
-    case 16: hipLaunchKernelGGL((accept_move_kernel<16, LEVELS>), grid, dim3(kBlock), 0, s, p); break;
-    case 32: hipLaunchKernelGGL((accept_move_kernel<32, LEVELS>), grid, dim3(kBlock), 0, s, p); break;
-    case 64: hipLaunchKernelGGL((accept_move_kernel<64, LEVELS>), grid, dim3(kBlock), 0, s, p); break;
-    default: hipLaunchKernelGGL((accept_move_kernel<128, LEVELS>), grid, dim3(kBlock), 0, s, p); break;
+    case 16: hipLaunchKernelGGL(accept_move_kernel<16>, grid, dim3(kBlock), 0, s, p); break;
+    case 32: hipLaunchKernelGGL(accept_move_kernel<32>, grid, dim3(kBlock), 0, s, p); break;
+    case 64: hipLaunchKernelGGL(accept_move_kernel<64>, grid, dim3(kBlock), 0, s, p); break;
+    default: hipLaunchKernelGGL(accept_move_kernel<128>, grid, dim3(kBlock), 0, s, p); break;
     }
 }
 
@@ -394,23 +449,16 @@ extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const
         if (reinterpret_cast<uintptr_t>(q) & 3u) return HQ_ERR_ALIGN;
     const AcceptPlan a = accept_plan(tree->tokens, cache->sequences, vocab, levels);
     char* ws = static_cast<char*>(workspace);
-    AcceptParams p{*cache, *tree, drafted, choices, logits, vocab, levels, batch.shift, a.splits,
-                   reinterpret_cast<Best*>(ws), reinterpret_cast<int32_t*>(ws + a.nodes),
-                   reinterpret_cast<int32_t*>(ws + a.last), kept, path, next};
+    AcceptParams p{*cache, *tree, drafted, choices, logits, vocab, levels, batch.shift, a.slots, a.splits,
+                   reinterpret_cast<Best*>(ws), reinterpret_cast<int32_t*>(ws + a.chain), kept, path, next};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t items = int64_t(2) * cache->layers * cache->kv_heads;
     if (items > 0x7fffffff) return HQ_ERR_ARG;
     const int per_block = kTreeWaves * kMoveItems;
     const int slices = int(std::min({(items + per_block - 1) / per_block, kMaxBlocks / cache->sequences, int64_t(4096)}));
-    if (a.by_levels) {
-        for (int level = 0; level < levels; ++level)
-            hipLaunchKernelGGL(accept_level_kernel, dim3(cache->sequences, a.splits), dim3(kBlock), 0, s, p, level);
-        hipLaunchKernelGGL(accept_last_kernel, dim3((cache->sequences + kTreeWaves - 1) / kTreeWaves), dim3(kBlock), 0, s, p);
-        launch_move<true>(p, dim3(cache->sequences, slices), s);
-    } else {
-        if (logits && tree->tokens)
-            hipLaunchKernelGGL(accept_rows_kernel, dim3(tree->tokens, a.splits), dim3(kBlock), 0, s, p);
-        launch_move<false>(p, dim3(cache->sequences, slices), s);
+    if (logits && tree->tokens) {
+        hipLaunchKernelGGL(accept_chain_kernel, dim3(cache->sequences, a.splits, a.slots), dim3(kBlock), 0, s, p);
     }
+    launch_move(p, dim3(cache->sequences, slices), s);
     return hipGetLastError() == hipSuccess ? HQ_OK : HQ_ERR_LAUNCH;
 }

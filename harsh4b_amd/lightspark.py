@@ -692,25 +692,34 @@ def add_rmsnorm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float, delta: t
     rows, n = shape
     if n == 0 or n > 1 << 30 or rows >= 1 << 24:
         raise ValueError("x must be [rows, n] with n from 1 to 2^30 and fewer than 2^24 rows")
+    if gamma is None:
+        raise ValueError("gamma is needed")
     for t, name, dims, dtype in ((gamma, "gamma", (n,), torch.float32), (delta, "delta", shape, torch.float32),
                                  (out, "out", shape, torch.float32), (q, "q", shape, torch.int8),
                                  (act_scales, "act_scales", (rows,), torch.float32)):
-        if t is None:
-            if name == "gamma":
-                raise ValueError("gamma is needed")
-        elif t.shape != dims or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        if t is not None and (t.shape != dims or t.dtype is not dtype or t.get_device() != index or
+                              not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor {list(dims)} on x's device")
-    if out is None and delta is not None:
-        out = x
+    if out is not None or q is not None or act_scales is not None:
+        _apart((out, q, act_scales), (x, gamma, delta), (out, x))
+    if delta is None:
+        out_ptr = None if out is None else out.data_ptr()
+        delta_ptr = None
+    else:
+        delta_ptr = delta.data_ptr()
+        if out is None:
+            if abs(delta_ptr - x.data_ptr()) < 4 * rows * n:
+                raise ValueError("x takes the sum: delta must not overlap it")
+            out = x
+        out_ptr = out.data_ptr()
     if q is None:
         q = torch.empty(shape, dtype=torch.int8, device=x.device)
     if act_scales is None:
         act_scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _apart((out, q, act_scales), (x, gamma, delta), (out, x))
     if rows:
         _launch(_native.lib().hq_add_rmsnorm_quant,
-                (x.data_ptr(), _ptr(delta), gamma.data_ptr(), _ptr(out), q.data_ptr(), act_scales.data_ptr(), rows, n,
-                 float(eps)), None, index, stream, (x, gamma, delta, out, q, act_scales), "hq_add_rmsnorm_quant")
+                (x.data_ptr(), delta_ptr, gamma.data_ptr(), out_ptr, q.data_ptr(), act_scales.data_ptr(), rows, n, eps),
+                None, index, stream, (x, gamma, delta, out, q, act_scales), "hq_add_rmsnorm_quant")
     return q, act_scales
 
 
