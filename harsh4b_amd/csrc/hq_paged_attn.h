@@ -73,6 +73,10 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int kChunkKeys = 64;
 constexpr int kSmallRows = 16;
 constexpr int kTileRows = 128;
+// Rows of a tile that streams K and V to registers: 16, of trees up to 32.
+template <bool TREE>
+constexpr int kStreamRows = TREE ? 2 * kSmallRows : kSmallRows;
+constexpr int kStreamNodes = 64;       // of a tree whose tiles do (its ancestors are held in registers)
 // Pieces aimed at: one for each place on the chip (two blocks a CU), all
 // started at once.  With twice as many, 16 windows of 1024 take 28 us (23), 3
 // chats of 40960 92 (86), a question of 501 tokens after 7000 142 (129).
@@ -83,6 +87,7 @@ constexpr int kLargeMin = 4;           // of a large one (100 tokens after 1024:
 // a prompt's 250 tokens takes 75 us so, 82 with 1, 79 with 3 (over data that
 // the last-level cache does not hold; where it does 67, 75, 72).
 constexpr int kLargeCost = 2;
+constexpr int kTreeCost = 2, kTreeCostHalf = 2, kTreeCostLarge = 3;
 // Where there is a tile for every CU, large ones of so few chunks stay whole:
 // a second block on the CU gains less than the join of the parts costs (4 x
 // 256 tokens at 512: 34 us, 43 in two pieces each; at 1024 51, 59; 1000 tokens
@@ -109,6 +114,7 @@ struct PagedAttnParams {
     int window, sinks;           // window 0: none
     int tile_tokens;             // tokens of a large tile
     int by_group;                // 65536 / groups + 1, for row_token
+    bool narrow;                 // (TREE) sequences of few chunks have tiles of 16 rows
     bool whole;                  // no tile is cut (short tables): no join
     bool planned;                // the plan is in plan_first, plan_item, plan_count
     int part_rows;               // rows of partial results there is room for
@@ -144,33 +150,34 @@ __device__ __forceinline__ bool paged_visible(int pos, int j, int window, int si
 // Keys below the k-th of a mask's 32.
 __device__ __forceinline__ uint32_t below(int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; }
 
-// Which of the slots j0 .. j0 + 31 a tree's node sees (pages aside): batch row
-// `row`, in slot `slot`, of a sequence whose tree's first node is row `first`,
-// in slot `base`.
-__device__ __forceinline__ uint32_t tree_mask(const PagedAttnParams& p, int row, int first, int base, int slot, int j0)
+// Which of the slots j0 .. j0 + 31 a tree's node sees (pages aside): a node of
+// depth `depth` in slot `slot`, of a sequence whose tree's first node is batch
+// row `first`, in slot `base`.  nodes: the node's ancestor bits from the node
+// in slot max(j0, base) on.
+__device__ __forceinline__ uint32_t tree_mask(const PagedAttnParams& p, int depth, int first, int base, int slot, int j0,
+                                              uint32_t nodes)
 {
-    const int depth = p.tree.depths[row];
-    if (depth < 0) return 0;
-    const int pos = base + depth;
-    const int to_base = base - j0;
+    const int pos = base + depth, to_base = base - j0, to_slot = slot + 1 - j0;
     uint32_t before = below(to_base);
     if (p.window > 0) before &= ~below(max(0, pos - p.window + 1) - j0) | below(p.sinks - j0);
-    if (to_base >= 32) return before & below(slot + 1 - j0);
-    // the row's bits of nodes -to_base ..
-    const uint32_t* bits = p.tree.ancestors + size_t(row) * kTreeWords;
-    const int word = to_base > 0 ? 0 : -to_base >> 5, shift = to_base > 0 ? 0 : -to_base & 31;
-    const uint32_t low = word < kTreeWords ? bits[word] : 0u, high = word + 1 < kTreeWords ? bits[word + 1] : 0u;
-    uint32_t nodes = uint32_t(((uint64_t(high) << 32) | low) >> shift);
-    if (to_base > 0) nodes <<= to_base;
-    nodes &= below(slot + 1 - j0);
+    nodes = to_base >= 32 ? 0u : nodes << max(to_base, 0);
     // (a path longer than the window: by the nodes' positions)
     if (p.window > 0 && depth >= p.window)
-        for (uint32_t left = nodes; left; left &= left - 1) {
+        for (uint32_t left = nodes & below(to_slot); left; left &= left - 1) {
             const int i = __builtin_ctz(left);
             const int above = p.tree.depths[first + i - to_base];
             if (depth - above >= p.window && base + above >= p.sinks) nodes &= ~(1u << i);
         }
-    return before | nodes;
+    return depth < 0 ? 0u : (before | nodes) & below(to_slot);
+}
+
+// A node's ancestor bits from node `from` on.
+__device__ __forceinline__ uint32_t tree_bits(const PagedAttnParams& p, int row, int from)
+{
+    const uint32_t* bits = p.tree.ancestors + size_t(row) * kTreeWords;
+    const int word = min(from >> 5, kTreeWords);
+    const uint32_t low = bits[min(word, kTreeWords - 1)], high = bits[min(word + 1, kTreeWords - 1)];
+    return uint32_t((uint64_t(word + 1 < kTreeWords ? high : 0u) << 32 | (word < kTreeWords ? low : 0u)) >> (from & 31));
 }
 
 constexpr float kLog2e = 0x1.715476p+0f;
@@ -263,7 +270,7 @@ struct SequencePlan {
     // pieces are that much longer, and no bound relies on it.
     int tile_tokens, tiles, chunks;
     bool small;
-    __device__ __forceinline__ int cost() const { return small ? 1 : kLargeCost; }   // of a chunk
+    int cost;                    // of a chunk
 };
 
 template <bool TREE>
@@ -275,18 +282,26 @@ __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, 
     s.small = true;
     s.tile_tokens = s.tiles = 1;
     s.length = max(0, p.b.lengths[b]);
-    if (p.b.starts) {
+    if (TREE || p.b.starts) {
         const int a = p.b.starts[b], z = p.b.starts[b + 1];
         *fall |= a > z;
         s.first = a;
         s.n = a < 0 || a >= z || z > p.b.tokens ? 0 : z - a;
-        s.small = s.n <= kSmallRows / p.b.groups;
+        s.small = s.n <= kStreamRows<TREE> / p.b.groups;
         s.tile_tokens = s.small ? max(1, s.n) : p.tile_tokens;
         s.tiles = s.small ? min(s.n, 1) : quotient(s.n + s.tile_tokens - 1, s.tile_tokens);
     }
+    if (TREE) s.cost = s.small ? kTreeCost : s.n * p.b.groups <= kTileRows / 2 ? kTreeCostHalf : kTreeCostLarge;
+    else s.cost = s.small ? 1 : kLargeCost;
     const int origin = s.length - s.n;
     // (a tree's nodes may all be roots: their positions are at or past the base)
     s.chunks = s.n ? span_of(p, TREE ? origin : origin + (s.tiles - 1) * s.tile_tokens, s.length - 1).count : 0;
+    if (TREE && p.narrow && s.chunks <= kWholeChunks && s.n > kSmallRows / p.b.groups && s.n <= kStreamNodes) {
+        s.small = true;
+        s.cost = kTreeCost;
+        s.tile_tokens = kSmallRows / p.b.groups;
+        s.tiles = quotient(s.n + s.tile_tokens - 1, s.tile_tokens);
+    }
     return s;
 }
 
@@ -300,9 +315,14 @@ struct Piece {
     int pieces, split, part;     // part: first partial row of this piece
     bool small;
     __device__ __forceinline__ int position(int i) const { return max(pos + i, -1); }
-    __device__ __forceinline__ uint32_t mask(const PagedAttnParams& p, int i, int j0) const   // (TREE) of its i-th token
+    // (TREE) what its i-th token, of depth `depth`, sees of the slots j0 .. j0 + 31; nodes: see tree_mask
+    __device__ __forceinline__ uint32_t mask(const PagedAttnParams& p, int i, int depth, int j0, uint32_t nodes) const
     {
-        return tree_mask(p, first + i, first - (pos - base), base, position(i), j0);
+        return tree_mask(p, depth, first - (pos - base), base, position(i), j0, nodes);
+    }
+    __device__ __forceinline__ uint32_t bits(const PagedAttnParams& p, int i, int j0) const
+    {
+        return tree_bits(p, first + i, max(0, j0 - base));
     }
 };
 
@@ -323,15 +343,17 @@ __device__ __forceinline__ int wave_prefix(int v)
 
 // Pieces a sequence's tiles are cut in for pieces of about `target` chunks;
 // tiles: of the whole batch (of one kv head).
+template <bool TREE>
 __device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequencePlan& s, int target, int tiles)
 {
-    if (p.whole) return 1;
+    if (p.whole || (s.small && s.tiles > 1)) return 1;
     if (!s.small && s.chunks <= kLargeWhole && int64_t(tiles) * p.b.kv_heads >= kTarget / 2) return 1;
-    const int size = max(target, s.small ? kSmallMin : kLargeMin * kLargeCost);
-    return max(1, int(float(s.chunks * s.cost()) / float(size) + 0.5f));
+    const int size = max(target, s.small ? kSmallMin * (TREE ? kTreeCost : 1) : kLargeMin * s.cost);
+    return max(1, int(float(s.chunks * s.cost) / float(size) + 0.5f));
 }
 
 // Sequence b's piece number `local`, of `cuts` a tile; its partial rows start at first_part.
+template <bool TREE>
 __device__ __forceinline__ void place_piece(const PagedAttnParams& p, const SequencePlan& s, int b, int local, int cuts,
                                             int first_part, Piece& out)
 {
@@ -340,10 +362,10 @@ __device__ __forceinline__ void place_piece(const PagedAttnParams& p, const Sequ
     out.small = s.small;
     out.length = s.length;
     int rest, tile;
-    if (out.small) {                                         // (one tile)
+    if (out.small) {                                         // (one tile, but for narrow ones, of one piece each)
         rest = quotient(local, p.b.kv_heads);
-        out.split = rest;
-        tile = 0;
+        out.split = TREE && cuts == 1 ? 0 : rest;
+        tile = TREE && cuts == 1 ? rest : 0;
     } else {
         // The longest first; and since blocks i and i + 256 share a CU, where
         // all have a place the second 256 the other way round (a prompt of
@@ -363,7 +385,7 @@ __device__ __forceinline__ void place_piece(const PagedAttnParams& p, const Sequ
     out.base = out.length - s.n;
     out.pos = out.base + tile * s.tile_tokens;
     out.part = first_part + (((tile * p.b.kv_heads + out.head) * out.pieces) + out.split) *
-                                (out.small ? kSmallRows : kTileRows);
+                                (out.small ? kStreamRows<TREE> : kTileRows);
 }
 
 // Chunks a piece should have, for all the batch's chunks (of one kv head).
@@ -390,7 +412,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedAttnParam
     SequencePlan mine{};
     for (int b = t; b < p.b.sequences; b += kPlanThreads) {
         mine = sequence_plan<TREE>(p, b, &fall);
-        units += int64_t(mine.tiles) * mine.chunks * mine.cost();
+        units += int64_t(mine.tiles) * mine.chunks * mine.cost;
         sum += mine.tiles;
     }
     if (sum) atomicAdd(&all_tiles, sum);
@@ -404,9 +426,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedAttnParam
             const int b = base + t;
             if (p.b.sequences > kPlanThreads && b < p.b.sequences) mine = sequence_plan<TREE>(p, b, &fall);
             if (b >= p.b.sequences) mine.tiles = 0;
-            const int cuts = cuts_of(p, mine, target, tiles);
+            const int cuts = cuts_of<TREE>(p, mine, target, tiles);
             const int here = mine.tiles * cuts * p.b.kv_heads;
-            const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
+            const int part = cuts > 1 ? here * (mine.small ? kStreamRows<TREE> : kTileRows) : 0;
             const uint64_t has = __ballot(here > 0);
             const int incl = wave_prefix(here), part_incl = wave_prefix(part);
             __syncthreads();                   // (wave_sum's last readers)
@@ -439,7 +461,7 @@ template <bool TREE>
 __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piece& out)
 {
     const int lane = threadIdx.x & (kWave - 1);
-    if (p.whole && !p.b.starts) {              // a tile a block: nothing to count
+    if (!TREE && p.whole && !p.b.starts) {     // a tile a block: nothing to count
         out.b = uniform(quotient(q, p.b.kv_heads));
         out.head = q - out.b * p.b.kv_heads;
         out.first = out.b;
@@ -459,7 +481,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         if (i >= count) return false;
         const int4 item = p.plan_item[i];
         const int b = uniform(item.x);
-        place_piece(p, sequence_plan<TREE>(p, b, &fall), b, q - first, uniform(item.y), uniform(item.z), out);
+        place_piece<TREE>(p, sequence_plan<TREE>(p, b, &fall), b, q - first, uniform(item.y), uniform(item.z), out);
         return true;
     }
     int64_t units = 0;
@@ -468,7 +490,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     for (int base = 0; base < p.b.sequences; base += kWave) {
         if (base + lane < p.b.sequences) {
             mine = sequence_plan<TREE>(p, base + lane, &fall);
-            units += int64_t(mine.tiles) * mine.chunks * mine.cost();
+            units += int64_t(mine.tiles) * mine.chunks * mine.cost;
             tiles += mine.tiles;
         }
     }
@@ -488,13 +510,13 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     // lanes hold; more would be worked out anew for every size tried.
     if (p.b.sequences <= kWave && !p.whole && int64_t(tiles) * p.b.kv_heads <= kTarget) {
         int larger = target;
-        for (int k = 0; k < 7; ++k) {
-            if (uniform(wave_isum64(mine.tiles * cuts_of(p, mine, larger, tiles))) * p.b.kv_heads <= kTarget) {
-                target = larger;
-                break;
-            }
-            larger += larger / 8 + 1;
+        bool fits = false;
+        for (int k = 0; k < 7 && !fits; ++k) {
+            fits = uniform(wave_isum64(mine.tiles * cuts_of<TREE>(p, mine, larger, tiles))) * p.b.kv_heads <= kTarget;
+            if (fits) target = larger;
+            else larger += larger / 8 + 1;
         }
+        if (TREE && !fits) target = 0x40000000;              // (no cuts: the launch has kTarget blocks)
     }
     int pieces = 0, rows = 0;
     bool got = false;
@@ -502,9 +524,9 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
         const bool in = base + lane < p.b.sequences;
         if (p.b.sequences > kWave && in) mine = sequence_plan<TREE>(p, base + lane, &fall);
         if (!in) mine.tiles = 0;
-        const int cuts = cuts_of(p, mine, target, tiles);
+        const int cuts = cuts_of<TREE>(p, mine, target, tiles);
         const int here = mine.tiles * cuts * p.b.kv_heads;
-        const int part = cuts > 1 ? here * (mine.small ? kSmallRows : kTileRows) : 0;
+        const int part = cuts > 1 ? here * (mine.small ? kStreamRows<TREE> : kTileRows) : 0;
         const int incl = wave_prefix(here), part_incl = wave_prefix(part);
         const uint64_t found = __ballot(q >= pieces + incl - here && q < pieces + incl);
         got |= found != 0;
@@ -518,7 +540,7 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
             s.tile_tokens = from(mine.tile_tokens);
             s.tiles = from(mine.tiles);
             s.small = from(mine.small);
-            place_piece(p, s, base + src, q - from(pieces + incl - here), from(cuts), from(rows + part_incl - part), out);
+            place_piece<TREE>(p, s, base + src, q - from(pieces + incl - here), from(cuts), from(rows + part_incl - part), out);
             if (q != 0) return true;
         }
         pieces += __builtin_amdgcn_readlane(incl, kWave - 1);
@@ -604,7 +626,7 @@ __device__ void redo_row(const PagedAttnParams& p, const Piece& w, const Span& s
     for (int c = c0; c < c1; ++c) {
         const int at = span.chunk(c) * kChunkKeys;
         paged_row<D>(p, p.query + row * D, w.b, w.head, at, int(min(end, int64_t(at) + kChunkKeys)),
-                     [&](int j) { return TREE ? (w.mask(p, token, j) & 1u) != 0
+                     [&](int j) { return TREE ? (w.mask(p, token, p.tree.depths[w.first + token], j, w.bits(p, token, j)) & 1u) != 0
                                               : paged_visible(w.position(token), j, p.window, p.sinks); },
                      m, l, o, seen);
     }
@@ -621,16 +643,20 @@ __device__ void redo_row(const PagedAttnParams& p, const Piece& w, const Span& s
 }
 
 // ---------------------------------------------------------------- small tiles
-template <int D>
+template <int D, bool TREE>
 struct SmallShared {
     float o[4][kSmallRows][D + 4];             // (+ 4: the rows start in different banks)
     float m[4][kSmallRows], l[4][kSmallRows];
-    int bad[kSmallRows];
+    int bad[kStreamRows<TREE>];
+    // two sets' query parts, lane by lane, and factors (see small_tile)
+    half8 q[TREE ? 2 : 1][TREE ? (D + 31) / 32 : 1][2][TREE ? kWave : 1];
+    float c[2][kSmallRows];
 };
 
-template <int D, bool TREE>
+// R sets of 16 rows on the same keys.
+template <int D, bool TREE, int R>
 __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span& span, int c0, int c1,
-                           SmallShared<D>& S)
+                           SmallShared<D, TREE>& S)
 {
     constexpr int STEPS = (D + 31) / 32;       // products over the dims
     constexpr int VEC = D / 16;                // dims a lane holds of a V row
@@ -639,16 +665,27 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const int G = p.b.groups;
     const int rows = w.n * G;
     const int ps = p.b.page_size;
-    const bool mine = n < rows;
-    const int token = mine ? row_token(p, n) : 0;
-    const int pos = w.position(token);
+    bool mine[R];
+    int token[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = 16 * r + n;
+        mine[r] = row < rows;
+        token[r] = mine[r] ? row_token(p, row) : 0;
+    }
     // (of a tree: no row sees less than all slots before the base, none more than those up to its own)
     const int pos_min = TREE ? w.base - 1 : w.position(0), pos_max = w.position(w.n - 1);
-    float4v acc[VEC];
+    float4v acc[R][VEC];
+    float m[R], l[R];
+    bool seen[R];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -__builtin_inff(), l = 0.0f;
-    bool seen = false;
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[r][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        m[r] = -__builtin_inff();
+        l[r] = 0.0f;
+        seen[r] = false;
+    }
 
     // this wave's steps of 32 keys: wave, wave + 4, ...; pages of 32 of them at a time, two a step, in a register
     const int steps = 2 * (c1 - c0);
@@ -698,11 +735,26 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         }
     };
     const int own = steps > wave ? (steps - wave + 3) / 4 : 0;
+    // (TREE) the rows' depths and ancestors: of at most kStreamNodes
+    int depth[TREE ? R : 1];
+    uint64_t bits[TREE ? R : 1];
+    if constexpr (TREE) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            depth[r] = p.tree.depths[w.first + token[r]];
+            bits[r] = *reinterpret_cast<const uint64_t*>(p.tree.ancestors + size_t(w.first + token[r]) * kTreeWords);
+        }
+    }
     // This lane's query row (n), dims 32 s + 8 g ..: its loads, the page
     // table's and then the first step's of K and V are under way together.
+    // Of two sets wave 0 and 2 split the first for all, 1 and 3 the second.
+    constexpr bool SHARED = R > 1;
+    const int q_set = SHARED ? wave & 1 : 0;
     float4v x[STEPS][2];
     {
-        const float* q = p.query + (size_t(w.first + token) * p.b.heads + w.head * G + (mine ? n - token * G : 0)) * D;
+        const int i = SHARED && q_set ? 1 : 0;
+        const float* q = p.query + (size_t(w.first + (i ? token[R - 1] : token[0])) * p.b.heads + w.head * G +
+                                    ((i ? mine[R - 1] : mine[0]) ? 16 * i + n - (i ? token[R - 1] : token[0]) * G : 0)) * D;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int d = D >= 32 ? 32 * s + 8 * g : 8 * (g & 1);
@@ -717,8 +769,8 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         load_k(pg0, pg1, j0);
         load_v(pg0, pg1, j0);
     }
-    half8 qhi[STEPS], qlo[STEPS];
-    float c;
+    half8 qhi[R][STEPS], qlo[SHARED ? 1 : R][STEPS];   // (of two sets the remainders stay in LDS)
+    float c[R];
     {
         const bool used = D >= 32 || g < 2;   // (a lane of no row: the tile's first row, not stored)
         float top = 0.0f;
@@ -733,13 +785,32 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
         top = max_over_g(top);
         const int e = row_exponent(top);
         const float down = __builtin_ldexpf(1.0f, -e);
+        c[0] = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
+            if (SHARED && STEPS > 1 && (s & 1) != wave >> 1) continue;
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[s][i] *= down;
-            split8(y[s], qhi[s], qlo[s]);
+            half8 hi, lo;
+            split8(y[s], hi, lo);
+            if constexpr (SHARED) {
+                S.q[q_set][s][0][lane] = hi;
+                S.q[q_set][s][1][lane] = lo;
+            } else {
+                qhi[0][s] = hi;
+                qlo[0][s] = lo;
+            }
         }
-        c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
+    }
+    if constexpr (SHARED) {
+        if (g == 0 && wave < 2) S.c[q_set][n] = c[0];
+        lds_sync();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            c[r] = S.c[r][n];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) qhi[r][s] = S.q[r][s][0][lane];
+        }
     }
     for (int k = 0; k < own; ++k) {
         // the next step's pages
@@ -751,62 +822,92 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
             next1 = __builtin_amdgcn_readlane(pg, 2 * (kn & 31) + 1);
             nj = key_of(wave + 4 * kn);
         }
-        float4v s[2];
+        float4v s[R][2];
+        if constexpr (SHARED) {
+            uint32_t at = lane;                // (the compiler would read the remainders once for all steps)
+            asm volatile("" : "+v"(at));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            s[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            // (products that follow one another go to different sums)
 #pragma unroll
             for (int d = 0; d < STEPS; ++d) {
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qlo[d], s[t], 0, 0, 0);
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qhi[d], s[t], 0, 0, 0);
+                half8 q[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) q[r] = S.q[r][d][1][at];
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], q[r], s[r][t], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qhi[r][d], s[r][t], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                s[0][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int d = 0; d < STEPS; ++d) {
+                    s[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qlo[0][d], s[0][t], 0, 0, 0);
+                    s[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][d], qhi[0][d], s[0][t], 0, 0, 0);
+                }
             }
         }
         if (kn < own) load_k(next0, next1, nj);
         // lane (n, g): row n, keys j0 + 16 t + 4 g + i
         const bool all = pg0 >= 0 && pg1 >= 0 && j0 + 31 <= pos_min &&
                          (p.window == 0 || j0 > pos_max - p.window || j0 + 32 <= p.sinks);
-        if (!all) {
-            const uint32_t mask = TREE ? w.mask(p, token, j0) : 0;
+        half8 hi[R], lo[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (!all) {
+                const int pos = w.position(token[r]);
+                const int from = max(0, j0 - w.base);
+                const uint32_t nodes = TREE && from < kStreamNodes ? uint32_t(bits[TREE ? r : 0] >> from) : 0u;
+                const uint32_t mask = TREE ? w.mask(p, token[r], depth[TREE ? r : 0], j0, nodes) : 0u;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = j0 + 16 * t + 4 * g + i;
+                        const bool there = (t ? pg1 : pg0) >= 0;
+                        const bool visible = there && (TREE ? ((mask >> (16 * t + 4 * g + i)) & 1u) != 0
+                                                            : paged_visible(pos, j, p.window, p.sinks));
+                        s[r][t][i] = visible ? s[r][t][i] : -__builtin_inff();
+                        seen[r] |= visible;
+                        if (r == 0 && (!there || j >= w.length))
+#pragma unroll
+                            for (auto& x : vf[4 * t + i]) x = 0;
+                    }
+            } else {
+                seen[r] = true;
+            }
+            float top = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                              fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
+            top = max_over_g(top);
+            top = fmaxf(m[r], top);
+            const float safe = top == -__builtin_inff() ? 0.0f : top;
+            if (__any(top > m[r])) {
+                const float alpha = exp2_fast((m[r] - safe) * c[r]);
+                l[r] *= alpha;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[r][i] *= alpha;
+                m[r] = top;
+            }
+            const float shift = 14.0f - safe * c[r];
+            float e[8];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int j = j0 + 16 * t + 4 * g + i;
-                    const bool there = (t ? pg1 : pg0) >= 0;
-                    const bool visible = there && (TREE ? ((mask >> (16 * t + 4 * g + i)) & 1u) != 0
-                                                        : paged_visible(pos, j, p.window, p.sinks));
-                    s[t][i] = visible ? s[t][i] : -__builtin_inff();
-                    seen |= visible;
-                    if (!there || j >= w.length)
-#pragma unroll
-                        for (auto& x : vf[4 * t + i]) x = 0;
+                    e[4 * t + i] = exp2_fast(__builtin_fmaf(s[r][t][i], c[r], shift));
+                    l[r] += e[4 * t + i];
                 }
-        } else {
-            seen = true;
+            split8(e, hi[r], lo[r]);
         }
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = max_over_g(top);
-        top = fmaxf(m, top);
-        const float safe = top == -__builtin_inff() ? 0.0f : top;
-        if (__any(top > m)) {
-            const float alpha = exp2_fast((m - safe) * c);
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] *= alpha;
-            m = top;
-        }
-        const float shift = 14.0f - safe * c;
-        float e[8];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[4 * t + i] = exp2_fast(__builtin_fmaf(s[t][i], c, shift));
-                l += e[4 * t + i];
-            }
-        half8 hi, lo;
-        split8(e, hi, lo);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             // dims VEC n + i: half (i & 1) of word i / 2 of each key
@@ -815,75 +916,83 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
             for (int d = 0; d < 4; ++d)
                 a[d] = __builtin_amdgcn_perm(vf[2 * d + 1][i / 2], vf[2 * d][i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
             const half8 v = __builtin_bit_cast(half8, a);
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, acc[i], 0, 0, 0);
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, acc[i], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[r], acc[r][i], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[r], acc[r][i], 0, 0, 0);
         }
         if (kn < own) load_v(next0, next1, nj);
         pg0 = next0;
         pg1 = next1;
         j0 = nj;
     }
-    l = sum_over_g(l);
-    if (TREE && p.tree.depths[w.first + token] < 0) seen = false;      // (of a tree that is none)
-    // join the four waves: lane (n, g) holds row n, dims VEC (4 g + i) + v
-    const uint64_t any_seen = __ballot(seen);
-    const bool row_seen = ((any_seen | (any_seen >> 16) | (any_seen >> 32) | (any_seen >> 48)) >> n) & 1;
-    if (g == 0) {
-        S.m[wave][n] = m * c;
-        S.l[wave][n] = row_seen ? l : -1.0f;               // (-1: this wave saw nothing of the row)
-        if (wave == 0) S.bad[n] = 0;
-    }
-    if (mine) {
+    // join the four waves, a set of rows at a time: lane (n, g) holds row n, dims VEC (4 g + i) + v
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float* to = &S.o[wave][n][VEC * (4 * g + i)];
-            if constexpr (VEC >= 4) {
+    for (int r = 0; r < R; ++r) {
+        l[r] = sum_over_g(l[r]);
+        if (TREE && depth[TREE ? r : 0] < 0) seen[r] = false;                    // (of a tree that is none)
+        const uint64_t any_seen = __ballot(seen[r]);
+        const bool row_seen = ((any_seen | (any_seen >> 16) | (any_seen >> 32) | (any_seen >> 48)) >> n) & 1;
+        if (r > 0) lds_sync();                                 // (the last set is joined)
+        if (g == 0) {
+            S.m[wave][n] = m[r] * c[r];
+            S.l[wave][n] = row_seen ? l[r] : -1.0f;            // (-1: this wave saw nothing of the row)
+            if (wave == 0) S.bad[16 * r + n] = 0;
+        }
+        if (mine[r]) {
 #pragma unroll
-                for (int v = 0; v < VEC; v += 4)
-                    *reinterpret_cast<float4v*>(to + v) = float4v{acc[v][i], acc[v + 1][i], acc[v + 2][i], acc[v + 3][i]};
+            for (int i = 0; i < 4; ++i) {
+                float* to = &S.o[wave][n][VEC * (4 * g + i)];
+                if constexpr (VEC >= 4) {
+#pragma unroll
+                    for (int v = 0; v < VEC; v += 4)
+                        *reinterpret_cast<float4v*>(to + v) = float4v{acc[r][v][i], acc[r][v + 1][i], acc[r][v + 2][i],
+                                                                      acc[r][v + 3][i]};
+                } else {
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) to[v] = acc[r][v][i];
+                }
+            }
+        }
+        lds_sync();
+        for (int i = threadIdx.x; i < min(rows - 16 * r, 16) * (D / 4); i += kBlock) {
+            const int in = i / (D / 4), d = 4 * (i % (D / 4)), tile_row = 16 * r + in;
+            float sm[4], sl[4];
+            float4v so[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                sm[v] = S.m[v][in];
+                sl[v] = S.l[v][in];
+                so[v] = *reinterpret_cast<const float4v*>(&S.o[v][in][d]);
+            }
+            const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+            float sum = 0.0f;
+            float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+            bool none = true;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float f = sm[v] == -__builtin_inff() ? 0.0f : exp2_fast(sm[v] - top);
+                if (sl[v] != -1.0f) {
+                    none = false;
+                    sum += sl[v] * f;
+                }
+                o += so[v] * f;
+            }
+            const bool bad = !none && (!finite(sum) || sum == 0.0f || !finite(o[0]) || !finite(o[1]) || !finite(o[2]) ||
+                                       !finite(o[3]));
+            if (bad) S.bad[tile_row] = 1;
+            const float f = none ? 0.0f : w.pieces == 1 ? 1.0f / sum : 1.0f / kWeightScale;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = none ? 0.0f : o[k] * f;
+            const int of = row_token(p, tile_row);
+            const size_t row = size_t(w.first + of) * p.b.heads + w.head * G + (tile_row - of * G);
+            if (w.pieces == 1) {
+                *reinterpret_cast<float4v*>(p.out + row * D + d) = o;
             } else {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) to[v] = acc[v][i];
+                const int part = w.part + tile_row;
+                *reinterpret_cast<float4v*>(p.part_o + size_t(part) * D + d) = o;
+                if (d == 0) p.part_ml[part] = none ? make_float2(-__builtin_inff(), 0.0f) : make_float2(top, sum * f);
             }
-        }
-    }
-    lds_sync();
-    for (int i = threadIdx.x; i < rows * (D / 4); i += kBlock) {
-        const int r = i / (D / 4), d = 4 * (i % (D / 4));
-        float sm[4], sl[4];
-        float4v so[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            sm[v] = S.m[v][r];
-            sl[v] = S.l[v][r];
-            so[v] = *reinterpret_cast<const float4v*>(&S.o[v][r][d]);
-        }
-        const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-        float sum = 0.0f;
-        float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-        bool none = true;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const float f = sm[v] == -__builtin_inff() ? 0.0f : exp2_fast(sm[v] - top);
-            if (sl[v] != -1.0f) {
-                none = false;
-                sum += sl[v] * f;
-            }
-            o += so[v] * f;
-        }
-        const bool bad = !none && (!finite(sum) || sum == 0.0f || !finite(o[0]) || !finite(o[1]) || !finite(o[2]) ||
-                                   !finite(o[3]));
-        if (bad) S.bad[r] = 1;
-        const float f = none ? 0.0f : w.pieces == 1 ? 1.0f / sum : 1.0f / kWeightScale;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = none ? 0.0f : o[k] * f;
-        const int of = row_token(p, r);
-        const size_t row = size_t(w.first + of) * p.b.heads + w.head * G + (r - of * G);
-        if (w.pieces == 1) {
-            *reinterpret_cast<float4v*>(p.out + row * D + d) = o;
-        } else {
-            *reinterpret_cast<float4v*>(p.part_o + size_t(w.part + r) * D + d) = o;
-            if (d == 0) p.part_ml[w.part + r] = none ? make_float2(-__builtin_inff(), 0.0f) : make_float2(top, sum * f);
         }
     }
     wait_all_memory();                         // (a row done again is stored again, by another wave)
@@ -935,8 +1044,8 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const int token = mine ? row_token(p, r) : 0;
     const size_t out_row = size_t(w.first + token) * p.b.heads + w.head * G + (mine ? r - token * G : 0);
     half8 qhi[STEPS], qlo[STEPS];
-    float c;
-    {
+    float c = 0.0f;
+    auto split_query = [&] {
         const float* q = p.query + out_row * D;
         float top = 0.0f;
         float x[STEPS][8];
@@ -961,7 +1070,9 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             split8(x[s], qhi[s], qlo[s]);
         }
         c = __builtin_ldexpf(kLog2e / __builtin_sqrtf(float(D)), e);
-    }
+    };
+    if constexpr (!TREE) split_query();
+    const int depth = TREE ? p.tree.depths[w.first + token] : 0;
     const bool active = 32 * wave < rows;      // (wave-uniform)
     const int pos_min = TREE ? w.base - 1 : uniform(w.position(row_token(p, min(32 * wave, rows - 1))));
     const int pos_max = uniform(w.position(row_token(p, min(32 * wave + 31, rows - 1))));
@@ -1134,7 +1245,8 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             const int x = int(opaque(lane)), g = x >> 5;
             const int row = 32 * wave + (x & 31);
             if constexpr (TREE) {
-                const uint32_t mask = w.mask(p, row < rows ? row_token(p, row) : 0, j0) >> (4 * g);
+                const int i = row < rows ? row_token(p, row) : 0;
+                const uint32_t mask = w.mask(p, i, depth, j0, w.bits(p, i, j0)) >> (4 * g);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const bool visible = ((both >> (i >> 3)) & 1u) & ((mask >> (8 * (i >> 2) + (i & 3))) & 1u);
@@ -1190,6 +1302,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         copy_v(page, at, c0);
         page = __builtin_amdgcn_readlane(pg, 4 + wave);
         if (c0 + 1 < c1) copy_k(page, at_next, c0 + 1);
+        if constexpr (TREE) split_query();     // (beside the first copies: pieces are short)
         wait_all_memory();
         lds_sync();
         // copies of chunk cc + 1's V, and (once K of cc is read) of cc + 2's K
@@ -1252,7 +1365,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             if (32 * dt + 8 * (i >> 2) < D) zero[i & 3] = __builtin_fmaf(acc[dt][i], 0.0f, zero[i & 3]);
     const uint64_t was_seen = __ballot(seen);
     bool none = (((was_seen | (was_seen >> 32)) >> n_end) & 1) == 0;
-    if (TREE) none |= p.tree.depths[w.first + token_end] < 0;          // (of a tree that is none)
+    if (TREE) none |= depth < 0;               // (of a tree that is none)
     // (a row that sees nothing has zeros, unless its tile holds something not finite)
     const bool ok = (zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f && (none || (finite(l) && l != 0.0f));
     const uint64_t wrong = __ballot(mine_end && !ok);
@@ -1281,14 +1394,14 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         redo_row<D, TREE>(p, w, span, c0, c1, 32 * wave + __builtin_ctz(left));
 }
 
-template <int D, bool LARGE>
+template <int D, bool LARGE, bool TREE>
 struct AttnShared {
-    SmallShared<D> small;
+    SmallShared<D, TREE> small;
 };
-template <int D>
-struct AttnShared<D, true> {
+template <int D, bool TREE>
+struct AttnShared<D, true, TREE> {
     union {
-        SmallShared<D> small;
+        SmallShared<D, TREE> small;
         LargeShared<D> large;
     };
 };
@@ -1296,7 +1409,7 @@ struct AttnShared<D, true> {
 template <int D, bool LARGE, bool TREE>
 __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnParams p)
 {
-    __shared__ AttnShared<D, LARGE> S;
+    __shared__ AttnShared<D, LARGE, TREE> S;
     Piece w;
     if (!plan_piece<TREE>(p, blockIdx.x, w)) return;
     // the join's directory: which rows have parts, and where
@@ -1314,8 +1427,14 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention_kernel(PagedAttnPar
         c0 = each * w.split + min(w.split, more);
         c1 = c0 + each + (w.split < more ? 1 : 0);
     }
-    if (w.small) small_tile<D, TREE>(p, w, span, c0, c1, S.small);
-    else if constexpr (LARGE) large_tile<D, TREE>(p, w, span, c0, c1, S.large);
+    if constexpr (TREE) {
+        if (w.small && w.n * p.b.groups <= kSmallRows) small_tile<D, true, 1>(p, w, span, c0, c1, S.small);
+        else if (w.small) small_tile<D, true, 2>(p, w, span, c0, c1, S.small);
+        else if constexpr (LARGE) large_tile<D, true>(p, w, span, c0, c1, S.large);
+    } else {
+        if (w.small) small_tile<D, false, 1>(p, w, span, c0, c1, S.small);
+        else if constexpr (LARGE) large_tile<D, false>(p, w, span, c0, c1, S.large);
+    }
 }
 
 // The join's threads are sets of groups * D / 4, one thread for four values of
@@ -1345,8 +1464,8 @@ static_assert(join_has_one_writer());
 // latency where the parts are few (32 chats: 4.9 us) and by the L2 and HBM
 // where they are many (501 tokens of 32 heads in 4 parts, 34 MB: 12 us).
 // Blocks of 512 threads take 5 us longer for the latter.
-template <int D>
-static __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParams p)
+template <int D, bool TREE>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParams p)
 {
     __shared__ float4v so[kJoinThreads];
     __shared__ float sl[kJoinThreads], sm[kJoinThreads];
@@ -1363,7 +1482,7 @@ static __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAt
         const int b = paged_sequence(p.b, t, &first, &count);
         if (cut == 0) return;
         if (b < 0) continue;
-        const int pieces = d.x >> 1, stride = (d.x & 1) ? kSmallRows : kTileRows;
+        const int pieces = d.x >> 1, stride = (d.x & 1) ? kStreamRows<TREE> : kTileRows;
         if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) continue;
         float m = -__builtin_inff(), l = 0.0f;
         float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1424,11 +1543,12 @@ struct AttnLayout {
 // Rows of partial results: pieces are of T >= work / kTarget chunks, and a
 // sequence of S > 1 pieces a tile has at least 1.5 T chunks a tile, so S <=
 // chunks / T + 1/2 < 2 chunks / T, and over all of them fewer than 2 kTarget.
-inline AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large)
+template <bool TREE>
+AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large)
 {
     AttnLayout L;
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
-    L.part_rows = 2 * kTarget * (large ? kTileRows : kSmallRows);
+    L.part_rows = 2 * kTarget * (large ? kTileRows : kStreamRows<TREE>);
     L.first = 256;                             // (the plan's, of sequences with rows)
     L.item = L.first + up((size_t(tokens) + 1) * sizeof(int32_t));
     L.desc = L.item + up(size_t(tokens) * sizeof(int4));
@@ -1438,8 +1558,12 @@ inline AttnLayout attn_layout(int tokens, int kv_heads, int head_dim, bool large
     return L;
 }
 
-// Whether a batch may hold a tile of more than 16 rows.
-inline bool attn_large(int tokens, int groups, bool single) { return !single && int64_t(tokens) * groups > kSmallRows; }
+// Whether a batch may hold a tile of more rows than stream to registers.
+template <bool TREE>
+bool attn_large(int tokens, int groups, bool single)
+{
+    return !single && int64_t(tokens) * groups > kStreamRows<TREE>;
+}
 
 template <int D, bool TREE>
 void launch_attention(const PagedAttnParams& p, bool large, int64_t blocks, hipStream_t s)
@@ -1448,7 +1572,7 @@ void launch_attention(const PagedAttnParams& p, bool large, int64_t blocks, hipS
     if (large) hipLaunchKernelGGL((paged_attention_kernel<D, true, TREE>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     else hipLaunchKernelGGL((paged_attention_kernel<D, false, TREE>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     if (!p.whole)
-        hipLaunchKernelGGL(paged_join_kernel<D>, dim3(unsigned(std::min<int64_t>(kJoinBlocks, int64_t(p.b.tokens) * p.b.kv_heads))), dim3(kJoinThreads), 0, s, p);
+        hipLaunchKernelGGL((paged_join_kernel<D, TREE>), dim3(unsigned(std::min<int64_t>(kJoinBlocks, int64_t(p.b.tokens) * p.b.kv_heads))), dim3(kJoinThreads), 0, s, p);
 }
 
 // The launches of a checked call (its batch is p.b already).
@@ -1464,8 +1588,8 @@ int run_attention(PagedAttnParams& p, const hq_pages* cache, const float* query,
     p.sinks = sinks;
     p.tile_tokens = kTileRows / p.b.groups;
     p.by_group = 65536 / p.b.groups + 1;
-    const bool large = attn_large(tokens, p.b.groups, starts == nullptr);
-    const AttnLayout L = attn_layout(tokens, p.b.kv_heads, cache->head_dim, large);
+    const bool large = attn_large<TREE>(tokens, p.b.groups, starts == nullptr);
+    const AttnLayout L = attn_layout<TREE>(tokens, p.b.kv_heads, cache->head_dim, large);
     char* ws = static_cast<char*>(workspace);
     p.part_rows = L.part_rows;
     p.cut = reinterpret_cast<int32_t*>(ws);
@@ -1477,12 +1601,17 @@ int run_attention(PagedAttnParams& p, const hq_pages* cache, const float* query,
     p.part_o = reinterpret_cast<float*>(ws + L.o);
     // chunks / T + 1 pieces a tile and kv head at most, so `target` and one of each in all; nor more than the
     // table's width allows.  A block without a piece ends at once.
-    const int64_t tiles = large ? int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences)
-                                : std::min(tokens, p.b.sequences);
+    const int64_t narrow = int64_t(tokens) / std::max(1, kSmallRows / p.b.groups) + std::min(tokens, p.b.sequences);
+    p.narrow = TREE && narrow * p.b.kv_heads <= kTarget / 2;
+    const int64_t tiles = p.narrow ? narrow
+                          : large  ? int64_t(tokens) / p.tile_tokens + (tokens < p.b.sequences ? tokens : p.b.sequences)
+                                   : std::min(tokens, p.b.sequences);
     const int64_t widest = (int64_t(cache->max_pages) * cache->page_size + kChunkKeys - 1) / kChunkKeys;
     p.whole = widest <= kWholeChunks;
+    // (of a tree's batch whose tiles all have a place, their pieces have one too: see plan_piece)
+    const bool placed = TREE && cache->sequences <= kWave && tiles * p.b.kv_heads <= kTarget;
     const int64_t blocks = p.whole ? tiles * p.b.kv_heads
-                                   : std::min(kTarget + tiles * p.b.kv_heads,
+                                   : std::min(kTarget + (placed ? 0 : tiles * p.b.kv_heads),
                                               tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
     p.planned = cache->sequences >= kPlanSequences && !(p.whole && !starts);
     if (blocks > kMaxBlocks || int64_t(tokens) * p.b.kv_heads > 0x7fffffff) return HQ_ERR_ARG;

@@ -6,7 +6,7 @@ using namespace hq;
 extern "C" size_t hq_paged_attention_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim, int single)
 {
     if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1) return 0;
-    return attn_layout(tokens, kv_heads, head_dim, attn_large(tokens, heads / kv_heads, single != 0)).total;
+    return attn_layout<false>(tokens, kv_heads, head_dim, attn_large<false>(tokens, heads / kv_heads, single != 0)).total;
 }
 
 extern "C" int hq_paged_attention(const hq_pages* cache, const float* query, const int32_t* starts, int tokens,

@@ -8,7 +8,7 @@ using namespace hq;
 extern "C" size_t hq_paged_attention_tree_workspace_bytes(int tokens, int heads, int kv_heads, int head_dim)
 {
     if (tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1) return 0;
-    return attn_layout(tokens, kv_heads, head_dim, attn_large(tokens, heads / kv_heads, false)).total;
+    return attn_layout<true>(tokens, kv_heads, head_dim, attn_large<true>(tokens, heads / kv_heads, false)).total;
 }
 
 extern "C" int hq_paged_attention_tree(const hq_pages* cache, const float* query, const hq_tree* tree, int heads,
