@@ -85,9 +85,10 @@ constexpr int kSmallMin = 2;           // fewest chunks of a small piece: a step
 constexpr int kLargeMin = 4;           // of a large one (100 tokens after 1024: 22.7 us, 23.6 with 2, 22.6 with 3)
 // A chunk of a large tile counts as two of a small one: a step of 24 chats and
 // a prompt's 250 tokens takes 75 us so, 82 with 1, 79 with 3 (over data that
-// the last-level cache does not hold; where it does 67, 75, 72).
+// the last-level cache does not hold; where it does 67, 75, 72).  Of trees it
+// counts as one: a batch of them waits for memory with either tile (32 chats of
+// 16 nodes 102 us, 113 with 2 for large tiles; of 32 nodes 122, 125).
 constexpr int kLargeCost = 2;
-constexpr int kTreeCost = 2, kTreeCostHalf = 2, kTreeCostLarge = 3;
 // Where there is a tile for every CU, large ones of so few chunks stay whole:
 // a second block on the CU gains less than the join of the parts costs (4 x
 // 256 tokens at 512: 34 us, 43 in two pieces each; at 1024 51, 59; 1000 tokens
@@ -291,14 +292,12 @@ __device__ __forceinline__ SequencePlan sequence_plan(const PagedAttnParams& p, 
         s.tile_tokens = s.small ? max(1, s.n) : p.tile_tokens;
         s.tiles = s.small ? min(s.n, 1) : quotient(s.n + s.tile_tokens - 1, s.tile_tokens);
     }
-    if (TREE) s.cost = s.small ? kTreeCost : s.n * p.b.groups <= kTileRows / 2 ? kTreeCostHalf : kTreeCostLarge;
-    else s.cost = s.small ? 1 : kLargeCost;
+    s.cost = s.small || TREE ? 1 : kLargeCost;
     const int origin = s.length - s.n;
     // (a tree's nodes may all be roots: their positions are at or past the base)
     s.chunks = s.n ? span_of(p, TREE ? origin : origin + (s.tiles - 1) * s.tile_tokens, s.length - 1).count : 0;
     if (TREE && p.narrow && s.chunks <= kWholeChunks && s.n > kSmallRows / p.b.groups && s.n <= kStreamNodes) {
         s.small = true;
-        s.cost = kTreeCost;
         s.tile_tokens = kSmallRows / p.b.groups;
         s.tiles = quotient(s.n + s.tile_tokens - 1, s.tile_tokens);
     }
@@ -348,7 +347,7 @@ __device__ __forceinline__ int cuts_of(const PagedAttnParams& p, const SequenceP
 {
     if (p.whole || (s.small && s.tiles > 1)) return 1;
     if (!s.small && s.chunks <= kLargeWhole && int64_t(tiles) * p.b.kv_heads >= kTarget / 2) return 1;
-    const int size = max(target, s.small ? kSmallMin * (TREE ? kTreeCost : 1) : kLargeMin * s.cost);
+    const int size = max(target, s.small ? kSmallMin : kLargeMin * s.cost);
     return max(1, int(float(s.chunks * s.cost) / float(size) + 0.5f));
 }
 
@@ -1534,6 +1533,64 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
     }
 }
 
+// The join of a tree's batch of many rows (a token's heads of one kv head), whose
+// parts are few: quads of a multiple of 64 threads, so that a wave has one row,
+// as many rows a block as fit, and no exchange between threads.  382 tokens of
+// 32 heads in 2 parts: 6.4 us, 9.1 by paged_join_kernel; 96 in 16 parts 10.3
+// and 9.1: where rows are few, their parts are many.
+constexpr int kJoinRows = 1024;
+
+template <int D>
+__global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(PagedAttnParams p)
+{
+    const int cut = *p.cut;
+    const int quads = p.b.groups * D / 4;                 // 64, 128 or 256
+    const int slots = kJoinThreads / quads;
+    const int slot = uniform(threadIdx.x / unsigned(quads)), quad = threadIdx.x - slot * quads;
+    const int r = quad / (D / 4), at = quad % (D / 4);
+    const unsigned all = unsigned(p.b.tokens) * unsigned(p.b.kv_heads);
+    for (unsigned i = blockIdx.x * slots + slot; i < all; i += gridDim.x * slots) {
+        const int t = int(i / unsigned(p.b.kv_heads)), h = int(i - unsigned(t) * unsigned(p.b.kv_heads));
+        const int2 d = p.desc[i];                         // (of any contents where the row is nobody's)
+        int first = 0, count = 0;
+        const int b = paged_sequence(p.b, t, &first, &count);
+        if (cut == 0) return;
+        if (b < 0) continue;
+        const int pieces = d.x >> 1, stride = (d.x & 1) ? kStreamRows<true> : kTileRows;
+        if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) continue;
+        float m = -__builtin_inff(), l = 0.0f, lost = 0.0f;
+        float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = 0; i0 < pieces; i0 += 4) {
+            float2 ml[4];
+            float4v x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const size_t row = size_t(d.y) + size_t(min(i0 + k, pieces - 1)) * stride + r;
+                ml[k] = p.part_ml[row];
+                x[k] = reinterpret_cast<const float4v*>(p.part_o + row * D)[at];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i0 + k >= pieces) continue;
+                if (ml[k].x == -__builtin_inff()) {
+                    lost += ml[k].y;
+                    continue;
+                }
+                const float top = fmaxf(m, ml[k].x);
+                const float a = exp2_fast(m - top), b = exp2_fast(ml[k].x - top);
+                l = l * a + ml[k].y * b;
+                o = o * a + x[k] * b;
+                m = top;
+            }
+        }
+        const float f = 1.0f / l;
+        float4v y = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+        if (m == -__builtin_inff()) y = float4v{lost, lost, lost, lost};   // nothing seen: 0; only scores of -inf: NaN
+        const size_t row = size_t(t) * p.b.heads + h * p.b.groups + r;
+        reinterpret_cast<float4v*>(p.out + row * D)[at] = y;
+    }
+}
+
 // -------------------------------------------------------------------- host
 struct AttnLayout {
     size_t first, item, desc, ml, o, total;
@@ -1571,8 +1628,19 @@ void launch_attention(const PagedAttnParams& p, bool large, int64_t blocks, hipS
     if (p.planned) hipLaunchKernelGGL(paged_plan_kernel<TREE>, dim3(1), dim3(kPlanThreads), 0, s, p);
     if (large) hipLaunchKernelGGL((paged_attention_kernel<D, true, TREE>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
     else hipLaunchKernelGGL((paged_attention_kernel<D, false, TREE>), dim3(unsigned(blocks)), dim3(kBlock), 0, s, p);
-    if (!p.whole)
-        hipLaunchKernelGGL((paged_join_kernel<D, TREE>), dim3(unsigned(std::min<int64_t>(kJoinBlocks, int64_t(p.b.tokens) * p.b.kv_heads))), dim3(kJoinThreads), 0, s, p);
+    if (p.whole) return;
+    const int64_t rows = int64_t(p.b.tokens) * p.b.kv_heads;
+    if constexpr (TREE) {
+        const int quads = p.b.groups * D / 4;
+        if (quads % kWave == 0 && rows >= kJoinRows) {
+            const int64_t blocks = (rows * quads + kJoinThreads - 1) / kJoinThreads;
+            hipLaunchKernelGGL(tree_join_kernel<D>, dim3(unsigned(std::min<int64_t>(kJoinBlocks, blocks))),
+                               dim3(kJoinThreads), 0, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((paged_join_kernel<D, TREE>), dim3(unsigned(std::min<int64_t>(kJoinBlocks, rows))),
+                       dim3(kJoinThreads), 0, s, p);
 }
 
 // The launches of a checked call (its batch is p.b already).

@@ -692,33 +692,45 @@ def add_rmsnorm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float, delta: t
     rows, n = shape
     if n == 0 or n > 1 << 30 or rows >= 1 << 24:
         raise ValueError("x must be [rows, n] with n from 1 to 2^30 and fewer than 2^24 rows")
-    if gamma is None:
-        raise ValueError("gamma is needed")
-    for t, name, dims, dtype in ((gamma, "gamma", (n,), torch.float32), (delta, "delta", shape, torch.float32),
-                                 (out, "out", shape, torch.float32), (q, "q", shape, torch.int8),
-                                 (act_scales, "act_scales", (rows,), torch.float32)):
-        if t is not None and (t.shape != dims or t.dtype is not dtype or t.get_device() != index or
-                              not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor {list(dims)} on x's device")
-    if out is not None or q is not None or act_scales is not None:
-        _apart((out, q, act_scales), (x, gamma, delta), (out, x))
-    if delta is None:
-        out_ptr = None if out is None else out.data_ptr()
-        delta_ptr = None
-    else:
+    f32 = torch.float32
+    if gamma is None or gamma.shape != (n,) or gamma.dtype is not f32 or gamma.get_device() != index or not gamma.is_contiguous():
+        raise ValueError("gamma must be a contiguous float32 tensor [n] on x's device")
+    size = 4 * rows * n
+    x_ptr, inputs = x.data_ptr(), [(gamma.data_ptr(), 4 * n)]
+    outputs = []                               # given ones: apart from the inputs and each other
+    delta_ptr = out_ptr = None
+    if delta is not None:
+        if delta.shape != shape or delta.dtype is not f32 or delta.get_device() != index or not delta.is_contiguous():
+            raise ValueError("delta must be a contiguous float32 tensor like x on its device")
         delta_ptr = delta.data_ptr()
+        inputs.append((delta_ptr, size))
         if out is None:
-            if abs(delta_ptr - x.data_ptr()) < 4 * rows * n:
-                raise ValueError("x takes the sum: delta must not overlap it")
             out = x
+    if out is not None:
+        if out.shape != shape or out.dtype is not f32 or out.get_device() != index or not out.is_contiguous():
+            raise ValueError("out must be a contiguous float32 tensor like x on its device")
         out_ptr = out.data_ptr()
+        outputs.append((out_ptr, size))
+    if out_ptr != x_ptr:                       # (x itself may take the sum)
+        inputs.append((x_ptr, size))
     if q is None:
         q = torch.empty(shape, dtype=torch.int8, device=x.device)
+    else:
+        if q.shape != shape or q.dtype is not torch.int8 or q.get_device() != index or not q.is_contiguous():
+            raise ValueError("q must be a contiguous int8 tensor like x on its device")
+        outputs.append((q.data_ptr(), size // 4))
     if act_scales is None:
-        act_scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+        act_scales = torch.empty(rows, dtype=f32, device=x.device)
+    else:
+        if (act_scales.shape != (rows,) or act_scales.dtype is not f32 or act_scales.get_device() != index or
+                not act_scales.is_contiguous()):
+            raise ValueError("act_scales must be a contiguous float32 tensor [rows] on x's device")
+        outputs.append((act_scales.data_ptr(), 4 * rows))
+    if outputs and rows:
+        _apart(outputs, inputs)
     if rows:
         _launch(_native.lib().hq_add_rmsnorm_quant,
-                (x.data_ptr(), delta_ptr, gamma.data_ptr(), out_ptr, q.data_ptr(), act_scales.data_ptr(), rows, n, eps),
+                (x_ptr, delta_ptr, gamma.data_ptr(), out_ptr, q.data_ptr(), act_scales.data_ptr(), rows, n, eps),
                 None, index, stream, (x, gamma, delta, out, q, act_scales), "hq_add_rmsnorm_quant")
     return q, act_scales
 

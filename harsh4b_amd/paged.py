@@ -168,19 +168,23 @@ def _launch(entry, args: tuple, nbytes: int | None, index: int, stream, tensors,
         check(status, what)
 
 
-def _apart(outputs: tuple, inputs: tuple, same: tuple = ()) -> None:
-    """Refuse outputs that overlap each other or an input (None: not given).
-    same: an output and the input that it may be, whole and in place."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), t) for t in (*outputs, *inputs)
-             if t is not None]
-    made = sum(t is not None for t in outputs)
-    for i in range(made):
-        low, high, t = spans[i]
-        for other_low, other_high, other in spans[i + 1:]:
-            if other_low < high and low < other_high:
-                if same and t is same[0] and other is same[1] and (low, high) == (other_low, other_high):
-                    continue
-                raise ValueError("outputs must not overlap each other or an input")
+def _span(t) -> tuple[int, int]:
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _apart(outputs, inputs) -> None:
+    """Refuse outputs that overlap each other or an input: (address, bytes) each."""
+    for i, (at, size) in enumerate(outputs):
+        for other, length in inputs:
+            if -length < other - at < size:
+                break
+        else:
+            for other, length in outputs[:i]:
+                if -length < other - at < size:
+                    break
+            else:
+                continue
+        raise ValueError("outputs must not overlap each other or an input")
 
 
 # --------------------------------------------------------------------------- append, attention

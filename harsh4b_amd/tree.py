@@ -28,7 +28,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
-from .paged import MAX_GROUPS, _F32, _I32, _apart, _cache, _index, _launch, _refuse, _starts
+from .paged import MAX_GROUPS, _F32, _I32, _apart, _cache, _index, _launch, _refuse, _span, _starts
 
 MAX_NODES = _native.HQ_TREE_NODES
 ANCESTOR_WORDS = MAX_NODES // 32
@@ -79,6 +79,7 @@ def tree_plan(parents: torch.Tensor, starts: torch.Tensor, status: torch.Tensor,
         raise ValueError("starts must be a contiguous int32 device tensor [sequences + 1]")
     if status is None or status.numel() != 1 or status.dtype is not _I32 or status.get_device() != index:
         _refuse("status", status, _I32, index, "[1]")
+    given = depths is not None or ancestors is not None
     if depths is None:
         depths = torch.empty_like(parents)
     if ancestors is None:
@@ -86,7 +87,9 @@ def tree_plan(parents: torch.Tensor, starts: torch.Tensor, status: torch.Tensor,
     tree = DraftTree(parents, starts, depths, ancestors)
     sequences = starts.shape[0] - 1
     packed = _tree(tree, tokens, sequences, index)
-    _apart((depths, ancestors, status), (parents, starts))
+    if given:
+        _apart(((depths.data_ptr(), 4 * tokens), (ancestors.data_ptr(), 4 * ANCESTOR_WORDS * tokens)),
+               ((parents.data_ptr(), 4 * tokens), (starts.data_ptr(), 4 * sequences + 4), (status.data_ptr(), 4)))
     if tokens:
         _launch(_native.lib().hq_tree_plan, (packed, sequences, status.data_ptr()), None, index, stream,
                 (*tree, status), "hq_tree_plan")
@@ -111,13 +114,18 @@ def paged_append_tree(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Ten
     heads = width // d - 2 * kv
     if width % d or heads < 1 or heads % kv or heads // kv > MAX_GROUPS:
         raise ValueError("qkv must be [tokens, (heads + 2 kv_heads) * head_dim] with 1 to 8 heads a kv head")
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t.shape != (d,) or t.dtype is not _F32 or t.get_device() != index or not t.is_contiguous():
-            _refuse(name, t, _F32, index, "[head_dim]")
+    if (q_norm.shape != (d,) or q_norm.dtype is not _F32 or q_norm.get_device() != index or
+            not q_norm.is_contiguous()):
+        _refuse("q_norm", q_norm, _F32, index, "[head_dim]")
+    if (k_norm.shape != (d,) or k_norm.dtype is not _F32 or k_norm.get_device() != index or
+            not k_norm.is_contiguous()):
+        _refuse("k_norm", k_norm, _F32, index, "[head_dim]")
     shape = rope_cos.shape
-    for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        if t.shape != shape or t.dtype is not _F32 or t.get_device() != index or not t.is_contiguous():
-            _refuse(name, t, _F32, index, "[positions, head_dim / 2]")
+    if rope_cos.dtype is not _F32 or rope_cos.get_device() != index or not rope_cos.is_contiguous():
+        _refuse("rope_cos", rope_cos, _F32, index, "[positions, head_dim / 2]")
+    if (rope_sin.shape != shape or rope_sin.dtype is not _F32 or rope_sin.get_device() != index or
+            not rope_sin.is_contiguous()):
+        _refuse("rope_sin", rope_sin, _F32, index, "[positions, head_dim / 2]")
     if len(shape) != 2 or 2 * shape[1] != d or shape[0] < 1:
         raise ValueError("rope_cos and rope_sin must be [positions, head_dim / 2]")
     packed = _tree(tree, tokens, sequences, index)
@@ -219,15 +227,15 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
     else:
         chosen, rows = _nodes(choices, "choices", tokens, index), None
     if out is None:
-        kept, after = (torch.empty(sequences, dtype=_I32, device=table.device) for _ in range(2))
-        path = torch.empty(tokens, dtype=_I32, device=table.device)
+        kept, path, after = torch.empty_like(lengths), torch.empty_like(drafted), torch.empty_like(lengths)
     else:
         kept, path, after = out
         _nodes(path, "path", tokens, index)
         for t, name in ((kept, "kept"), (after, "next")):
             if t.shape != (sequences,) or t.dtype is not _I32 or t.get_device() != index or not t.is_contiguous():
                 _refuse(name, t, _I32, index, "[sequences]")
-        _apart((kept, path, after), (keys, values, table, lengths, status, *tree, drafted, choices, logits))
+        _apart([_span(t) for t in (kept, path, after)],
+               [_span(t) for t in (keys, values, table, lengths, status, *tree, drafted, choices, logits) if t is not None])
     if tokens == 0:
         vocab, rows = 0, None                  # (nothing is read)
     _launch(_native.lib().hq_pages_accept,
