@@ -45,8 +45,8 @@ __global__ __launch_bounds__(kBlock) void norm_quant_long_kernel(NormParams p)
 // Up to 256 NPT values a row: a block a row, held in registers, thread t its
 // values t, t + 256, .. (partial t of the spec's sum), so that every array is
 // read or written once and all of a row's loads are on their way together.
-// Bound by HBM for many rows of 2560 (2048: 68 MB in 16.9 us, 4.0 TB/s; 8192:
-// 48 us, 5.7 TB/s) and by latency for few (8 rows: 4.3 us, a launch, a round
+// Bound by HBM for many rows of 2560 (2048: 68 MB in 16.1 us, 4.2 TB/s; 8192:
+// 48 us, 5.7 TB/s) and by latency for few (8 rows: 3.8 us, a launch, a round
 // trip and three reductions).  A wave a row with its values in fours, whose
 // loads and stores are wider and need no barrier, takes longer at every size (8
 // rows 5.6 us, 2048 18.5, 8192 58): a wave then has the divisions of a whole row
@@ -57,38 +57,49 @@ __global__ __launch_bounds__(kBlock) void norm_quant_kernel(NormParams p)
     __shared__ float red[kBlock];
     const int t = threadIdx.x, n = p.n;
     const size_t at = size_t(blockIdx.x) * n;
+    // (a row as a buffer: what lies past it reads as zero, which changes neither sum nor maximum, and is not written)
+    const auto x = raw_rsrc(p.x + at, 4 * n), gamma = raw_rsrc(p.gamma, 4 * n);
+    auto load = [&](__amdgpu_buffer_rsrc_t from, int k) {
+        return bits_f32(__builtin_amdgcn_raw_buffer_load_b32(from, 4 * (t + kBlock * k), 0, 0));
+    };
     float v[NPT], gam[NPT];
 #pragma unroll
-    for (int k = 0; k < NPT; ++k) {
-        const int i = min(t + kBlock * k, n - 1);
-        v[k] = p.x[at + i];
-        gam[k] = p.gamma[i];
-    }
+    for (int k = 0; k < NPT; ++k) v[k] = load(x, k);
     if (p.delta) {
+        const auto delta = raw_rsrc(p.delta + at, 4 * n);
         float d[NPT];
 #pragma unroll
-        for (int k = 0; k < NPT; ++k) d[k] = p.delta[at + min(t + kBlock * k, n - 1)];
+        for (int k = 0; k < NPT; ++k) d[k] = load(delta, k);
+#pragma unroll
+        for (int k = 0; k < NPT; ++k) gam[k] = load(gamma, k);
 #pragma unroll
         for (int k = 0; k < NPT; ++k) v[k] = v[k] + d[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < NPT; ++k) gam[k] = load(gamma, k);
     }
     float ss = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NPT; ++k)
-        if (t + kBlock * k < n) ss = __builtin_fmaf(v[k], v[k], ss);
+    for (int k = 0; k < NPT; ++k) ss = __builtin_fmaf(v[k], v[k], ss);
     const float total = block_tree_sum256(ss, red);
+    if (p.sum) {
+        const auto sum = raw_rsrc(p.sum + at, 4 * n);
+#pragma unroll
+        for (int k = 0; k < NPT; ++k) __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[k]), sum, 4 * (t + kBlock * k), 0, 0);
+    }
     const float r = __builtin_sqrtf(total / float(n) + p.eps);
     float amax = 0.0f;
 #pragma unroll
     for (int k = 0; k < NPT; ++k) {
-        if (p.sum && t + kBlock * k < n) p.sum[at + t + kBlock * k] = v[k];
         v[k] = (v[k] / r) * gam[k];
-        amax = fmaxf(amax, fabsf(v[k]));               // (past n: the last value again)
+        amax = fmaxf(amax, fabsf(v[k]));               // (past n: 0, or a NaN, which does not count)
     }
     amax = fmaxf(block_max_nonneg(amax, red), 1e-5f);
     const float inv = 127.0f / amax;
+    const auto q = raw_rsrc(p.q + at, n);
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
-        if (t + kBlock * k < n) p.q[at + t + kBlock * k] = quant_i8(v[k], inv);
+        __builtin_amdgcn_raw_buffer_store_b8(uint8_t(quant_i8(v[k], inv)), q, t + kBlock * k, 0, 0);
     if (t == 0) p.act[blockIdx.x] = amax / 127.0f;
 }
 

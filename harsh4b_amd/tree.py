@@ -210,7 +210,9 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
         raise ValueError("pages_accept needs the cache's lengths and status")
     index = _index(table)
     cache, sequences, _, _ = _cache(index, keys, values, table, lengths, None, status, 5)
-    tokens = drafted.shape[0] if isinstance(drafted, torch.Tensor) and drafted.dim() == 1 else -1
+    if not isinstance(drafted, torch.Tensor) or drafted.dim() != 1:
+        _refuse("drafted", drafted, _I32, index, "[tokens]")
+    tokens = drafted.shape[0]
     ids = _nodes(drafted, "drafted", tokens, index)
     packed = _tree(tree, tokens, sequences, index)
     if (choices is None) == (logits is None):
