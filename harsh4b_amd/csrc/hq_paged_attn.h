@@ -1245,7 +1245,8 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
             const int row = 32 * wave + (x & 31);
             if constexpr (TREE) {
                 const int i = row < rows ? row_token(p, row) : 0;
-                const uint32_t mask = w.mask(p, i, depth, j0, w.bits(p, i, j0)) >> (4 * g);
+                const uint32_t nodes = j0 + 32 > w.base ? w.bits(p, i, j0) : 0u;
+                const uint32_t mask = w.mask(p, i, depth, j0, nodes) >> (4 * g);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const bool visible = ((both >> (i >> 3)) & 1u) & ((mask >> (8 * (i >> 2) + (i & 3))) & 1u);
@@ -1538,7 +1539,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 // as many rows a block as fit, and no exchange between threads.  382 tokens of
 // 32 heads in 2 parts: 6.4 us, 9.1 by paged_join_kernel; 96 in 16 parts 10.3
 // and 9.1: where rows are few, their parts are many.
-constexpr int kJoinRows = 1024;
+constexpr int kJoinRows = 2048;
 
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(PagedAttnParams p)
@@ -1560,18 +1561,20 @@ __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(PagedAttnParams
         if (pieces < 2 || d.y < 0 || int64_t(d.y) + int64_t(pieces - 1) * stride + p.b.groups > p.part_rows) continue;
         float m = -__builtin_inff(), l = 0.0f, lost = 0.0f;
         float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i0 = 0; i0 < pieces; i0 += 4) {
-            float2 ml[4];
-            float4v x[4];
+        constexpr int AHEAD = 4;
+        for (int i0 = 0; i0 < pieces; i0 += AHEAD) {
+            float2 ml[AHEAD];
+            float4v x[AHEAD];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const size_t row = size_t(d.y) + size_t(min(i0 + k, pieces - 1)) * stride + r;
+            for (int k = 0; k < AHEAD; ++k) {
+                if (i0 + k >= pieces) break;
+                const size_t row = size_t(d.y) + size_t(i0 + k) * stride + r;
                 ml[k] = p.part_ml[row];
                 x[k] = reinterpret_cast<const float4v*>(p.part_o + row * D)[at];
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (i0 + k >= pieces) continue;
+            for (int k = 0; k < AHEAD; ++k) {
+                if (i0 + k >= pieces) break;
                 if (ml[k].x == -__builtin_inff()) {
                     lost += ml[k].y;
                     continue;

@@ -1155,3 +1155,204 @@ def test_calls_on_other_streams():
     q, scale = add_rmsnorm_quant(x, gamma, 1e-6, stream=stream)
     torch.cuda.synchronize()
     assert (q == 127).all() and torch.equal(scale, add_rmsnorm_quant(x, gamma, 1e-6)[1])
+
+
+# ------------------------------------------------------------------ every kind of tile, join and path
+def crowd(trees, bases, others=140):
+    """With many sequences of one node beside them: no tiles of 16 rows for few."""
+    return trees + [[-1]] * others, bases + [2] * others
+
+
+@gpu
+@pytest.mark.parametrize("groups,d", [(4, 128), (8, 64), (3, 128), (5, 32), (4, 16)])
+@pytest.mark.parametrize("rows", [16, 17, 24, 31, 32, 33, 64, 65, 128, 129])
+def test_tiles_of_so_many_rows(groups, d, rows):
+    n = max(1, rows // groups)
+    trees, bases = crowd(some_trees(rows, [n, n + 1]), [77, 600])
+    Trees(trees, bases, 2, groups, d, 16, seed=rows).check()
+
+
+@gpu
+@pytest.mark.parametrize("groups,d", [(4, 128), (2, 128), (4, 64), (8, 64), (8, 32)])
+def test_joins_of_many_rows(groups, d):
+    # more than 2048 rows to join, of tiles in several pieces and of tiles in one
+    rng = np.random.default_rng(d)
+    sizes = [int(n) for n in rng.integers(9, 17, 24)]
+    s = Trees(some_trees(d, sizes), [int(b) for b in rng.integers(300, 1500, 24)], 8, groups, d, 64, seed=d)
+    assert s.tokens * 8 >= 2048
+    s._check()
+    s._check(window=700, sinks=3)
+
+
+@gpu
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("n", [7, 40])
+def test_queries_that_are_not_finite(what, n):
+    # a row's value makes its own result NaN and no other
+    trees, bases = crowd(some_trees(n, [n, n]), [90, 700])
+    s = Trees(trees, bases, page=16, seed=41)
+    expect, bound = _reference(s, trees, 0, 0)
+    bad = ((0, 1, 7), (2, 5, 127), (n + 1, 0, 0), (2 * n - 1, 7, 64), (2 * n + 5, 3, 1))
+    for t, h, i in bad:
+        s.query[t, h, i] = float(what)
+    got = s.attend()
+    lost = np.isnan(got).any(axis=-1)
+    assert sorted(map(tuple, np.argwhere(lost))) == sorted((t, h) for t, h, _ in bad)
+    off = np.where(lost[..., None], 0.0, np.abs(got - expect)).reshape(s.tokens, -1).max(axis=1)
+    assert (off <= bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 300.0, 1e6, 1e36])
+def test_queries_of_any_size(scale):
+    for trees, bases in (crowd(some_trees(1, [7, 40]), [100, 90]), (some_trees(1, [7, 40]), [100, 90])):
+        s = Trees(trees, bases, page=16, seed=9)
+        s.query *= np.float32(scale)
+        s.check()
+
+
+@gpu
+def test_large_and_small_values():
+    trees, bases = crowd(some_trees(2, [8, 30, 100]), [100, 90, 300])
+    s = Trees(trees, bases, page=16, seed=10)
+    s.values[:] = np.where(np.isnan(s.values), s.values, s.values * np.float16(12000))
+    s.keys[:, :, ::2] *= np.float16(2.0 ** -14)           # subnormal keys
+    s.check()
+
+
+@gpu
+def test_offsets_past_32_bits():
+    # pools of more than 2^32 bytes and 2^31 elements: the pages in use lie at their end
+    from harsh4b_amd.tree import pages_accept, paged_append_tree, paged_attention_tree
+    trees = [chain(1), random_tree(np.random.default_rng(1), 20)]
+    s = Trees(trees, [49, 20], kv=8, groups=1, d=128, page=256, seed=15, spare=0)
+    pages = (1 << 31) // (8 * 256 * 128) + 8
+    keys = torch.zeros((1, pages, 8, 256, 128), dtype=torch.float16, device="cuda")
+    values = torch.zeros_like(keys)
+    n = s.keys.shape[0]
+    keys[0, -n:], values[0, -n:] = up(s.keys), up(s.values)
+    d, t = s.device(), plan(trees)
+    table = torch.where(d["table"] >= 0, d["table"] + (pages - n), d["table"])
+    got = paged_attention_tree(d["query"], keys[0], values[0], table, d["lengths"], t)
+    np.testing.assert_array_equal(got.cpu().numpy(), s.check())
+    inputs = [up(a) for a in _append_inputs(s, 8, 1, 128)]
+    status = ints([0])
+    paged_append_tree(*inputs, 1e-6, keys[0], values[0], table, d["lengths"], status, t)
+    paged_append_tree(*inputs, 1e-6, d["keys"], d["values"], d["table"], d["lengths"], status, t)
+    assert torch.equal(keys[0, -n:].nan_to_num(5.0), d["keys"].nan_to_num(5.0)) and int(status.item()) == 0
+    choices = ints([1] * 21)
+    drafted = ints([0] + [1] * 20)
+    for pools, book in (((keys, values), table), ((d["keys"][None], d["values"][None]), d["table"])):
+        pages_accept(*pools, book, d["lengths"], status, t, drafted, choices=choices)
+    assert torch.equal(keys[0, -n:].nan_to_num(5.0), d["keys"].nan_to_num(5.0)) and int(status.item()) == 0
+    assert not keys[0, :-n].any()
+
+
+@gpu
+@pytest.mark.parametrize("sequences", [2, 300])
+def test_captured_batches_that_are_cut(sequences):
+    """Tiles in pieces and their joins, with the plan in every wave and in a
+    launch of its own: two graphs, replayed in turn with eager work between."""
+    from harsh4b_amd.tree import paged_attention_tree
+    scenes = []
+    for seed, sizes, bases in ((61, [8, 60], [900, 1111]), (62, [100, 3], [1300, 700])):
+        spare = sequences - 2
+        s = Trees(some_trees(seed, sizes) + [[-1, 0]] * spare, bases + [30] * spare, 8, 4, 128, 64, seed=seed)
+        d, t = s.device(), plan(s.trees)
+        scenes.append((d, t, paged_attention_tree(**d, tree=t).clone()))
+    torch.cuda.synchronize()
+    graphs = []
+    for d, t, _ in scenes:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = paged_attention_tree(**d, tree=t)
+        graphs.append((g, out))
+    for i in range(6):
+        (g, out), (d, t, expect) = graphs[i % 2], scenes[i % 2]
+        out.fill_(7.0)
+        g.replay()
+        other = scenes[1 - i % 2]
+        assert torch.equal(paged_attention_tree(**other[0], tree=other[1]), other[2]), i
+        torch.cuda.synchronize()
+        assert torch.equal(out, expect), i
+
+
+@gpu
+def test_captured_greedy_paths():
+    # chains of a large vocabulary, replayed on other logits and drafts with eager work between
+    from harsh4b_amd.tree import pages_accept
+    rng = np.random.default_rng(6)
+    trees = some_trees(6, [9, 16, 1, 30], deep=6)
+    table, lengths, keys, values = _cache_of(trees, [5, 30, 0, 17])
+    n, vocab = sum(len(t) for t in trees), 60001
+    eager, replayed = ([up(keys), up(values)] for _ in range(2))
+    t, book, size, status = plan(trees), ints(table), ints(lengths), ints([0])
+    logits, drafted = torch.zeros((n, vocab), device="cuda"), ints([0] * n)
+    call = lambda pools: pages_accept(*pools, book, size, status, t, drafted, logits=logits, levels=7)
+    call([up(keys), up(values)])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = call(replayed)
+    for i in range(6):
+        logits.copy_(torch.randn_like(logits))
+        choices = rng.integers(0, vocab, n)
+        logits[torch.arange(n, device="cuda"), up(choices)] = 30.0
+        ids, at = rng.integers(0, vocab, n), 0
+        for tree in trees:
+            for k, p in enumerate(tree):
+                if p >= 0 and rng.random() < 0.7:
+                    ids[at + k] = choices[at + p]
+            at += len(tree)
+        drafted.copy_(ints(ids))
+        expect = call(eager)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, expect)), i
+        assert torch.equal(eager[0], replayed[0]) and torch.equal(eager[1], replayed[1]), i
+        at = 0
+        for b, tree in enumerate(trees):
+            path, choice = walk(tree, ids[at:at + len(tree)].tolist(), choices[at:at + len(tree)].tolist(), 7)
+            assert expect[1][at:at + len(path)].tolist() == path and int(expect[2][b]) == choice
+            at += len(tree)
+
+
+@gpu
+def test_drafted_tokens_outside_the_vocabulary():
+    # they are nobody's choice; given choices are any numbers
+    from harsh4b_amd.tree import pages_accept
+    trees = [[-1, 0, 0, 0], [-1, 0]]
+    table, lengths, keys, values = _cache_of(trees, [3, 4])
+    drafted = ints([0, -1, 50, 2**31 - 1, 0, -2**31])
+    logits = torch.zeros((6, 50), device="cuda")
+    logits[:, 49] = 1.0
+    got = pages_accept(up(keys), up(values), ints(table), ints(lengths), ints([0]), plan(trees), drafted, logits=logits)
+    assert [g.tolist() for g in got] == [[4, 5], [0, -1, -1, -1, 0, -1], [49, 49]]
+    got = pages_accept(up(keys), up(values), ints(table), ints(lengths), ints([0]), plan(trees), drafted,
+                       choices=ints([2**31 - 1, 7, 7, -5, -2**31, 9]))
+    assert [g.tolist() for g in got] == [[5, 6], [0, 3, -1, -1, 0, 1], [-5, 9]]
+
+
+@gpu
+def test_trees_that_were_not_planned():
+    # depths and ancestors of any contents: no access out of range, and rows of other sequences have their results
+    from harsh4b_amd.tree import paged_append_tree, paged_attention_tree
+    trees = some_trees(9, [9, 70, 12])
+    s = Trees(trees, [40, 300, 7], 2, 4, 64, 16, seed=9)
+    d, t = s.device(), plan(trees)
+    expect = s.check()
+    rng = np.random.default_rng(2)
+    inputs = [up(a) for a in _append_inputs(s, 2, 4, 64)]
+    for _ in range(3):
+        depths, ancestors = t.depths.clone(), t.ancestors.clone()
+        depths[9:79] = ints(rng.integers(-2**31, 2**31, 70))
+        ancestors[9:79] = ints(rng.integers(-2**31, 2**31, (70, 8)))
+        for window in (0, 5):
+            out = paged_attention_tree(**d, tree=t._replace(depths=depths, ancestors=ancestors), window=window)
+        out = paged_attention_tree(**d, tree=t._replace(depths=depths, ancestors=ancestors))
+        keep = [*range(9), *range(79, 91)]
+        np.testing.assert_array_equal(out.cpu().numpy()[keep], expect[keep])
+        status = ints([0])
+        paged_append_tree(*inputs, 1e-6, d["keys"].clone(), d["values"].clone(), d["table"], d["lengths"], status,
+                          t._replace(depths=depths))
+        assert int(status.item()) == 2
