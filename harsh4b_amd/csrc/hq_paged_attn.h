@@ -52,7 +52,19 @@
 // chunks are those of as many tokens in a row, and only the chunks that reach
 // past the tree's base (or lie at a window's edge) have masks: 32 keys' as one
 // word, the slots before the base by their range, the nodes by the row's
-// ancestor bits (tree_mask).
+// ancestor bits (tree_mask).  Trees of up to 32 rows (8 nodes of 4 heads) have
+// a third kind of tile:
+//   pair   two sets of 16 rows in each wave on the same keys, like small tiles
+//          otherwise, with the query's parts split once for the block and its
+//          remainders read from LDS (in registers 20 spill).  Bound by HBM: 32
+//          chats of 2048 to 4096 positions and trees of up to 8 nodes (425 MB)
+//          in 91 us, 4.7 TB/s.
+// More rows go to large tiles, though of 33 to 64 half the waves only copy: 32
+// chats of 16 nodes 100 us; the same rows as two waves a set, each with half of
+// a chunk's keys, 131 (half the time for the copies of the next chunk), as two
+// blocks of pairs that share an L2 113, as two sets of waves of one block 118
+// (3 us of arithmetic a step of 32 keys).  A prompt's length of tree (2 x 64
+// nodes at 40960, 140 GFLOP with the two parts) takes 133 us, 1.05 PFLOP/s.
 #pragma once
 
 #include <algorithm>
@@ -115,7 +127,10 @@ struct PagedAttnParams {
     int window, sinks;           // window 0: none
     int tile_tokens;             // tokens of a large tile
     int by_group;                // 65536 / groups + 1, for row_token
-    bool narrow;                 // (TREE) sequences of few chunks have tiles of 16 rows
+    // (TREE) sequences of few chunks have tiles of 16 rows, where each such tile of the batch has a CU: K and V are
+    // read once a tile, but from a cache, and a step's arithmetic is half (one chat of 300 and 8 nodes 11.2 us, 15.2
+    // in a pair)
+    bool narrow;
     bool whole;                  // no tile is cut (short tables): no join
     bool planned;                // the plan is in plan_first, plan_item, plan_count
     int part_rows;               // rows of partial results there is room for
@@ -1302,7 +1317,7 @@ __device__ void large_tile(const PagedAttnParams& p, const Piece& w, const Span&
         copy_v(page, at, c0);
         page = __builtin_amdgcn_readlane(pg, 4 + wave);
         if (c0 + 1 < c1) copy_k(page, at_next, c0 + 1);
-        if constexpr (TREE) split_query();     // (beside the first copies: pieces are short)
+        if constexpr (TREE) split_query();     // (beside the first copies)
         wait_all_memory();
         lds_sync();
         // copies of chunk cc + 1's V, and (once K of cc is read) of cc + 2's K

@@ -27,6 +27,8 @@ __device__ __forceinline__ bool tree_rows(const int32_t* starts, int b, int toke
 
 // -------------------------------------------------------------------- plan
 // A wave a sequence: its parents in LDS, and each lane walks up from its node.
+// Bound by latency: a launch and three dependent reads (one tree of 8 nodes 2.1
+// us, 64 of 60 3.5; a chain of 256 has 256 steps of an LDS read each).
 __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequences, int32_t* status)
 {
     __shared__ int parent_of[kTreeWaves][kTreeNodes];
@@ -221,40 +223,56 @@ __device__ Best row_part_best(const float* row, int vocab, int part, int splits,
 }
 
 // The argmax of the chains' rows: blocks (sequence, part of its rows, first of
-// the chain's levels that the block takes, every slots-th).  Every wave works
-// the chain out, while the root's row is read.
+// the chain's levels that the block takes, every slots-th).  A block's first
+// wave works the chain out, from three round trips: the sequence's numbers, its
+// nodes', and the nodes' logits at their parents, which lie scattered over the
+// rows.  Then the rows are bound by HBM: 32 chats' chains of 138 rows of 151936
+// (84 MB, 17.8 us at the rate of a copy) in 26 us; every row of the batch takes
+// 124, and a launch for each level would be seven.  A block that takes the levels
+// one after another (no slots) 45: the longest chain sets the time.
 __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
 {
     __shared__ Best red[kTreeWaves];
-    Sequence s;
-    s.load(p, blockIdx.x);
-    if (s.rows == 0) return;
-    auto take_row = [&](int u) {
-        const size_t row = size_t(s.first) + u;
+    __shared__ int rows[kTreeNodes], shared_rows;
+    if (threadIdx.x < kWave) {
+        const int lane = threadIdx.x;
+        int taken = 0;
+        Sequence s;
+        s.load(p, blockIdx.x);
+        if (s.settle()) {
+            Best own[kTreeLanes];              // a node's logit at its parent
+#pragma unroll
+            for (int k = 0; k < kTreeLanes; ++k) {
+                const int u = s.parent[k], i = s.token[k];
+                own[k] = Best{-__builtin_inff(), 0x7fffffff};
+                if (u >= 0 && i >= 0 && i < p.vocab && s.below(k, u))
+                    own[k] = Best{p.logits[size_t(s.first + u) * p.vocab + i], i};
+            }
+            const bool writes = blockIdx.y == 0 && blockIdx.z == 0 && lane == 0;
+            int u = 0;
+            for (int level = 0; u >= 0 && level < p.levels; ++level) {
+                if (writes) p.chain[s.first + level] = u;
+                if (level % p.slots == int(blockIdx.z)) {
+                    if (lane == 0) rows[taken] = s.first + u;
+                    ++taken;
+                }
+                Best x{-__builtin_inff(), 0x7fffffff};
+#pragma unroll
+                for (int k = 0; k < kTreeLanes; ++k)
+                    if (s.below(k, u)) x = better(x, own[k]);
+                const int choice = __builtin_amdgcn_readfirstlane(wave_best(x).i);
+                u = choice == 0x7fffffff ? -1 : s.child(u, choice);
+                if (u < 0 && level + 1 < s.n && writes) p.chain[s.first + level + 1] = -1;
+            }
+        }
+        if (lane == 0) shared_rows = taken;
+    }
+    lds_sync();
+    const int taken = __builtin_amdgcn_readfirstlane(shared_rows);
+    for (int k = 0; k < taken; ++k) {
+        const size_t row = __builtin_amdgcn_readfirstlane(rows[k]);
         const Best x = row_part_best(p.logits + row * p.vocab, p.vocab, blockIdx.y, p.splits, red);
         if (threadIdx.x == 0) p.best[row * p.splits + blockIdx.y] = x;
-    };
-    const bool writes = blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0;
-    if (blockIdx.z == 0) take_row(0);
-    if (!s.settle()) return;
-    Best own[kTreeLanes];              // a node's logit at its parent
-#pragma unroll
-    for (int k = 0; k < kTreeLanes; ++k) {
-        const int u = s.parent[k], i = s.token[k];
-        own[k] = Best{-__builtin_inff(), 0x7fffffff};
-        if (u >= 0 && i >= 0 && i < p.vocab && s.below(k, u)) own[k] = Best{p.logits[size_t(s.first + u) * p.vocab + i], i};
-    }
-    int u = 0;
-    for (int level = 0; u >= 0 && level < p.levels; ++level) {
-        if (writes) p.chain[s.first + level] = u;
-        if (level > 0 && level % p.slots == int(blockIdx.z)) take_row(u);
-        Best x{-__builtin_inff(), 0x7fffffff};
-#pragma unroll
-        for (int k = 0; k < kTreeLanes; ++k)
-            if (s.below(k, u)) x = better(x, own[k]);
-        const int choice = __builtin_amdgcn_readfirstlane(wave_best(x).i);
-        u = choice == 0x7fffffff ? -1 : s.child(u, choice);
-        if (u < 0 && level + 1 < s.n && writes) p.chain[s.first + level + 1] = -1;
     }
 }
 
@@ -283,8 +301,13 @@ __device__ __forceinline__ void chain_choices(const AcceptParams& p, const Seque
 }
 
 // The path, and its K and V to their slots: blocks (sequence, slice of the
-// layers' heads).  A block's first wave walks the path.
-constexpr int kMoveItems = 4;          // a wave's rows of (layer, K or V, kv head)
+// layers' heads).  A block's first wave walks the path; with all four walking
+// for themselves the walks are most of the time.  Bound by latency, five or six
+// dependent reads (one chat 4.2 us, of 36 layers and 8 kv heads), and where many
+// move by rows of 256 bytes that lie apart (32 chats, 12 MB: 8.6 us).
+// Of a wave's rows (layer, K or V, kv head) four: 8.6 us, 12.6 with two, 8.6
+// with eight (one chat 5.1), 10.6 with sixteen.
+constexpr int kMoveItems = 4;
 
 template <int D>
 __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
@@ -380,8 +403,9 @@ struct AcceptPlan {
     size_t chain, total;         // (best is at 0)
 };
 
-// Blocks aimed at for the rows of the chains' levels, many of which no chain reaches.
-constexpr int kChainBlocks = 512;
+// Blocks aimed at for the rows of the chains' levels, many of which no chain
+// reaches (32 chats of 16 nodes: 26 us, 28 with 512, 30 with 2048).
+constexpr int kChainBlocks = 1024;
 
 static AcceptPlan accept_plan(int tokens, int sequences, int vocab, int levels)
 {
