@@ -731,7 +731,7 @@ def add_rmsnorm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float, delta: t
     if rows:
         _launch(_native.lib().hq_add_rmsnorm_quant,
                 (x_ptr, delta_ptr, gamma.data_ptr(), out_ptr, q.data_ptr(), act_scales.data_ptr(), rows, n, eps),
-                None, index, stream, (x, gamma, delta, out, q, act_scales), "hq_add_rmsnorm_quant")
+                None, index, stream, stream and (x, gamma, delta, out, q, act_scales), "hq_add_rmsnorm_quant")
     return q, act_scales
 
 

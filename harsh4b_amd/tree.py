@@ -92,7 +92,7 @@ def tree_plan(parents: torch.Tensor, starts: torch.Tensor, status: torch.Tensor,
                ((parents.data_ptr(), 4 * tokens), (starts.data_ptr(), 4 * sequences + 4), (status.data_ptr(), 4)))
     if tokens:
         _launch(_native.lib().hq_tree_plan, (packed, sequences, status.data_ptr()), None, index, stream,
-                (*tree, status), "hq_tree_plan")
+                stream and (*tree, status), "hq_tree_plan")
     return tree
 
 
@@ -140,7 +140,7 @@ def paged_append_tree(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Ten
         _launch(_native.lib().hq_paged_append_tree,
                 (cache, qkv.data_ptr(), packed, heads, q_norm.data_ptr(), k_norm.data_ptr(), eps, rope_cos.data_ptr(),
                  rope_sin.data_ptr(), shape[0], out.data_ptr()), None, index, stream,
-                (qkv, q_norm, k_norm, rope_cos, rope_sin, keys, values, table, lengths, status, *tree, out),
+                stream and (qkv, q_norm, k_norm, rope_cos, rope_sin, keys, values, table, lengths, status, *tree, out),
                 "hq_paged_append_tree")
     return out
 
@@ -182,7 +182,7 @@ def paged_attention_tree(query: torch.Tensor, keys: torch.Tensor, values: torch.
         _launch(_native.lib().hq_paged_attention_tree,
                 (cache, query.data_ptr(), packed, heads, window, sinks, out.data_ptr()),
                 _attention_workspace_bytes(tokens, heads, kv, d), index, stream,
-                (query, keys, values, table, lengths, *tree, out), "hq_paged_attention_tree")
+                stream and (query, keys, values, table, lengths, *tree, out), "hq_paged_attention_tree")
     return out
 
 
@@ -243,5 +243,6 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
     _launch(_native.lib().hq_pages_accept,
             (cache, packed, ids, chosen, rows, vocab, levels, kept.data_ptr(), path.data_ptr(), after.data_ptr()),
             _accept_workspace_bytes(tokens, sequences, vocab, levels), index, stream,
-            (keys, values, table, lengths, status, *tree, drafted, choices, logits, kept, path, after), "hq_pages_accept")
+            stream and (keys, values, table, lengths, status, *tree, drafted, choices, logits, kept, path, after),
+            "hq_pages_accept")
     return kept, path, after
