@@ -14,6 +14,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr int kTreeLanes = kTreeNodes / kWave;   // nodes a lane holds: lane, lane + 64, ..
 constexpr int kTreeWaves = kBlock / kWave;
+constexpr int kTreePages = kTreeNodes / 16 + 1;  // a tree may lie in
 
 // A sequence's rows; false: its starts are no range of the batch's rows.
 __device__ __forceinline__ bool tree_rows(const int32_t* starts, int b, int tokens, int* first, int* count)
@@ -86,8 +87,7 @@ struct AcceptParams {
     int vocab, levels, shift;
     int slots;                   // levels of a chain looked at side by side
     int splits;                  // parts of a row of logits
-    Best* best;                  // [tokens, splits] (the chains' rows)
-    int32_t* chain;              // [tokens] a sequence's chain in its first rows, then -1
+    Best* best;                  // [tokens, splits] of the chain's node at level l in a sequence's row l
     int32_t* kept;
     int32_t* path;
     int32_t* next;
@@ -128,9 +128,8 @@ struct Sequence {
     int first, n, base;
     int rows;                    // its rows of the batch (whether it takes part or not)
     bool bad;
-    int parent[kTreeLanes], token[kTreeLanes], choice[kTreeLanes];
-
-    int depth, status;
+    int parent[kTreeLanes], token[kTreeLanes], choice[kTreeLanes], depth[kTreeLanes];
+    int status;
 
     // Two round trips, the second under way when this returns: the sequence's
     // numbers, then its nodes' together.
@@ -145,20 +144,20 @@ struct Sequence {
         base = __builtin_amdgcn_readfirstlane(length) - rows;
         n = 0;
         if (rows == 0) return;
-        depth = p.t.depths[first];
 #pragma unroll
         for (int k = 0; k < kTreeLanes; ++k) {
             const int i = lane + k * kWave;
             parent[k] = i < rows ? p.t.parents[first + i] : -2;
             token[k] = i < rows ? p.drafted[first + i] : 0;
             choice[k] = i < rows && p.choices ? p.choices[first + i] : 0;
+            depth[k] = i < rows ? p.t.depths[first + i] : -1;
         }
     }
     // Whether it takes part.
     __device__ __forceinline__ bool settle()
     {
         if (rows == 0) return false;
-        bad = __builtin_amdgcn_readfirstlane(depth) < 0 || rows > kTreeNodes || base < 0;
+        bad = __builtin_amdgcn_readfirstlane(depth[0]) < 0 || rows > kTreeNodes || base < 0;
         if (!bad && (__builtin_amdgcn_readfirstlane(status) & (HQ_PAGES_FULL | HQ_PAGES_REFUSED)) == 0) n = rows;
         return n != 0;
     }
@@ -233,7 +232,7 @@ __device__ Best row_part_best(const float* row, int vocab, int part, int splits,
 __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
 {
     __shared__ Best red[kTreeWaves];
-    __shared__ int rows[kTreeNodes], shared_rows;
+    __shared__ int node[kTreeNodes], nodes, first;
     if (threadIdx.x < kWave) {
         const int lane = threadIdx.x;
         int taken = 0;
@@ -248,12 +247,11 @@ __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
                 if (u >= 0 && i >= 0 && i < p.vocab && s.below(k, u))
                     own[k] = Best{p.logits[size_t(s.first + u) * p.vocab + i], i};
             }
-            const bool writes = blockIdx.y == 0 && blockIdx.z == 0 && lane == 0;
+            if (lane == 0) first = s.first;
             int u = 0;
             for (int level = 0; u >= 0 && level < p.levels; ++level) {
-                if (writes) p.chain[s.first + level] = u;
                 if (level % p.slots == int(blockIdx.z)) {
-                    if (lane == 0) rows[taken] = s.first + u;
+                    if (lane == 0) node[taken] = u;
                     ++taken;
                 }
                 Best x{-__builtin_inff(), 0x7fffffff};
@@ -262,47 +260,47 @@ __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
                     if (s.below(k, u)) x = better(x, own[k]);
                 const int choice = __builtin_amdgcn_readfirstlane(wave_best(x).i);
                 u = choice == 0x7fffffff ? -1 : s.child(u, choice);
-                if (u < 0 && level + 1 < s.n && writes) p.chain[s.first + level + 1] = -1;
             }
         }
-        if (lane == 0) shared_rows = taken;
+        if (lane == 0) nodes = taken;
     }
     lds_sync();
-    const int taken = __builtin_amdgcn_readfirstlane(shared_rows);
+    const int taken = __builtin_amdgcn_readfirstlane(nodes);
+    if (taken == 0) return;
+    const size_t from = __builtin_amdgcn_readfirstlane(first);
     for (int k = 0; k < taken; ++k) {
-        const size_t row = __builtin_amdgcn_readfirstlane(rows[k]);
-        const Best x = row_part_best(p.logits + row * p.vocab, p.vocab, blockIdx.y, p.splits, red);
-        if (threadIdx.x == 0) p.best[row * p.splits + blockIdx.y] = x;
+        const float* row = p.logits + (from + __builtin_amdgcn_readfirstlane(node[k])) * p.vocab;
+        const Best x = row_part_best(row, p.vocab, blockIdx.y, p.splits, red);
+        if (threadIdx.x == 0) p.best[(from + blockIdx.z + size_t(k) * p.slots) * p.splits + blockIdx.y] = x;
     }
 }
 
-// The choices along a sequence's chain, into LDS, by a wave: splits lanes (a
-// power of two) a level, 64 / splits levels at a time.
+// The choices at the levels of a sequence's chain, into LDS, by a wave: splits
+// lanes (a power of two) a level, 64 / splits levels at a time.  What lies past
+// the chain's end is of any contents, and the walk, which ends there, does not
+// come to it.
 __device__ __forceinline__ void chain_choices(const AcceptParams& p, const Sequence& s, int* level_choice)
 {
     const int lane = threadIdx.x & (kWave - 1);
     const int part = lane & (p.splits - 1), each = kWave / p.splits;
-    const int levels = min(p.levels, s.n);
+    int deepest = 0;
+#pragma unroll
+    for (int k = 0; k < kTreeLanes; ++k) deepest = max(deepest, s.depth[k]);
+    deepest = -wave_imin64_all(-deepest);
+    const int levels = min(min(p.levels, s.n), deepest + 1);
     for (int from = 0; from < levels; from += each) {
         const int level = from + lane / p.splits;
-        // (what follows the chain's end is of any contents)
-        int ended = 0;
-        int u = level < levels ? p.chain[s.first + level] : -1;
-        if (u < 0 || u >= s.n) u = -1;
-        Best x{-__builtin_inff(), 0x7fffffff};
-        if (u >= 0) x = p.best[size_t(s.first + u) * p.splits + part];
+        Best x = p.best[size_t(s.first + min(level, levels - 1)) * p.splits + part];
         for (int o = p.splits / 2; o >= 1; o >>= 1)
             x = better(x, Best{__shfl_xor(x.v, o, kWave), __shfl_xor(x.i, o, kWave)});
         if (level < levels && part == 0) level_choice[level] = x.i;
-        ended = __any(level < levels && u < 0);
-        if (ended) break;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // The path, and its K and V to their slots: blocks (sequence, slice of the
 // layers' heads).  A block's first wave walks the path; with all four walking
-// for themselves the walks are most of the time.  Bound by latency, five or six
+// for themselves the walks are most of the time.  Bound by latency, four or five
 // dependent reads (one chat 4.2 us, of 36 layers and 8 kv heads), and where many
 // move by rows of 256 bytes that lie apart (32 chats, 12 MB: 8.6 us).
 // Of a wave's rows (layer, K or V, kv head) four: 8.6 us, 12.6 with two, 8.6
@@ -313,7 +311,7 @@ template <int D>
 __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
 {
     constexpr int PIECES = D / 8, ROWS = kWave / PIECES;   // 16-byte pieces of a K row, rows a wave moves at a time
-    __shared__ int level_choice[kTreeNodes], path[kTreeNodes];
+    __shared__ int level_choice[kTreeNodes], path[kTreeNodes], page_at[kTreePages];
     __shared__ int shared_count, shared_base;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int b = blockIdx.x;
@@ -321,6 +319,11 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
     if (wave == 0) {
         Sequence s;
         s.load(p, b);
+        if (lane < kTreePages) {               // the pages of the tree's slots
+            const int e = (s.base >> p.shift) + lane;
+            const int page = s.rows && s.base >= 0 && e < p.c.max_pages ? p.c.table[size_t(b) * p.c.max_pages + e] : -1;
+            page_at[lane] = page < p.c.pages ? page : -1;
+        }
         int count = 0, choice = -1;
         if (s.settle()) {
             if (p.logits) chain_choices(p, s, level_choice);
@@ -362,11 +365,7 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
         const int v = i < count ? path[i] : -1;
         bool moves = i < count && v != i;
         if (!__any(moves)) continue;
-        auto page_of = [&](int slot) {
-            const int e = slot >> p.shift;
-            const int page = e < p.c.max_pages ? p.c.table[size_t(b) * p.c.max_pages + e] : -1;
-            return page < p.c.pages ? page : -1;
-        };
+        auto page_of = [&](int slot) { return page_at[(slot >> p.shift) - (base >> p.shift)]; };
         const int to = moves ? page_of(base + i) : 0, of = moves ? page_of(base + v) : 0;
         if (to < 0 || of < 0) {
             moves = false;
@@ -400,7 +399,7 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
 // -------------------------------------------------------------------- host
 struct AcceptPlan {
     int slots, splits;
-    size_t chain, total;         // (best is at 0)
+    size_t bytes;
 };
 
 // Blocks aimed at for the rows of the chains' levels, many of which no chain
@@ -410,15 +409,13 @@ constexpr int kChainBlocks = 1024;
 static AcceptPlan accept_plan(int tokens, int sequences, int vocab, int levels)
 {
     AcceptPlan a{};
-    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
     if (vocab) {                                       // (a power of two: see chain_choices)
         a.slots = int(std::max<int64_t>(1, std::min<int64_t>({levels, tokens, 16, kMaxBlocks / sequences})));
         a.splits = 1;
         const int64_t rows = int64_t(sequences) * a.slots;
         while (a.splits < kWave && a.splits * rows < kChainBlocks && a.splits * 2048 < vocab) a.splits *= 2;
     }
-    a.chain = up(size_t(tokens) * a.splits * sizeof(Best));
-    a.total = a.chain + up(vocab ? size_t(tokens) * 4 : 0);
+    a.bytes = size_t(tokens) * a.splits * sizeof(Best);
     return a;
 }
 
@@ -449,7 +446,7 @@ extern "C" int hq_tree_plan(const hq_tree* tree, int sequences, int32_t* status,
 extern "C" size_t hq_pages_accept_workspace_bytes(int tokens, int sequences, int vocab, int levels)
 {
     if (tokens < 0 || sequences < 1 || vocab < 0 || levels < 1 || levels > kTreeNodes) return 0;
-    return std::max<size_t>(256, accept_plan(tokens, sequences, vocab, levels).total);
+    return std::max<size_t>(256, accept_plan(tokens, sequences, vocab, levels).bytes);
 }
 
 extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const int32_t* drafted, const int32_t* choices,
@@ -472,9 +469,8 @@ extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const
                           static_cast<const void*>(path), static_cast<const void*>(next)})
         if (reinterpret_cast<uintptr_t>(q) & 3u) return HQ_ERR_ALIGN;
     const AcceptPlan a = accept_plan(tree->tokens, cache->sequences, vocab, levels);
-    char* ws = static_cast<char*>(workspace);
     AcceptParams p{*cache, *tree, drafted, choices, logits, vocab, levels, batch.shift, a.slots, a.splits,
-                   reinterpret_cast<Best*>(ws), reinterpret_cast<int32_t*>(ws + a.chain), kept, path, next};
+                   static_cast<Best*>(workspace), kept, path, next};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t items = int64_t(2) * cache->layers * cache->kv_heads;
     if (items > 0x7fffffff) return HQ_ERR_ARG;
