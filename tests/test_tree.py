@@ -1356,3 +1356,107 @@ def test_trees_that_were_not_planned():
         paged_append_tree(*inputs, 1e-6, d["keys"].clone(), d["values"].clone(), d["table"], d["lengths"], status,
                           t._replace(depths=depths))
         assert int(status.item()) == 2
+
+
+@gpu
+@pytest.mark.parametrize("kv,groups", [(2, 4), (1, 8)])
+def test_few_trees_among_many_sequences(kv, groups):
+    # the plan in a launch of its own, with tiles of 16 rows
+    trees = [[] for _ in range(300)]
+    for b, n in ((3, 5), (77, 20), (299, 9)):
+        trees[b] = random_tree(np.random.default_rng(b), n)
+    Trees(trees, [int(b) for b in np.random.default_rng(1).integers(0, 90, 300)], kv, groups, 32, 16, seed=2).check()
+
+
+@gpu
+@pytest.mark.parametrize("held", [1, 4])
+def test_append_while_the_cache_refuses(held):
+    # the queries as ever, no K and V
+    from harsh4b_amd.tree import paged_append_tree
+    trees = some_trees(3, [5, 9])
+    s = Trees(trees, [20, 33], 2, 4, 64, 16, seed=3)
+    inputs = _append_inputs(s, 2, 4, 64)
+    expect, _, _, _ = _append(s, trees, inputs)
+    d, status = s.device(), ints([held])
+    q = paged_append_tree(*[up(a) for a in inputs], 1e-6, d["keys"], d["values"], d["table"], d["lengths"], status, plan(trees))
+    np.testing.assert_array_equal(q.cpu().numpy(), expect)
+    np.testing.assert_array_equal(d["keys"].cpu().numpy(), s.keys)
+    np.testing.assert_array_equal(d["values"].cpu().numpy(), s.values)
+    assert int(status.item()) == held
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 5)])
+def test_a_server_s_trees(window, sinks):
+    """Steps of sequences that come, grow by accepted paths across page borders,
+    pause and end, against a list of each one's rows; growth straight from one
+    tree to the next, or under a window through the kept length."""
+    from harsh4b_amd.paged import PagedCache
+    kv, groups, d, rows = 2, 4, 32, 5
+    rng = np.random.default_rng(window + 1)
+    c = PagedCache(2, 90, kv, d, sequences=rows, max_pages=20, page_size=16)
+    c.keys.fill_(float("nan"))
+    c.values.fill_(float("nan"))
+    angle = np.arange(320)[:, None] * 10000.0 ** (-np.arange(0, d, 2) / d)
+    cos, sin = up(np.cos(angle).astype(np.float32)), up(np.sin(angle).astype(np.float32))
+    norm = torch.ones(d, device="cuda")
+    kept_rows = [[] for _ in range(rows)]             # of each sequence: [(keys, values) of both layers, ..] by position
+    kept = [0] * rows
+    for step in range(30):
+        for b in range(rows):
+            if kept[b] > 200 or (kept[b] and rng.random() < 0.05):
+                kept[b], kept_rows[b] = 0, []
+        sizes = [int(n) if rng.random() < 0.8 else 0 for n in rng.integers(1, 24, rows)]
+        trees = [random_tree(rng, n, 6) if n else [] for n in sizes]
+        bases = list(kept)
+        if window:
+            c.resize(kept, window, sinks)
+        c.resize([k + n for k, n in zip(kept, sizes)], window, sinks)
+        tree = c.plan_tree(np.concatenate([t for t in trees if t] or [[]]).astype(int).tolist(), starts_of(trees).tolist())
+        tokens = sum(sizes)
+        if tokens == 0:
+            continue
+        queries = []
+        for layer in range(2):
+            qkv = up((2 * rng.standard_normal((tokens, (kv * groups + 2 * kv) * d))).astype(np.float32))
+            queries.append(c.append_tree(layer, qkv, norm, norm, cos, sin, 1e-6, tree))
+        table, keys, values = c.table.cpu().numpy(), c.keys.cpu().numpy(), c.values.cpu().numpy()
+        lengths = c.lengths.tolist()
+        assert lengths == [k + n for k, n in zip(kept, sizes)]
+        for b in range(rows):
+            low = max(0, bases[b] - window + 1) if window else 0
+            for j in range(lengths[b]):
+                if sinks <= j < low:
+                    continue
+                page = table[b, j // 16]
+                assert page >= 0, (step, b, j)
+                here = keys[:, page, :, j % 16], values[:, page, :, j % 16]
+                if j < bases[b]:
+                    np.testing.assert_array_equal(here[0], kept_rows[b][j][0])
+                    np.testing.assert_array_equal(here[1], kept_rows[b][j][1])
+        for layer in range(2):
+            out = c.attend_tree(layer, queries[layer], tree, window, sinks).cpu().numpy()
+            s = Scene.__new__(Scene)
+            s.keys, s.values, s.table, s.lengths = keys[layer], values[layer], table, lengths
+            s.query, s.starts, s.tokens = queries[layer].cpu().numpy(), starts_of(trees), tokens
+            expect, bound = _reference(s, trees, window, sinks)
+            off = np.abs(out - expect).reshape(tokens, -1).max(axis=1)
+            assert (off <= bound).all(), (step, layer, off.max())
+        drafted, choices = some_choices(step, trees, 2)
+        got, path, after = c.accept(tree, drafted, choices=choices, levels=7)
+        got, path, after, at = got.tolist(), path.tolist(), after.tolist(), 0
+        for b, t in enumerate(trees):
+            if not t:
+                assert got[b] == -1 and after[b] == -1
+                continue
+            p, choice = walk(t, drafted[at:at + len(t)], choices[at:at + len(t)], 7)
+            assert path[at:at + len(t)] == p + [-1] * (len(t) - len(p)) and after[b] == choice
+            for v in p:
+                j = bases[b] + v
+                page = table[b, j // 16]
+                kept_rows[b].append((keys[:, page, :, j % 16].copy(), values[:, page, :, j % 16].copy()))
+            kept[b] = bases[b] + len(p)
+            assert got[b] == kept[b] == len(kept_rows[b])
+            at += len(t)
+        c.check_status()
+    assert max(kept) > 30
