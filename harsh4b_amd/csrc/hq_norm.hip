@@ -85,7 +85,8 @@ __global__ __launch_bounds__(kBlock) void norm_quant_kernel(NormParams p)
     if (p.sum) {
         const auto sum = raw_rsrc(p.sum + at, 4 * n);
 #pragma unroll
-        for (int k = 0; k < NPT; ++k) __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[k]), sum, 4 * (t + kBlock * k), 0, 0);
+        for (int k = 0; k < NPT; ++k)
+            __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[k]), sum, 4 * (t + kBlock * k), 0, 0);
     }
     const float r = __builtin_sqrtf(total / float(n) + p.eps);
     float amax = 0.0f;

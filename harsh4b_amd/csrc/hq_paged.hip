@@ -79,7 +79,8 @@ __global__ __launch_bounds__(kBlock) void paged_append_kernel(AppendParams p)
     const int page = paged_page(p.b, b, pos);
     const int depth = TREE ? p.depths[t] : 0;
     const int angle = TREE ? pos - (t - first) + depth : pos;      // (pos - (t - first): the tree's base)
-    const bool placed = (TREE ? pos >= t - first && depth >= 0 && depth <= t - first : pos >= 0) && angle < p.rope_positions && page >= 0;
+    const bool inside = TREE ? pos >= t - first && depth >= 0 && depth <= t - first : pos >= 0;
+    const bool placed = inside && angle < p.rope_positions && page >= 0;
     const bool held = (*p.b.status & (HQ_PAGES_FULL | HQ_PAGES_REFUSED)) != 0;
     if (!placed && lane == 0) atomicOr(p.b.status, HQ_PAGES_BAD);
     // pairs (i, i + D/2): of D = 128 in one lane, else in lanes D/2 apart

@@ -640,8 +640,11 @@ __device__ void redo_row(const PagedAttnParams& p, const Piece& w, const Span& s
     for (int c = c0; c < c1; ++c) {
         const int at = span.chunk(c) * kChunkKeys;
         paged_row<D>(p, p.query + row * D, w.b, w.head, at, int(min(end, int64_t(at) + kChunkKeys)),
-                     [&](int j) { return TREE ? (w.mask(p, token, p.tree.depths[w.first + token], j, w.bits(p, token, j)) & 1u) != 0
-                                              : paged_visible(w.position(token), j, p.window, p.sinks); },
+                     [&](int j) {
+                         if constexpr (!TREE) return paged_visible(w.position(token), j, p.window, p.sinks);
+                         const int depth = p.tree.depths[w.first + token];
+                         return (w.mask(p, token, depth, j, w.bits(p, token, j)) & 1u) != 0;
+                     },
                      m, l, o, seen);
     }
     if (w.pieces == 1) {
@@ -766,9 +769,9 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
     const int q_set = SHARED ? wave & 1 : 0;
     float4v x[STEPS][2];
     {
-        const int i = SHARED && q_set ? 1 : 0;
-        const float* q = p.query + (size_t(w.first + (i ? token[R - 1] : token[0])) * p.b.heads + w.head * G +
-                                    ((i ? mine[R - 1] : mine[0]) ? 16 * i + n - (i ? token[R - 1] : token[0]) * G : 0)) * D;
+        const int i = SHARED && q_set ? 1 : 0, of = i ? token[R - 1] : token[0];
+        const int head = (i ? mine[R - 1] : mine[0]) ? 16 * i + n - of * G : 0;
+        const float* q = p.query + (size_t(w.first + of) * p.b.heads + w.head * G + head) * D;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int d = D >= 32 ? 32 * s + 8 * g : 8 * (g & 1);
@@ -931,9 +934,11 @@ __device__ void small_tile(const PagedAttnParams& p, const Piece& w, const Span&
                 a[d] = __builtin_amdgcn_perm(vf[2 * d + 1][i / 2], vf[2 * d][i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
             const half8 v = __builtin_bit_cast(half8, a);
 #pragma unroll
-            for (int r = 0; r < R; ++r) acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[r], acc[r][i], 0, 0, 0);
+            for (int r = 0; r < R; ++r)
+                acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[r], acc[r][i], 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < R; ++r) acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[r], acc[r][i], 0, 0, 0);
+            for (int r = 0; r < R; ++r)
+                acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[r], acc[r][i], 0, 0, 0);
         }
         if (kn < own) load_v(next0, next1, nj);
         pg0 = next0;

@@ -372,8 +372,10 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
             if (writes) atomicOr(p.c.status, HQ_PAGES_BAD);
         }
         const size_t place = (lane % PIECES) * 8;
-        const size_t dst = size_t(max(to, 0)) * heads * head + size_t((base + i) & (p.c.page_size - 1)) * D + place;
-        const size_t src = size_t(max(of, 0)) * heads * head + size_t((base + max(v, 0)) & (p.c.page_size - 1)) * D + place;
+        auto offset = [&](int page, int slot) {
+            return size_t(max(page, 0)) * heads * head + size_t(slot & (p.c.page_size - 1)) * D + place;
+        };
+        const size_t dst = offset(to, base + i), src = offset(of, base + max(v, 0));
         for (int item = (blockIdx.y * kTreeWaves + wave) * kMoveItems; item < items;
              item += gridDim.y * kTreeWaves * kMoveItems) {
             uint4v x[kMoveItems];
@@ -449,15 +451,15 @@ extern "C" size_t hq_pages_accept_workspace_bytes(int tokens, int sequences, int
     return std::max<size_t>(256, accept_plan(tokens, sequences, vocab, levels).bytes);
 }
 
-extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const int32_t* drafted, const int32_t* choices,
-                               const float* logits, int vocab, int levels, int32_t* kept, int32_t* path, int32_t* next,
-                               void* workspace, void* stream)
+extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const int32_t* drafted,
+                               const int32_t* choices, const float* logits, int vocab, int levels, int32_t* kept,
+                               int32_t* path, int32_t* next, void* workspace, void* stream)
 {
     const int bad = tree_check(tree);
     if (bad) return bad;
     PagedBatch batch;
-    const int err = paged_check(cache, cache ? cache->keys : nullptr, tree->starts, tree->tokens, cache ? cache->kv_heads : 0,
-                                cache ? cache->values : nullptr, &batch);
+    if (!cache) return HQ_ERR_ARG;
+    const int err = paged_check(cache, cache->keys, tree->starts, tree->tokens, cache->kv_heads, cache->values, &batch);
     if (err) return err;
     if (cache->layers < 1 || !cache->status || !kept || !next || !workspace || levels < 1 || levels > kTreeNodes)
         return HQ_ERR_ARG;
@@ -475,7 +477,8 @@ extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const
     const int64_t items = int64_t(2) * cache->layers * cache->kv_heads;
     if (items > 0x7fffffff) return HQ_ERR_ARG;
     const int per_block = kTreeWaves * kMoveItems;
-    const int slices = int(std::min({(items + per_block - 1) / per_block, kMaxBlocks / cache->sequences, int64_t(4096)}));
+    const int slices = int(std::min({(items + per_block - 1) / per_block, kMaxBlocks / cache->sequences,
+                                     int64_t(4096)}));
     if (logits && tree->tokens) {
         hipLaunchKernelGGL(accept_chain_kernel, dim3(cache->sequences, a.splits, a.slots), dim3(kBlock), 0, s, p);
     }

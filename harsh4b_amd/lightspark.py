@@ -693,7 +693,8 @@ def add_rmsnorm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float, delta: t
     if n == 0 or n > 1 << 30 or rows >= 1 << 24:
         raise ValueError("x must be [rows, n] with n from 1 to 2^30 and fewer than 2^24 rows")
     f32 = torch.float32
-    if gamma is None or gamma.shape != (n,) or gamma.dtype is not f32 or gamma.get_device() != index or not gamma.is_contiguous():
+    if (gamma is None or gamma.shape != (n,) or gamma.dtype is not f32 or gamma.get_device() != index or
+            not gamma.is_contiguous()):
         raise ValueError("gamma must be a contiguous float32 tensor [n] on x's device")
     size = 4 * rows * n
     x_ptr, inputs = x.data_ptr(), [(gamma.data_ptr(), 4 * n)]

@@ -236,8 +236,8 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
         for t, name in ((kept, "kept"), (after, "next")):
             if t.shape != (sequences,) or t.dtype is not _I32 or t.get_device() != index or not t.is_contiguous():
                 _refuse(name, t, _I32, index, "[sequences]")
-        _apart([_span(t) for t in (kept, path, after)],
-               [_span(t) for t in (keys, values, table, lengths, status, *tree, drafted, choices, logits) if t is not None])
+        given = keys, values, table, lengths, status, *tree, drafted, choices, logits
+        _apart([_span(t) for t in (kept, path, after)], [_span(t) for t in given if t is not None])
     if tokens == 0:
         vocab, rows = 0, None                  # (nothing is read)
     _launch(_native.lib().hq_pages_accept,
