@@ -27,13 +27,17 @@ __device__ __forceinline__ bool tree_rows(const int32_t* starts, int b, int toke
 }
 
 // -------------------------------------------------------------------- plan
-// A wave a sequence: its parents in LDS, and each lane walks up from its node.
-// Bound by latency: a launch and three dependent reads (one tree of 8 nodes 2.1
-// us, 64 of 60 3.5; a chain of 256 has 256 steps of an LDS read each).
+// A wave a sequence.  Each node holds the bits of the nodes up to some above it
+// and which one comes next; a round takes over that one's, so that after k
+// rounds 2^k nodes are covered: a chain of 256 has 8 rounds (6.0 us; walking up
+// node by node, 255 steps, 65).  A node's depth is the number of its bits, less its
+// own.  Bound by latency, a launch and three dependent reads (one tree of 8
+// nodes 2.1 us, 64 of 60 3.8).
 __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequences, int32_t* status)
 {
-    __shared__ int parent_of[kTreeWaves][kTreeNodes];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    __shared__ uint4v seen_of[kTreeWaves][kTreeNodes][2];
+    __shared__ int next_of[kTreeWaves][kTreeNodes];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int b = blockIdx.x * kTreeWaves + wave;
     if (b >= sequences) return;
     int first, n;
@@ -41,29 +45,62 @@ __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequen
         if (lane == 0) atomicOr(status, HQ_PAGES_BAD);
         return;
     }
+    first = __builtin_amdgcn_readfirstlane(first);
+    n = __builtin_amdgcn_readfirstlane(n);
+    uint4v seen[kTreeLanes][2];
+    int next[kTreeLanes];
     bool bad = n > kTreeNodes;
-    for (int i = lane; i < n && i < kTreeNodes; i += kWave) {
-        const int p = t.parents[first + i];
-        bad |= p < -1 || p >= i;
-        parent_of[wave][i] = p;
+#pragma unroll
+    for (int k = 0; k < kTreeLanes; ++k) {
+        const int i = lane + k * kWave;
+        next[k] = i < n ? t.parents[first + i] : -1;
+        bad |= next[k] < -1 || next[k] >= i;
+        seen[k][0] = seen[k][1] = uint4v{0, 0, 0, 0};
+        const uint32_t bit = 1u << (lane & 31);
+        seen[k][k / 2][2 * (k % 2)] = lane < 32 ? bit : 0u;
+        seen[k][k / 2][2 * (k % 2) + 1] = lane < 32 ? 0u : bit;
     }
     bad = __any(bad);
-    if (bad && lane == 0) atomicOr(status, HQ_PAGES_BAD);
-    for (int i = lane; i < n; i += kWave) {
-        uint32_t words[kTreeWords] = {};
-        int depth = -1;
-        if (!bad) {
-            // (a parent stands before its node: the walk ends)
-            for (int at = i; at >= 0; at = parent_of[wave][at]) {
-                ++depth;
-#pragma unroll
-                for (int w = 0; w < kTreeWords; ++w) words[w] |= at >> 5 == w ? 1u << (at & 31) : 0u;
-            }
+    if (bad) {
+        if (lane == 0) atomicOr(status, HQ_PAGES_BAD);
+        for (int i = lane; i < n; i += kWave) {
+            t.depths[first + i] = -1;
+            uint4v* const to = reinterpret_cast<uint4v*>(t.ancestors + size_t(first + i) * kTreeWords);
+            to[0] = to[1] = uint4v{0, 0, 0, 0};
         }
+        return;
+    }
+    while (true) {
+        bool more = false;
+        unrolled<kTreeLanes>([&](auto lanes) {
+            constexpr int k = decltype(lanes)::value;
+            if (k * kWave >= n) return;
+            seen_of[wave][lane + k * kWave][0] = seen[k][0];
+            seen_of[wave][lane + k * kWave][1] = seen[k][1];
+            next_of[wave][lane + k * kWave] = next[k];
+            more |= next[k] >= 0;
+        });
+        if (!__any(more)) break;
+        // (a wave's LDS accesses take effect in their order: all of a round's reads come before the next one's writes)
+        unrolled<kTreeLanes>([&](auto lanes) {
+            constexpr int k = decltype(lanes)::value;
+            if (k * kWave >= n || next[k] < 0) return;
+            seen[k][0] |= seen_of[wave][next[k]][0];
+            seen[k][1] |= seen_of[wave][next[k]][1];
+            next[k] = next_of[wave][next[k]];
+        });
+    }
+#pragma unroll
+    for (int k = 0; k < kTreeLanes; ++k) {
+        const int i = lane + k * kWave;
+        if (i >= n) continue;
+        int depth = -1;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) depth += __popc(seen[k][0][w]) + __popc(seen[k][1][w]);
         t.depths[first + i] = depth;
-        uint4* to = reinterpret_cast<uint4*>(t.ancestors + size_t(first + i) * kTreeWords);
-        to[0] = make_uint4(words[0], words[1], words[2], words[3]);
-        to[1] = make_uint4(words[4], words[5], words[6], words[7]);
+        uint4v* const to = reinterpret_cast<uint4v*>(t.ancestors + size_t(first + i) * kTreeWords);
+        to[0] = seen[k][0];
+        to[1] = seen[k][1];
     }
 }
 
