@@ -32,7 +32,7 @@ __device__ __forceinline__ bool tree_rows(const int32_t* starts, int b, int toke
 // rounds 2^k nodes are covered: a chain of 256 has 8 rounds (6.0 us; walking up
 // node by node, 255 steps, 65).  A node's depth is the number of its bits, less its
 // own.  Bound by latency, a launch and three dependent reads (one tree of 8
-// nodes 2.1 us, 64 of 60 3.8).
+// nodes 2.5 us, 64 of 60 4.0).
 __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequences, int32_t* status)
 {
     __shared__ uint4v seen_of[kTreeWaves][kTreeNodes][2];
@@ -339,7 +339,7 @@ __device__ __forceinline__ void chain_choices(const AcceptParams& p, const Seque
 // layers' heads).  A block's first wave walks the path; with all four walking
 // for themselves the walks are most of the time.  Bound by latency, four or five
 // dependent reads (one chat 4.2 us, of 36 layers and 8 kv heads), and where many
-// move by rows of 256 bytes that lie apart (32 chats, 12 MB: 8.6 us).
+// move by rows of 256 bytes that lie apart (32 chats, 12 MB: 8.3 to 9.3 us).
 // Of a wave's rows (layer, K or V, kv head) four: 8.6 us, 12.6 with two, 8.6
 // with eight (one chat 5.1), 10.6 with sixteen.
 constexpr int kMoveItems = 4;

@@ -203,7 +203,8 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
     keys/values [layers, pages, kv_heads, page_size, head_dim], move to the
     slots behind the base.  Returns int32 (kept [sequences], path [tokens],
     next [sequences]): the lengths to resize to, the path's nodes in a
-    sequence's first rows (then -1), and the choice at the path's end; a
+    sequence's first rows (then -1), and the choice at the path's end (before a
+    fork, and before growth under a window, resize to kept itself); a
     sequence without nodes, or all while status says that the cache refused to
     grow, have kept -1 (a resize leaves them) and next -1."""
     if status is None or lengths is None:

@@ -347,8 +347,11 @@ int hq_paged_attention_tree(const hq_pages* cache, const float* query, const hq_
  * [tokens, vocab], choices NULL) in hq_argmax's order.  The path's K and V move
  * to slots base, base + 1, .. in every layer of the cache.  Tables and lengths
  * stay: kept (int32 [sequences]) receives base + the path's nodes, for a
- * hq_pages_resize to it (or beyond, to the next trees; where that call has a
- * window, to it first, since the next queries begin there).  path (int32 [tokens]):
+ * hq_pages_resize to it (or beyond, to the next trees; to it first where that
+ * call has a window, since the next queries begin there, and before a
+ * hq_pages_fork, since slots from there on are written again: a growth copies a
+ * shared page from the old length on).  Forks between the nodes' resize and this
+ * call move a shared page's rows for all of its holders.  path (int32 [tokens]):
  * the i-th node of the path at row starts[b] + i, then -1.  next (int32
  * [sequences]): the choice at the path's last node.  A sequence without nodes,
  * with a root of depth -1 or with a negative base (these two set HQ_PAGES_BAD),

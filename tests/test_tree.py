@@ -1460,3 +1460,53 @@ def test_a_server_s_trees(window, sinks):
             at += len(t)
         c.check_status()
     assert max(kept) > 30
+
+
+@gpu
+@pytest.mark.parametrize("base", [0, 5, 16, 27, 31])
+def test_forks_between_trees(base):
+    """A path kept, its sequence forked at its end, and other trees in both: they
+    share what was kept, and neither's nodes or moves reach the other."""
+    from harsh4b_amd.paged import PagedCache
+    kv, groups, d = 2, 4, 16
+    rng = np.random.default_rng(base)
+    c = PagedCache(2, 16, kv, d, sequences=3, max_pages=6, page_size=16)
+    cos, sin = torch.ones((96, d // 2), device="cuda"), torch.zeros((96, d // 2), device="cuda")
+    norm = torch.ones(d, device="cuda")
+
+    def rows_of(b, n):                                 # K and V of both layers at positions 0 .. n - 1
+        table, keys, values = c.table.cpu().numpy(), c.keys.cpu().numpy(), c.values.cpu().numpy()
+        return [np.stack([pool[:, table[b, j // 16], :, j % 16] for j in range(n)]) for pool in (keys, values)]
+
+    def step(bases, trees):
+        c.resize([b + len(t) if t else -1 for b, t in zip(bases, trees)])
+        tree = c.plan_tree(np.concatenate(trees).astype(int).tolist(), starts_of(trees).tolist())
+        tokens = sum(len(t) for t in trees)
+        for layer in range(2):
+            c.append_tree(layer, up(rng.standard_normal((tokens, (groups + 2) * kv * d)).astype(np.float32)), norm, norm,
+                          cos, sin, 1e-6, tree)
+        return tree
+
+    if base:
+        step([0] * 3, [chain(base), [], []])
+    comb = [-1, 0, 0, 2, 2, 4, 4, 6, 6, 8, 8, 10, 10, 12, 12, 14, 14, 16, 16, 18]    # the even nodes are the path
+    tree = step([base] * 3, [comb, [], []])
+    before = rows_of(0, base + len(comb))
+    kept, path, _ = c.accept(tree, [i % 2 for i in range(len(comb))], choices=[0] * len(comb))
+    n = base + 10
+    assert kept.tolist() == [n, -1, -1] and path.tolist()[:11] == list(range(0, 20, 2)) + [-1]
+    c.resize(kept)
+    c.fork([-1, 0, 0])
+    assert c.lengths.tolist() == [n] * 3
+    shared = [np.concatenate([pool[:base], pool[base:][::2]]) for pool in before]
+    tree = step([n] * 3, [chain(7), comb, []])
+    nodes = [rows_of(0, n + 7), rows_of(1, n + len(comb))]
+    kept, _, _ = c.accept(tree, [0] * 7 + [i % 2 for i in range(len(comb))], choices=[0] * (7 + len(comb)))
+    assert kept.tolist() == [n + 7, n + 10, -1]
+    c.resize(kept)
+    expect = [nodes[0], [np.concatenate([pool[:n], pool[n:][::2]]) for pool in nodes[1]], shared]
+    for b, length in enumerate((n + 7, n + 10, n)):
+        for got, want, start in zip(rows_of(b, length), expect[b], shared):
+            np.testing.assert_array_equal(got, want)
+            np.testing.assert_array_equal(got[:n], start)
+    c.check_status()
