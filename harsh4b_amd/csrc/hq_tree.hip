@@ -262,14 +262,25 @@ __device__ Best row_part_best(const float* row, int vocab, int part, int splits,
 // the chain's levels that the block takes, every slots-th).  A block's first
 // wave works the chain out, from three round trips: the sequence's numbers, its
 // nodes', and the nodes' logits at their parents, which lie scattered over the
-// rows.  Then the rows are bound by HBM: 32 chats' chains of 138 rows of 151936
-// (84 MB, 17.8 us at the rate of a copy) in 26 us; every row of the batch takes
-// 124, and a launch for each level would be seven.  A block that takes the levels
-// one after another (no slots) 45: the longest chain sets the time.
+// rows; the root is known without, so its row is on its way meanwhile (24.7 us
+// for the below, 26.6 if it waits too).  Then the rows are bound by HBM: 32
+// chats' chains of 138 rows of 151936 (84 MB, 17.8 us at the rate of a copy);
+// every row of the batch takes 124, and a launch for each level would be seven.
+// A block that takes the levels one after another (no slots) 45: the longest
+// chain sets the time.
 __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
 {
     __shared__ Best red[kTreeWaves];
     __shared__ int node[kTreeNodes], nodes, first;
+    if (blockIdx.z == 0) {
+        int root, rows;
+        tree_rows(p.t.starts, blockIdx.x, p.t.tokens, &root, &rows);
+        if (rows == 0) return;
+        const size_t at = __builtin_amdgcn_readfirstlane(root);
+        const Best x = row_part_best(p.logits + at * p.vocab, p.vocab, blockIdx.y, p.splits, red);
+        if (threadIdx.x == 0) p.best[at * p.splits + blockIdx.y] = x;
+        if (p.levels <= p.slots) return;
+    }
     if (threadIdx.x < kWave) {
         const int lane = threadIdx.x;
         int taken = 0;
@@ -287,7 +298,7 @@ __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
             if (lane == 0) first = s.first;
             int u = 0;
             for (int level = 0; u >= 0 && level < p.levels; ++level) {
-                if (level % p.slots == int(blockIdx.z)) {
+                if (level && level % p.slots == int(blockIdx.z)) {
                     if (lane == 0) node[taken] = u;
                     ++taken;
                 }
@@ -308,7 +319,8 @@ __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
     for (int k = 0; k < taken; ++k) {
         const float* row = p.logits + (from + __builtin_amdgcn_readfirstlane(node[k])) * p.vocab;
         const Best x = row_part_best(row, p.vocab, blockIdx.y, p.splits, red);
-        if (threadIdx.x == 0) p.best[(from + blockIdx.z + size_t(k) * p.slots) * p.splits + blockIdx.y] = x;
+        const size_t level = blockIdx.z + size_t(k + (blockIdx.z == 0)) * p.slots;
+        if (threadIdx.x == 0) p.best[(from + level) * p.splits + blockIdx.y] = x;
     }
 }
 
@@ -442,7 +454,7 @@ struct AcceptPlan {
 };
 
 // Blocks aimed at for the rows of the chains' levels, many of which no chain
-// reaches (32 chats of 16 nodes: 26 us, 28 with 512, 30 with 2048).
+// reaches (32 chats of 16 nodes, the root's too waiting: 26 us, 28 with 512, 30 with 2048).
 constexpr int kChainBlocks = 1024;
 
 static AcceptPlan accept_plan(int tokens, int sequences, int vocab, int levels)
