@@ -178,7 +178,8 @@ struct Sequence {
         bad = !tree_rows(p.t.starts, b, p.t.tokens, &first, &rows);
         first = __builtin_amdgcn_readfirstlane(first);
         rows = __builtin_amdgcn_readfirstlane(rows);
-        base = __builtin_amdgcn_readfirstlane(length) - rows;
+        // (a length near -2^31: in 32 bits the difference would wrap round to a slot past any table)
+        base = int(max(int64_t(__builtin_amdgcn_readfirstlane(length)) - rows, int64_t(-1)));
         n = 0;
         if (rows == 0) return;
 #pragma unroll

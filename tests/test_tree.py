@@ -1510,3 +1510,30 @@ def test_forks_between_trees(base):
             np.testing.assert_array_equal(got, want)
             np.testing.assert_array_equal(got[:n], start)
     c.check_status()
+
+
+# ------------------------------------------------------------------ accept: lengths, plans and vocabularies that do not fit
+@gpu
+@pytest.mark.parametrize("by", ["choices", "logits"])
+@pytest.mark.parametrize("length", [-2**31, -2**31 + 5, -2**31 + 9, -5, -1, 0, 9])
+def test_accept_of_lengths_below_the_tree(length, by):
+    # a base before the sequence, at the lowest lengths too: it takes no part, and the others do
+    from harsh4b_amd.tree import pages_accept
+    trees, bases = [chain(6), star(10), chain(4)], [20, 30, 5]
+    table, lengths, keys, values = _cache_of(trees, bases, d=64)
+    n = sum(len(t) for t in trees)
+    drafted, choices = [1] * n, [1] * n
+    drafted[6 + 1:6 + 9] = [0] * 8                      # (the star's last child: a row that would move)
+    ek, ev, kept, path, after = _expect_accept([trees[0], [], trees[2]], bases, table, keys, values,
+                                               drafted[:6] + drafted[16:], choices[:6] + choices[16:])
+    lengths[1] = length
+    how = dict(choices=ints(choices))
+    if by == "logits":
+        how = dict(logits=torch.zeros((n, 40), device="cuda"))
+        how["logits"][:, 1] = 1.0
+    status, dk, dv, size = ints([0]), up(keys), up(values), ints(lengths)
+    got = pages_accept(dk, dv, ints(table), size, status, plan(trees), ints(drafted), **how)
+    assert [g.tolist() for g in got] == [kept, path[:6] + [-1] * 10 + path[6:], after]
+    assert int(status.item()) == 2 and size.tolist() == lengths
+    np.testing.assert_array_equal(dk.cpu().numpy(), ek)
+    np.testing.assert_array_equal(dv.cpu().numpy(), ev)
