@@ -326,10 +326,12 @@ __global__ __launch_bounds__(kBlock) void accept_chain_kernel(AcceptParams p)
 }
 
 // The choices at the levels of a sequence's chain, into LDS, by a wave: splits
-// lanes (a power of two) a level, 64 / splits levels at a time.  What lies past
-// the chain's end is of any contents, and the walk, which ends there, does not
-// come to it.
-__device__ __forceinline__ void chain_choices(const AcceptParams& p, const Sequence& s, int* level_choice)
+// lanes (a power of two) a level, 64 / splits levels at a time.  Returns the
+// levels that it has: those of the plan's depths, which the walk may not leave
+// (a chain follows the parents, and goes on past them where the plan was made
+// of others).  What lies past the chain's end is of any contents, and the walk,
+// which ends there, does not come to it.
+__device__ __forceinline__ int chain_choices(const AcceptParams& p, const Sequence& s, int* level_choice)
 {
     const int lane = threadIdx.x & (kWave - 1);
     const int part = lane & (p.splits - 1), each = kWave / p.splits;
@@ -337,7 +339,7 @@ __device__ __forceinline__ void chain_choices(const AcceptParams& p, const Seque
 #pragma unroll
     for (int k = 0; k < kTreeLanes; ++k) deepest = max(deepest, s.depth[k]);
     deepest = -wave_imin64_all(-deepest);
-    const int levels = min(min(p.levels, s.n), deepest + 1);
+    const int levels = min(min(p.levels, s.n), min(deepest, kTreeNodes - 1) + 1);
     for (int from = 0; from < levels; from += each) {
         const int level = from + lane / p.splits;
         Best x = p.best[size_t(s.first + min(level, levels - 1)) * p.splits + part];
@@ -346,6 +348,7 @@ __device__ __forceinline__ void chain_choices(const AcceptParams& p, const Seque
         if (level < levels && part == 0) level_choice[level] = x.i;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    return levels;
 }
 
 // The path, and its K and V to their slots: blocks (sequence, slice of the
@@ -376,8 +379,9 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
         }
         int count = 0, choice = -1;
         if (s.settle()) {
-            if (p.logits) chain_choices(p, s, level_choice);
-            for (int u = 0; u >= 0; u = count < p.levels ? s.child(u, choice) : -1) {
+            const int levels = p.logits ? chain_choices(p, s, level_choice) : p.levels;
+            int u = 0;
+            for (; u >= 0 && count < levels; u = count < p.levels ? s.child(u, choice) : -1) {
                 if (lane == 0) path[count] = u;
                 if (p.logits) {
                     choice = __builtin_amdgcn_readfirstlane(level_choice[count]);
@@ -388,6 +392,7 @@ __global__ __launch_bounds__(kBlock) void accept_move_kernel(AcceptParams p)
                 }
                 ++count;
             }
+            s.bad = u >= 0;                    // (the path goes on where the plan has no level)
         }
         if (lane == 0) {
             shared_count = count;

@@ -357,7 +357,9 @@ int hq_paged_attention_tree(const hq_pages* cache, const float* query, const hq_
  * with a root of depth -1 or with a negative base (these two set HQ_PAGES_BAD),
  * and all of them while status has HQ_PAGES_FULL or HQ_PAGES_REFUSED set, get
  * kept -1, next -1 and a path of -1; nothing moves.  A row that would move from
- * or to a slot without a page stays and sets HQ_PAGES_BAD.  Rows of no sequence
+ * or to a slot without a page stays and sets HQ_PAGES_BAD.  Where the depths are
+ * not those of `parents` (a plan of other trees), a path by logits ends at the
+ * deepest of them, and sets HQ_PAGES_BAD if it would go on.  Rows of no sequence
  * are not touched; the logits of rows off the path may be read or not.  The
  * outputs overlap no input.  `workspace`: hq_pages_accept_workspace_bytes(...) bytes (vocab 0: the
  * choices are given), 256-byte aligned, of any contents. */

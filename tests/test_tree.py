@@ -1537,3 +1537,40 @@ def test_accept_of_lengths_below_the_tree(length, by):
     assert int(status.item()) == 2 and size.tolist() == lengths
     np.testing.assert_array_equal(dk.cpu().numpy(), ek)
     np.testing.assert_array_equal(dv.cpu().numpy(), ev)
+
+
+@gpu
+@pytest.mark.parametrize("what", ["zeros", "short", "largest", "random"])
+def test_accept_of_depths_that_are_not_the_trees(what):
+    # a plan of other trees: by logits the path ends at its deepest level and says so, choices do not look at depths;
+    # two runs agree, and the other sequences have their paths
+    from harsh4b_amd.tree import pages_accept
+    trees, bases = [chain(9), chain(40), random_tree(np.random.default_rng(5), 30, 6)], [20, 3, 50]
+    n, at = sum(len(t) for t in trees), slice(9, 49)
+    drafted, choices = [7] * n, [7] * n
+    table, lengths, keys, values = _cache_of(trees, bases)
+    logits = torch.zeros((n, 5000), device="cuda")
+    logits[:, 7] = 1.0
+    t = plan(trees)
+    rng = np.random.default_rng(8)
+    for _ in range(3):
+        depths = t.depths.clone()
+        false = {"zeros": np.zeros(40), "short": np.minimum(np.arange(40), 11), "largest": np.full(40, 2**31 - 1),
+                 "random": rng.integers(-2**31, 2**31, 40)}[what].astype(np.int64)
+        false[0] = abs(false[0]) % 2**31
+        depths[at] = ints(false)
+        levels = min(40, int(max(0, false.max())) + 1)
+        for how, expect in ((dict(logits=logits), levels), (dict(choices=ints(choices)), 40)):
+            runs = []
+            for _ in range(2):
+                status, dk = ints([0]), up(keys)
+                got = pages_accept(dk, up(values), ints(table), ints(lengths), status, t._replace(depths=depths),
+                                   ints(drafted), **how)
+                runs.append([g.tolist() for g in got] + [int(status.item())])
+            assert runs[0] == runs[1]
+            kept, path, after, code = runs[0]
+            assert path[at] == list(range(expect)) + [-1] * (40 - expect) and code == (0 if expect == 40 else 2)
+            assert kept[1] == 3 + expect and after == [7, 7, 7]
+            for b, rows in ((0, slice(0, 9)), (2, slice(49, n))):
+                p, _ = walk(trees[b], drafted[rows], choices[rows])
+                assert path[rows] == p + [-1] * (len(trees[b]) - len(p)) and kept[b] == bases[b] + len(p)
