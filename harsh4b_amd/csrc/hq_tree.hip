@@ -26,6 +26,16 @@ __device__ __forceinline__ bool tree_rows(const int32_t* starts, int b, int toke
     return !bad;
 }
 
+// What the lanes of a wave wrote to LDS before is what they read after: a wave's
+// LDS accesses take effect in their order, and the fences keep the compiler from
+// another one (no instruction; to it the lanes' addresses may well be apart).
+__device__ __forceinline__ void wave_lds_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // -------------------------------------------------------------------- plan
 // A wave a sequence.  Each node holds the bits of the nodes up to some above it
 // and which one comes next; a round takes over that one's, so that after k
@@ -81,7 +91,7 @@ __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequen
             more |= next[k] >= 0;
         });
         if (!__any(more)) break;
-        // (a wave's LDS accesses take effect in their order: all of a round's reads come before the next one's writes)
+        wave_lds_order();
         unrolled<kTreeLanes>([&](auto lanes) {
             constexpr int k = decltype(lanes)::value;
             if (k * kWave >= n || next[k] < 0) return;
@@ -89,6 +99,7 @@ __global__ __launch_bounds__(kBlock) void tree_plan_kernel(hq_tree t, int sequen
             seen[k][1] |= seen_of[wave][next[k]][1];
             next[k] = next_of[wave][next[k]];
         });
+        wave_lds_order();                      // (all of a round's reads come before the next one's writes)
     }
 #pragma unroll
     for (int k = 0; k < kTreeLanes; ++k) {
