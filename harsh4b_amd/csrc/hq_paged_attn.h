@@ -1556,18 +1556,20 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 
 // The join of a tree's batch of many rows (a token's heads of one kv head), whose
 // parts are few: quads of a multiple of 64 threads, so that a wave has one row,
-// as many rows a block as fit, and no exchange between threads.  382 tokens of
-// 32 heads in 2 parts: 6.4 us, 9.1 by paged_join_kernel; 96 in 16 parts 10.3
-// and 9.1: where rows are few, their parts are many.
+// as many rows a block as fit, and no exchange between threads (6 heads of 128
+// are 192 threads: one row, and a wave left over).  382 tokens of 32 heads in 2
+// parts: 6.4 us, 9.1 by paged_join_kernel; 96 in 16 parts 10.3 and 9.1: where
+// rows are few, their parts are many.
 constexpr int kJoinRows = 2048;
 
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(PagedAttnParams p)
 {
     const int cut = *p.cut;
-    const int quads = p.b.groups * D / 4;                 // 64, 128 or 256
+    const int quads = p.b.groups * D / 4;                 // 64, 128, 192 or 256
     const int slots = kJoinThreads / quads;
     const int slot = uniform(threadIdx.x / unsigned(quads)), quad = threadIdx.x - slot * quads;
+    if (slot >= slots) return;                            // (left over: the row after is another block's)
     const int r = quad / (D / 4), at = quad % (D / 4);
     const unsigned all = unsigned(p.b.tokens) * unsigned(p.b.kv_heads);
     for (unsigned i = blockIdx.x * slots + slot; i < all; i += gridDim.x * slots) {

@@ -1574,3 +1574,16 @@ def test_accept_of_depths_that_are_not_the_trees(what):
             for b, rows in ((0, slice(0, 9)), (2, slice(49, n))):
                 p, _ = walk(trees[b], drafted[rows], choices[rows])
                 assert path[rows] == p + [-1] * (len(trees[b]) - len(p)) and kept[b] == bases[b] + len(p)
+
+
+# ------------------------------------------------------------------ joins and plans of mixed batches
+@gpu
+@pytest.mark.parametrize("kv,groups,d", [(8, 6, 128), (8, 8, 128), (8, 5, 128), (4, 6, 64)])
+def test_joins_of_rows_of_other_widths(kv, groups, d):
+    # 192 and 256 threads a row (a wave left over, none); rows that are no whole waves
+    rng = np.random.default_rng(groups * d)
+    sizes = [int(n) for n in rng.integers(17, 27, 26)]
+    s = Trees(some_trees(d, sizes), [int(b) for b in rng.integers(300, 1500, 26)], kv, groups, d, 64, seed=d)
+    assert s.tokens * kv >= 2048
+    s._check()
+    s._check(window=700, sinks=3)
