@@ -476,6 +476,8 @@ constexpr int kChainBlocks = 1024;
 // Parts of a row at most: the rows of one chat of 16 nodes take 6.8 us (6.1 with
 // up to 64 parts), and the move, each of whose blocks joins them, 6.3 (12.5).
 constexpr int kMostParts = 16;
+// Values of a row of logits: the places of its last block's threads, up to 255 past its end, are ints.
+constexpr int kMostVocab = 1 << 30;
 
 static AcceptPlan accept_plan(int tokens, int sequences, int vocab, int levels)
 {
@@ -516,7 +518,7 @@ extern "C" int hq_tree_plan(const hq_tree* tree, int sequences, int32_t* status,
 
 extern "C" size_t hq_pages_accept_workspace_bytes(int tokens, int sequences, int vocab, int levels)
 {
-    if (tokens < 0 || sequences < 1 || vocab < 0 || levels < 1 || levels > kTreeNodes) return 0;
+    if (tokens < 0 || sequences < 1 || vocab < 0 || vocab > kMostVocab || levels < 1 || levels > kTreeNodes) return 0;
     return std::max<size_t>(256, accept_plan(tokens, sequences, vocab, levels).bytes);
 }
 
@@ -533,7 +535,7 @@ extern "C" int hq_pages_accept(const hq_pages* cache, const hq_tree* tree, const
     if (cache->layers < 1 || !cache->status || !kept || !next || !workspace || levels < 1 || levels > kTreeNodes)
         return HQ_ERR_ARG;
     if (tree->tokens && (!drafted || !path || !choices == !logits)) return HQ_ERR_ARG;
-    if (logits ? vocab < 1 : vocab != 0) return HQ_ERR_ARG;
+    if (logits ? vocab < 1 || vocab > kMostVocab : vocab != 0) return HQ_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return HQ_ERR_ALIGN;
     for (const void* q : {static_cast<const void*>(drafted), static_cast<const void*>(choices),
                           static_cast<const void*>(logits), static_cast<const void*>(kept),

@@ -32,6 +32,7 @@ from .paged import MAX_GROUPS, _F32, _I32, _apart, _cache, _index, _launch, _ref
 
 MAX_NODES = _native.HQ_TREE_NODES
 ANCESTOR_WORDS = MAX_NODES // 32
+MAX_VOCAB = 1 << 30
 
 _pack = struct.Struct("2i4P").pack
 
@@ -226,6 +227,8 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
                 logits.get_device() != index or not logits.is_contiguous()):
             _refuse("logits", logits, _F32, index, "[tokens, vocab]")
         vocab = logits.shape[1]
+        if vocab > MAX_VOCAB:
+            raise ValueError("logits must have a vocabulary of at most 2^30")
         chosen, rows = None, logits.data_ptr()
     else:
         chosen, rows = _nodes(choices, "choices", tokens, index), None

@@ -344,7 +344,7 @@ int hq_paged_attention_tree(const hq_pages* cache, const float* query, const hq_
  * drafted token (int32 [tokens]) is the choice at its parent (the first of equal
  * ones), and so on, at most `levels` nodes with the root (1 .. HQ_TREE_NODES).  The
  * choices are given (int32 [tokens], logits NULL) or the argmax of logits (fp32
- * [tokens, vocab], choices NULL) in hq_argmax's order.  The path's K and V move
+ * [tokens, vocab], vocab at most 2^30, choices NULL) in hq_argmax's order.  The path's K and V move
  * to slots base, base + 1, .. in every layer of the cache.  Tables and lengths
  * stay: kept (int32 [sequences]) receives base + the path's nodes, for a
  * hq_pages_resize to it (or beyond, to the next trees; to it first where that

@@ -1587,3 +1587,25 @@ def test_joins_of_rows_of_other_widths(kv, groups, d):
     assert s.tokens * kv >= 2048
     s._check()
     s._check(window=700, sinks=3)
+
+
+# ------------------------------------------------------------------ vocabularies past what the kernels count
+def test_accept_refuses_vocabularies_past_2_30():
+    lib = native().lib()
+    c, p, _ = _struct()
+    t = ctypes.byref(_tree_struct(p))
+    for vocab in ((1 << 30) + 1, (1 << 31) - 256, (1 << 31) - 1):
+        assert lib.hq_pages_accept(ctypes.byref(c), t, p, None, p, vocab, 4, p, p, p, p, None) == 1
+        assert lib.hq_pages_accept_workspace_bytes(3, 1, vocab, 4) == 0
+    assert lib.hq_pages_accept_workspace_bytes(3, 1, 1 << 30, 4) > 0
+
+
+@gpu
+def test_python_refuses_vocabularies_past_2_30():
+    from harsh4b_amd.tree import DraftTree, pages_accept
+    table, lengths, keys, values = _cache_of([[-1]], [3])
+    none = DraftTree(ints([]), ints([0, 0]), ints([]), ints(np.zeros((0, 8))))
+    for vocab in ((1 << 30) + 1, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="vocabulary"):
+            pages_accept(up(keys), up(values), ints(table), ints(lengths), ints([0]), none, ints([]),
+                         logits=torch.zeros((0, vocab), device="cuda"))
