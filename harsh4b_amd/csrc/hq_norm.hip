@@ -18,8 +18,11 @@ struct NormParams {
     float eps;
 };
 
-// Longer rows: a block a row, which is read three times (the second and third
-// from the caches).
+// Longer rows: a block a row, which is read three times, a value a thread at a
+// time (the second and third from the caches).  Bound by the latency of its 3 n
+// / 256 reads one after another where rows are few (8 rows of 12288 29 us, of
+// 16384 40), and by the same beside HBM where they are many (2048 of 12288 111
+// us, 3.0 TB/s, of 16384 154; 2048 of 10240 in registers 44, 6.2 TB/s).
 __global__ __launch_bounds__(kBlock) void norm_quant_long_kernel(NormParams p)
 {
     __shared__ float red[kBlock];

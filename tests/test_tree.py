@@ -1609,3 +1609,32 @@ def test_python_refuses_vocabularies_past_2_30():
         with pytest.raises(ValueError, match="vocabulary"):
             pages_accept(up(keys), up(values), ints(table), ints(lengths), ints([0]), none, ints([]),
                          logits=torch.zeros((0, vocab), device="cuda"))
+
+
+# ------------------------------------------------------------------ rows longer than a block holds in registers
+@gpu
+@pytest.mark.parametrize("n", [10240, 10241, 12001, 20001])
+def test_long_rows_that_are_not_finite(n):
+    # as test_rows_that_are_not_finite, in place and beside the input: the single row calls' bits, row by row
+    from harsh4b_amd.lightspark import add_rmsnorm_quant, quantize_activation, rmsnorm
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((9, n)).astype(np.float32)
+    x[1] = 0
+    x[2, n - 1] = np.inf
+    x[3, 7] = np.nan
+    x[4] *= np.float32(1e30)
+    x[5] *= np.float32(1e-30)
+    x[6, n - 257] = -np.inf
+    x[7] = np.finfo(np.float32).max
+    x[8, 300], x[8, n - 1] = np.inf, -np.inf
+    gamma, delta = rng.uniform(0.5, 1.5, n).astype(np.float32), rng.standard_normal((9, n)).astype(np.float32)
+    delta[1] = 0
+    dg, total = up(gamma), up(x) + up(delta)
+    for out in (None, torch.empty((9, n), device="cuda")):
+        dx = up(x)
+        q, s = add_rmsnorm_quant(dx, dg, 1e-6, delta=up(delta), out=out)
+        assert (dx if out is None else out).cpu().numpy().tobytes() == total.cpu().numpy().tobytes()
+        for i in range(9):
+            eq, es = quantize_activation(rmsnorm(total[i].contiguous(), dg, 1e-6))
+            assert torch.equal(q[i], eq), i
+            assert s[i].cpu().numpy().tobytes() == es[0].cpu().numpy().tobytes() or (s[i].isnan() and es[0].isnan()), i
