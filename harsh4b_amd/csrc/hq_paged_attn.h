@@ -521,7 +521,12 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
     // at the end: larger ones that all have a place, if up to twice the size
     // gives such (800 tokens after 8200: 233 us, 273 without; 400 after 4600
     // 84, 108; 700 after 800 56, 63).  Of up to 64 sequences, whose plans the
-    // lanes hold; more would be worked out anew for every size tried.
+    // lanes hold; more would be worked out anew for every size tried.  Where no
+    // such size gives it (one long sequence among short ones that take most of
+    // the places), the first stays, and the launch has the blocks: trees of 16
+    // nodes on 46 chats of 300 and one of 40960 take 82 us so, 104 with sizes up
+    // to four times the first and 1172 uncut (of 8 nodes 74, 70 and 564; 62 of
+    // 3000 and one of 40960 207, 377 and 640).
     if (p.b.sequences <= kWave && !p.whole && int64_t(tiles) * p.b.kv_heads <= kTarget) {
         int larger = target;
         bool fits = false;
@@ -530,7 +535,6 @@ __device__ __forceinline__ bool plan_piece(const PagedAttnParams& p, int q, Piec
             if (fits) target = larger;
             else larger += larger / 8 + 1;
         }
-        if (TREE && !fits) target = 0x40000000;              // (no cuts: the launch has kTarget blocks)
     }
     int pieces = 0, rows = 0;
     bool got = false;
@@ -1559,7 +1563,9 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnParam
 // as many rows a block as fit, and no exchange between threads (6 heads of 128
 // are 192 threads: one row, and a wave left over).  382 tokens of 32 heads in 2
 // parts: 6.4 us, 9.1 by paged_join_kernel; 96 in 16 parts 10.3 and 9.1: where
-// rows are few, their parts are many.
+// rows are few, their parts are many.  Where both are (46 chats of 300 positions
+// in one part, one of 40960 in 46, trees of 16 nodes) the call takes 83 us, 79 by
+// paged_join_kernel.
 constexpr int kJoinRows = 2048;
 
 template <int D>
@@ -1701,10 +1707,8 @@ int run_attention(PagedAttnParams& p, const hq_pages* cache, const float* query,
                                    : std::min(tokens, p.b.sequences);
     const int64_t widest = (int64_t(cache->max_pages) * cache->page_size + kChunkKeys - 1) / kChunkKeys;
     p.whole = widest <= kWholeChunks;
-    // (of a tree's batch whose tiles all have a place, their pieces have one too: see plan_piece)
-    const bool placed = TREE && cache->sequences <= kWave && tiles * p.b.kv_heads <= kTarget;
     const int64_t blocks = p.whole ? tiles * p.b.kv_heads
-                                   : std::min(kTarget + (placed ? 0 : tiles * p.b.kv_heads),
+                                   : std::min(kTarget + tiles * p.b.kv_heads,
                                               tiles * p.b.kv_heads * ((widest + kSmallMin - 1) / kSmallMin));
     p.planned = cache->sequences >= kPlanSequences && !(p.whole && !starts);
     if (blocks > kMaxBlocks || int64_t(tokens) * p.b.kv_heads > 0x7fffffff) return HQ_ERR_ARG;

@@ -1638,3 +1638,69 @@ def test_long_rows_that_are_not_finite(n):
             eq, es = quantize_activation(rmsnorm(total[i].contiguous(), dg, 1e-6))
             assert torch.equal(q[i], eq), i
             assert s[i].cpu().numpy().tobytes() == es[0].cpu().numpy().tobytes() or (s[i].isnan() and es[0].isnan()), i
+
+
+# ------------------------------------------------------------------ pieces of batches of long and short chats
+def _pieces(s, groups):
+    """Pieces of each sequence's first tile, as the attention leaves them in its workspace: behind the plan (256 bytes,
+    tokens + 1 ints and tokens times four, each up to 256 bytes) a row's and kv head's 2 * pieces + small, first part."""
+    from harsh4b_amd import paged, tree
+    lib = native().lib()
+    d, t = s.device(), plan(s.trees)
+    kv, dim = s.keys.shape[1], s.keys.shape[3]
+    size = lib.hq_paged_attention_tree_workspace_bytes(s.tokens, kv * groups, kv, dim)
+    workspace = torch.zeros(size + 256, dtype=torch.uint8, device="cuda")
+    at = -workspace.data_ptr() % 256
+    index = d["keys"].get_device()
+    cache, sequences, _, _ = paged._cache(index, d["keys"], d["values"], d["table"], d["lengths"], None, None, 4)
+    out = torch.empty_like(d["query"])
+    code = lib.hq_paged_attention_tree(cache, d["query"].data_ptr(), tree._tree(t, s.tokens, sequences, index), kv * groups,
+                                       0, 0, out.data_ptr(), workspace.data_ptr() + at, torch.cuda.current_stream().cuda_stream)
+    assert code == 0
+    torch.cuda.synchronize()
+    up256 = lambda n: (n + 255) // 256 * 256
+    at += 256 + up256(4 * (s.tokens + 1)) + up256(16 * s.tokens)
+    desc = workspace[at:at + 8 * s.tokens * kv].cpu().numpy().view(np.int32).reshape(s.tokens, kv, 2)
+    return [int(desc[first, 0, 0]) >> 1 for first in s.starts[:-1]], out.cpu().numpy()
+
+
+def _check_pieces(s, groups):
+    """No piece has more than a small multiple of the chunks that the batch's work gives each of 512 places: sizes go up
+    to 2.04 times those (at least 4; tiles of 16 rows, at most 256 of 8 chunks, add 4), and a sequence of less than 3/2
+    sizes is one piece, as are large tiles of up to 16 chunks."""
+    pieces, out = _pieces(s, groups)
+    kv, dim = s.keys.shape[1], s.keys.shape[3]
+    chunks = [-(-n // 64) for n in s.lengths]
+    tiles = [1 if len(t) * groups <= 32 else -(-len(t) // (128 // groups)) for t in s.trees]
+    target = -(-sum(c * t for c, t in zip(chunks, tiles)) * kv // 512)
+    longest = max(-(-c // p) for c, p in zip(chunks, pieces))
+    assert longest <= max(16, 3.1 * (target + 4) + 2), (longest, target)
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("bases,nodes,kv,groups", [([300] * 59 + [20000], 8, 8, 4), ([300] * 46 + [40960], 16, 8, 2),
+                                                   ([40000] + [300] * 10, 16, 32, 1), ([3000] * 31 + [30000] + [3000] * 30, 5, 8, 3),
+                                                   ([500] * 56 + [16384], 16, 8, 4)])
+def test_one_long_chat_among_short_ones(bases, nodes, kv, groups):
+    # the long one is cut, though the short ones take most places, and the results are the definition's
+    rng = np.random.default_rng(nodes + kv)
+    s = Trees([random_tree(rng, nodes) for _ in bases], bases, kv, groups, 16, 64, seed=kv)
+    out = _check_pieces(s, groups)
+    expect, bound = _reference(s, s.trees, 0, 0)
+    off = np.abs(out - expect).reshape(s.tokens, -1).max(axis=1)
+    assert (off <= bound).all(), (off.max(), bound[np.argmax(off - bound)])
+
+
+@gpu
+def test_pieces_of_drawn_batches():
+    rng = np.random.default_rng(77)
+    for i in range(40):
+        kv, groups = [(8, 4), (8, 1), (16, 2), (32, 1), (4, 8), (2, 6)][i % 6]
+        count = int(rng.integers(2, 65))
+        bases = [int(np.exp(rng.uniform(np.log(20), np.log(rng.choice([400, 4000]))))) for _ in range(count)]
+        for b in rng.integers(0, count, rng.integers(1, 4)):
+            bases[b] = int(rng.integers(8000, 24000))
+        trees = [random_tree(rng, int(n)) for n in rng.integers(1, rng.choice([8, 40]), count)]
+        print(f"[gpu] drawn {i}: {count} sequences, {kv} kv heads of {groups}", flush=True)
+        _check_pieces(Trees(trees, bases, kv, groups, 16, 64, seed=i), groups)
