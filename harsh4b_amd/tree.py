@@ -198,7 +198,8 @@ def pages_accept(keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, 
     """Keep the path that the model's choices follow (hq_pages_accept): from
     each sequence's root the child whose drafted token (int32 [tokens]) is the
     choice at its parent, and so on, at most `levels` nodes (a tree's depth + 1
-    where the caller knows it: fewer launches).  The choices are given (int32
+    where the caller knows it: by logits fewer blocks, of which up to 16 levels
+    side by side have some each).  The choices are given (int32
     [tokens], e.g. a sampler's), or the largest of `logits` (float32 [tokens,
     vocab], ties to the lowest index).  The path's K and V, in every layer of
     keys/values [layers, pages, kv_heads, page_size, head_dim], move to the
